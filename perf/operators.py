@@ -171,7 +171,7 @@ def _wide(x):
 
 def _act(name, z):
     if name == "relu":
-        return torch.where(z > 0, z, torch.zeros_like(z))
+        return torch.where(z < 0, torch.zeros_like(z), z)
     if name == "gelu":
         return 0.5 * z * (1 + torch.erf(z * math.sqrt(0.5)))
     if name == "gelu_tanh":
