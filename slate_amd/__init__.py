@@ -14,7 +14,7 @@ __version__ = "2026.10.0"
 
 from . import _native  # noqa: F401  (loads _host, tries _hip)
 from .core.enums import (  # noqa: F401
-    AllDevices, AnyDevice, Diag, Direction, Equed, GridOrder, HostNum, Job, Layout, LayoutConvert,
+    Activation, AllDevices, AnyDevice, Diag, Direction, Equed, GridOrder, HostNum, Job, Layout, LayoutConvert,
     MethodCholQR, MethodEig, MethodGels, MethodGemm, MethodHemm, MethodLU, MethodSVD, MethodTrsm,
     MOSI, Norm, NormScope, Op, Option, Side, Target, TileKind, Uplo)
 from .core.exceptions import (  # noqa: F401
@@ -36,6 +36,8 @@ from .utils.watchdog import Watchdog  # noqa: F401
 from .models.blas3 import (  # noqa: F401
     gemm, hemm, her2k, herk, multiply, rank_2k_update, rank_k_update, symm, syr2k, syrk,
     triangular_multiply, triangular_solve, trmm, trsm)
+from .models.ffn import (  # noqa: F401
+    clip_norm, gemm_bias_act, gemm_bias_act_grad, gemm_gated, gemm_gated_grad, global_norm)
 from .models.chol import posv, potrf, potri, potrs  # noqa: F401
 from .models.aux import (  # noqa: F401
     add, allgather_dense, colNorms, copy, copy_conj_transpose, from_dense, gather, norm, redistribute, scale,

@@ -137,7 +137,7 @@ def build(verbose=False, hip=True, host=True):
         # same kernel objects (minus the pybind11 units) + the C++ host
         # runtime / drivers of csrc/native, linked against HIP and RCCL only
         kobjs = [o for o in sorted(glob.glob(os.path.join(BUILD, "_hip", "*.hip.o")))
-                 if os.path.basename(o) not in ("bindings.hip.o", "devpool.hip.o")]
+                 if os.path.basename(o) not in ("bindings.hip.o", "bindings_ffn.hip.o", "devpool.hip.o")]
         out.append(_build_module(
             "libslate_amd_native", os.path.join(HERE, "csrc", "native"), [".hip"], hipcc,
             HIPFLAGS + ["-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(ROCM, "include")],

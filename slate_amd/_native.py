@@ -72,6 +72,15 @@ def code(dtype) -> str:
         raise TypeError(f"unsupported dtype {dtype}") from None
 
 
+# element types of the fused products (models/ffn.py) and of copies
+REAL_CODE = {torch.bfloat16: 'b', torch.float16: 'h', torch.float32: 's', torch.float64: 'd'}
+
+
+def raw_stream(t: torch.Tensor) -> int:
+    """The current stream of t's own device (0 for host tensors)."""
+    return torch.cuda.current_stream(t.device).cuda_stream if t.is_cuda else 0
+
+
 def hip_available() -> bool:
     return _hip is not None and torch.cuda.is_available()
 

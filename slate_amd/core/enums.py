@@ -205,6 +205,15 @@ class Norm(_CharEnum):
     Max = 'M'
 
 
+class Activation(_CharEnum):
+    """Elementwise function in the epilogue of `gemm_bias_act` / `gemm_gated`."""
+    Identity = 'I'
+    Relu = 'R'
+    Gelu = 'G'              # z Phi(z), Phi the normal distribution (erf)
+    Gelu_tanh = 'T'         # z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2
+    Silu = 'S'              # z / (1 + exp(-z))
+
+
 class Job(_CharEnum):
     NoVec = 'N'
     Vec = 'V'

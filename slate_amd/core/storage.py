@@ -114,6 +114,8 @@ class MatrixStorage:
         self.local = {}            # slot -> contiguous local buffer (block-cyclic case)
         self.origin_slot = None
         self.lock = threading.RLock()
+        self._valid = {}           # slot -> table version at which prepare_local found it whole
+        self._marked = None        # (slot, table version) after the last mark_local_modified
         self.pools = {}
         self.pool_chunks = {}
         self.pool_blocks = {}      # (i, j, slot) -> (chunk, idx)
@@ -368,7 +370,10 @@ class MatrixStorage:
     def mark_local_modified(self, slot):
         """After a whole-local-buffer kernel wrote `slot` (the post-condition
         of every driver: with SLATE_AMD_DEBUG=1 the MOSI checker runs here)."""
+        if self._marked == (slot, self.table.version()):
+            return                     # nothing changed a state since
         self.table.mark_all(slot, _host.MOSI_Modified)
+        self._marked = (slot, self.table.version())
         from ..utils.debug import Debug
         if Debug.enabled():
             Debug.assert_mosi(self, "mark_local_modified")
@@ -377,6 +382,8 @@ class MatrixStorage:
         """Make the contiguous local buffer valid in `slot` and return it."""
         bc = self.bc
         slate_assert(bc is not None, "prepare_local requires block-cyclic storage")
+        if self._valid.get(slot) == self.table.version() and slot in self.local:
+            return self.local[slot]    # no tile state changed since it was found whole
         with self.lock:
             if self.origin_slot is None:
                 self.allocate_local(slot)
@@ -407,6 +414,7 @@ class MatrixStorage:
             from ..utils.debug import Debug
             if Debug.enabled():
                 Debug.assert_mosi(self, "prepare_local")
+            self._valid[slot] = self.table.version()
             return self.local[slot]
 
     def sync_origin(self):

@@ -14,6 +14,7 @@ namespace py = pybind11;
 using namespace slate_hip;
 
 void register_devpool(py::module& m);   // devpool.hip
+void register_ffn(py::module& m);       // bindings_ffn.hip
 
 static inline hipStream_t S(uintptr_t s) { return reinterpret_cast<hipStream_t>(s); }
 
@@ -396,6 +397,7 @@ PYBIND11_MODULE(_hip, m) {
     m.def("gemm_ptrs", &py_gemm_ptrs);
     register_kernels(m);
     register_devpool(m);
+    register_ffn(m);
     // CU-masked streams: isolate latency-bound panel kernels from the bulk
     // trailing-update GEMM (hipExtStreamCreateWithCUMask).  Returns the raw
     // handle for torch.cuda.ExternalStream.

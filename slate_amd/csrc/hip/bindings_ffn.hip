@@ -1,0 +1,102 @@
+// pybind11 entry points of the fused feed-forward products, their gradients,
+// gradient clipping, and copies to and from the 16-bit element types.
+#include <pybind11/pybind11.h>
+#include <pybind11/stl.h>
+#include "ffn.hpp"
+
+namespace py = pybind11;
+using namespace slate_hip;
+
+namespace {
+
+inline hipStream_t S(uintptr_t s) { return reinterpret_cast<hipStream_t>(s); }
+inline const void* P(uintptr_t p) { return reinterpret_cast<const void*>(p); }
+inline void* W(uintptr_t p) { return reinterpret_cast<void*>(p); }
+
+template <typename F> void real_dispatch(char dt, F&& f) {
+    switch (dt) {
+        case 'b': f(__bf16()); break;
+        case 'h': f(_Float16()); break;
+        case 's': f(float()); break;
+        case 'd': f(double()); break;
+        default: throw std::invalid_argument("element type must be bfloat16, float16, float32 or float64");
+    }
+}
+
+using Mats = std::vector<std::tuple<uintptr_t, i64, uintptr_t, i64, i64, i64>>;
+std::vector<ClipMat> mats(const Mats& v) {
+    std::vector<ClipMat> c;
+    c.reserve(v.size());
+    for (auto& [A, lda, B, ldb, m, n] : v)
+        if (m > 0 && n > 0) c.push_back({P(A), W(B), m, n, lda, ldb});
+    return c;
+}
+
+}  // namespace
+
+void register_ffn(py::module& m) {
+    m.def("gemm_act_ws", [](int es, int mode, i64 mm, i64 n, i64 k) { return gemm_act_plan(es, mode, mm, n, k).bytes; });
+    m.def("gemm_act", [](char dt, int mode, char ta, char tb, i64 mm, i64 n, i64 k, double alpha,
+                         uintptr_t A0, i64 lda0, uintptr_t A1, i64 lda1, uintptr_t B0, i64 ldb0, uintptr_t B1, i64 ldb1,
+                         uintptr_t C0, i64 ldc0, uintptr_t C1, i64 ldc1, uintptr_t bias, i64 incb, int bias_mode,
+                         int act, double beta, uintptr_t R, i64 ldr, uintptr_t Z0, i64 ldz0, uintptr_t Z1, i64 ldz1,
+                         uintptr_t ws, uintptr_t st) {
+        GemmActArgs a;
+        a.m = mm; a.n = n; a.k = k;
+        a.mode = mode; a.alpha = alpha; a.beta = beta; a.act = act;
+        a.A[0] = P(A0); a.lda[0] = lda0; a.A[1] = P(A1); a.lda[1] = lda1;
+        a.B[0] = P(B0); a.ldb[0] = ldb0; a.B[1] = P(B1); a.ldb[1] = ldb1;
+        a.C[0] = W(C0); a.ldc[0] = ldc0; a.C[1] = W(C1); a.ldc[1] = ldc1;
+        a.Z[0] = W(Z0); a.ldz[0] = ldz0; a.Z[1] = W(Z1); a.ldz[1] = ldz1;
+        a.bias = P(bias); a.incb = incb; a.bias_mode = bias_mode;
+        a.R = P(R); a.ldr = ldr;
+        a.part = W(ws);
+        real_dispatch(dt, [&](auto z) {
+            using T = decltype(z);
+            const GemmActPlan p = gemm_act_plan(sizeof(T), mode, mm, n, k);
+            if (p.bytes && !ws) throw std::invalid_argument("gemm_act: workspace missing");
+            gemm_act<T>(a, ta, tb, p, S(st));
+        });
+    });
+    m.def("act_grad_ws", [](char dt, int bias_mode, i64 mm, i64 n) {
+        i64 bytes = 0;
+        real_dispatch(dt, [&](auto z) {
+            const int es = sizeof(z);
+            if (bias_mode) bytes = (i64)act_grad_chunks(bias_mode, es, mm, n) * (bias_mode == 1 ? mm : n) * (es == 8 ? 8 : 4);
+        });
+        return bytes;
+    });
+    m.def("act_grad", [](char dt, i64 mm, i64 n, int act, uintptr_t dC, i64 lddc, uintptr_t Z1, i64 ldz1, uintptr_t Z2,
+                         i64 ldz2, uintptr_t dZ1, uintptr_t dZ2, i64 lddz, uintptr_t db, i64 incb, int bias_mode,
+                         bool wide, uintptr_t ws, uintptr_t st) {
+        ActGradArgs a;
+        a.m = mm; a.n = n; a.act = act;
+        a.dC = P(dC); a.lddc = lddc; a.Z1 = P(Z1); a.ldz1 = ldz1; a.Z2 = P(Z2); a.ldz2 = ldz2;
+        a.dZ1 = W(dZ1); a.dZ2 = W(dZ2); a.lddz = lddz;
+        a.db = W(db); a.incb = incb; a.bias_mode = bias_mode; a.wide = wide;
+        a.part = W(ws);
+        if (bias_mode && !ws) throw std::invalid_argument("act_grad: workspace missing");
+        real_dispatch(dt, [&](auto z) { act_grad<decltype(z)>(a, S(st)); });
+    });
+    m.def("clip_ws", [](const Mats& v) { const auto c = mats(v); return clip_parts(c.data(), (int)c.size()); });
+    m.def("clip_sum", [](char ta, const Mats& v, uintptr_t part, uintptr_t st) {
+        const auto c = mats(v);
+        return (i64)clip_sum(ta, c.data(), (int)c.size(), (double*)W(part), S(st));
+    });
+    m.def("clip_join", [](uintptr_t part, i64 parts, uintptr_t out, uintptr_t st) {
+        clip_join((const double*)P(part), (int)parts, (double*)W(out), S(st));
+    });
+    m.def("clip_scale", [](char ta, char tb, const Mats& v, double limit, uintptr_t part, i64 parts, uintptr_t norm,
+                           bool scale, uintptr_t st) {
+        const auto c = mats(v);
+        clip_scale(ta, tb, c.data(), (int)c.size(), limit, (const double*)P(part), (int)parts, (double*)W(norm), scale,
+                   S(st));
+    });
+    m.def("gecopy16", [](char ds, char dd, char uplo, char trans, i64 mm, i64 n, uintptr_t A, i64 lda, uintptr_t B,
+                         i64 ldb, uintptr_t st) {
+        real_dispatch(ds, [&](auto zs) { real_dispatch(dd, [&](auto zd) {
+            using Ts = decltype(zs); using Td = decltype(zd);
+            gecopy16<Ts, Td>(uplo, trans, mm, n, static_cast<const Ts*>(P(A)), lda, static_cast<Td*>(W(B)), ldb, S(st));
+        }); });
+    });
+}

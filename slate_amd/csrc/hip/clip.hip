@@ -1,0 +1,249 @@
+// The common norm of many matrices, and their scaling to at most a given one:
+//   s = sqrt(sum_i |A_i|^2),  B_i = min(1, limit / s) A_i   (B_i = A_i where s
+// is not finite).
+// Memory bound, and launch bound for many small matrices: one launch takes up
+// to CLIP_MATS of them, described in its arguments (no table to copy, so a
+// captured call replays by itself).  Squares are summed in 64 bits, which
+// neither overflow nor underflow for 16- and 32-bit elements; 64-bit elements
+// go to one of three sums by size, the outer two scaled.  The first pass writes
+// one partial sum per block; every block of the second adds them all in the
+// same order, so that there is no third launch and no atomic, and the result
+// is the same on every run.
+#include "ffn.hpp"
+
+namespace slate_hip {
+
+namespace {
+
+constexpr int CLIP_MATS = 48, CLIP_UNIT = 16384, CLIP_BLOCKS = 1024;
+
+struct ClipArgs {
+    ClipMat v[CLIP_MATS];
+    int first[CLIP_MATS + 1];      // units before matrix i
+    int count;
+    double* part;                  // this launch's first partial
+    const double* all;             // every partial (second pass)
+    int parts;
+    double limit;
+    double* norm;
+};
+
+template <typename T> __device__ inline void clip_add(double (&s)[3], T x) {
+    const double d = (double)x;
+    if constexpr (sizeof(T) == 8) {
+        const double a = fabs(d);
+        // borders: squares of the middle range stay inside the type
+        if (a > 1e145) { const double q = d * 0x1p-600; s[2] += q * q; }
+        else if (a < 1e-145) { const double q = d * 0x1p600; s[0] += q * q; }
+        else s[1] += d * d;                                                 // a NaN lands here
+    } else {
+        s[1] += d * d;
+    }
+}
+
+// a block's sum of each entry, in all threads
+__device__ inline double clip_block_sum(double x, double* lds) {
+    x = wave_sum(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+// f(i, j, vector): thread's share of unit u of matrix v, E rows at a time
+template <int E, typename F> __device__ inline void clip_walk(i64 m, i64 n, i64 u, bool flat, F&& f) {
+    const i64 total = m * n, lo = u * CLIP_UNIT, hi = min(total, lo + CLIP_UNIT);
+    if (flat) {
+        for (i64 q = lo + threadIdx.x * E; q < hi; q += 256 * E) f(q, (i64)0);
+        return;
+    }
+    i64 q = lo + threadIdx.x * E;
+    if (q >= hi) return;
+    i64 j = q / m, i = q - j * m;
+    const i64 dj = 256 * E / m, di = 256 * E - dj * m;
+    for (; q < hi; q += 256 * E) {
+        f(i, j);
+        i += di;
+        j += dj;
+        if (i >= m) { i -= m; ++j; }
+    }
+}
+
+__device__ inline int clip_find(const ClipArgs& a, int u) {
+    int lo = 0, hi = a.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.first[mid] <= u) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) clip_sum_kernel(ClipArgs a) {
+    constexpr int E = 16 / sizeof(T);
+    typedef T vE __attribute__((ext_vector_type(E)));
+    __shared__ double lds[4];
+    double s[3] = {0, 0, 0};
+    for (int u = blockIdx.x; u < a.first[a.count]; u += gridDim.x) {
+        const int c = clip_find(a, u);
+        const ClipMat v = a.v[c];
+        const T* A = static_cast<const T*>(v.A);
+        const bool flat = v.lda == v.m || v.n == 1;
+        const i64 uu = u - a.first[c];
+        // whole vectors: aligned, and no vector crosses a column's end
+        if ((uintptr_t)A % 16 == 0 && (flat ? (v.m * v.n) % E == 0 : (v.lda % E == 0 && v.m % E == 0))) {
+            clip_walk<E>(v.m, v.n, uu, flat, [&](i64 i, i64 j) {
+                const vE x = *reinterpret_cast<const vE*>(A + i + j * v.lda);
+                #pragma unroll
+                for (int e = 0; e < E; ++e) clip_add(s, (T)x[e]);
+            });
+        } else {
+            clip_walk<1>(v.m, v.n, uu, flat, [&](i64 i, i64 j) { clip_add(s, A[i + j * v.lda]); });
+        }
+    }
+    #pragma unroll
+    for (int h = 0; h < 3; ++h) {
+        const double x = clip_block_sum(s[h], lds);
+        if (threadIdx.x == 0) a.part[3 * (i64)blockIdx.x + h] = x;
+    }
+}
+
+// the norm and the factor from all partial sums, in every thread
+__device__ inline double clip_norm_of(const ClipArgs& a, double* lds) {
+    double s[3] = {0, 0, 0};
+    for (int i = threadIdx.x; i < a.parts; i += 256)
+        #pragma unroll
+        for (int h = 0; h < 3; ++h) s[h] += a.all[3 * (i64)i + h];
+    #pragma unroll
+    for (int h = 0; h < 3; ++h) s[h] = clip_block_sum(s[h], lds);
+    if (s[1] != s[1]) return s[1];
+    // the middle sum counts beside the large one only while it is not lost in it
+    if (s[2] > 0) return sqrt(s[2] + (s[1] * 0x1p-600) * 0x1p-600) * 0x1p600;
+    if (s[1] > 0) return sqrt(s[1] + (s[0] * 0x1p-600) * 0x1p-600);
+    return sqrt(s[0]) * 0x1p-600;
+}
+
+template <typename TA, typename TB>
+__global__ void __launch_bounds__(256) clip_scale_kernel(ClipArgs a) {
+    using R = std::conditional_t<sizeof(TA) == 8, double, float>;
+    constexpr int E = 16 / sizeof(TA);
+    typedef TA vA __attribute__((ext_vector_type(E)));
+    typedef TB vB __attribute__((ext_vector_type(E)));
+    __shared__ double lds[4];
+    const double norm = clip_norm_of(a, lds);
+    if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
+    const bool cut = norm > a.limit && norm < __builtin_huge_val();
+    const R f = cut ? (R)(a.limit / norm) : R(1);
+    for (int u = blockIdx.x; u < a.first[a.count]; u += gridDim.x) {
+        const int c = clip_find(a, u);
+        const ClipMat v = a.v[c];
+        const TA* A = static_cast<const TA*>(v.A);
+        TB* B = static_cast<TB*>(v.B);
+        if (!cut && v.A == v.B) continue;
+        const bool flat = (v.lda == v.m && v.ldb == v.m) || v.n == 1;
+        const i64 uu = u - a.first[c];
+        if ((uintptr_t)A % 16 == 0 && (uintptr_t)B % sizeof(vB) == 0 &&
+            (flat ? (v.m * v.n) % E == 0 : (v.lda % E == 0 && v.ldb % E == 0 && v.m % E == 0))) {
+            clip_walk<E>(v.m, v.n, uu, flat, [&](i64 i, i64 j) {
+                const vA x = *reinterpret_cast<const vA*>(A + i + j * v.lda);
+                vB y;
+                #pragma unroll
+                for (int e = 0; e < E; ++e) y[e] = (TB)(cut ? (R)x[e] * f : (R)x[e]);
+                *reinterpret_cast<vB*>(B + i + j * v.ldb) = y;
+            });
+        } else {
+            clip_walk<1>(v.m, v.n, uu, flat, [&](i64 i, i64 j) {
+                const R x = (R)A[i + j * v.lda];
+                B[i + j * v.ldb] = (TB)(cut ? x * f : x);
+            });
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) clip_join_kernel(const double* part, int parts, double* out) {
+    __shared__ double lds[4];
+    #pragma unroll
+    for (int h = 0; h < 3; ++h) {
+        double s = 0;
+        for (int i = threadIdx.x; i < parts; i += 256) s += part[3 * (i64)i + h];
+        s = clip_block_sum(s, lds);
+        if (threadIdx.x == 0) out[h] = s;
+    }
+}
+
+// the matrices [at, at + CLIP_MATS) as one launch's arguments; -> its units
+int clip_fill(ClipArgs& a, const ClipMat* v, int count, int at) {
+    a.count = std::max(0, std::min(CLIP_MATS, count - at));
+    a.first[0] = 0;
+    for (int i = 0; i < a.count; ++i) {
+        a.v[i] = v[at + i];
+        a.first[i + 1] = a.first[i] + (int)((a.v[i].m * a.v[i].n + CLIP_UNIT - 1) / CLIP_UNIT);
+    }
+    return a.first[a.count];
+}
+
+template <typename TA, typename TB>
+void clip_scale_run(const ClipMat* v, int count, double limit, const double* part, int parts, double* norm, hipStream_t s) {
+    for (int at = 0; at == 0 || at < count; at += CLIP_MATS) {
+        ClipArgs a;
+        const int blocks = std::min(CLIP_BLOCKS, clip_fill(a, v, count, at));
+        a.limit = limit;
+        a.all = part;
+        a.parts = parts;
+        a.norm = at == 0 ? norm : nullptr;
+        hipLaunchKernelGGL((clip_scale_kernel<TA, TB>), dim3(std::max(1, blocks)), dim3(256), 0, s, a);
+        HIP_LAUNCH_CHECK();
+    }
+}
+
+}  // namespace
+
+i64 clip_parts(const ClipMat* v, int count) {
+    i64 parts = 0;
+    for (int at = 0; at < count; at += CLIP_MATS) {
+        i64 units = 0;
+        for (int i = at; i < std::min(count, at + CLIP_MATS); ++i) {
+            const i64 u = (v[i].m * v[i].n + CLIP_UNIT - 1) / CLIP_UNIT;
+            if (u + units > 0x7fffffff) throw std::invalid_argument("clip_norm: matrices too large for one call");
+            units += u;
+        }
+        parts += std::min<i64>(CLIP_BLOCKS, units);
+    }
+    return 3 * parts;
+}
+
+int clip_sum(char ta, const ClipMat* v, int count, double* part, hipStream_t s) {
+    int done = 0;
+    for (int at = 0; at < count; at += CLIP_MATS) {
+        ClipArgs a;
+        const int blocks = std::min(CLIP_BLOCKS, clip_fill(a, v, count, at));
+        a.part = part + 3 * (i64)done;
+        done += blocks;
+        if (ta == 'b') hipLaunchKernelGGL((clip_sum_kernel<__bf16>), dim3(blocks), dim3(256), 0, s, a);
+        else if (ta == 'h') hipLaunchKernelGGL((clip_sum_kernel<_Float16>), dim3(blocks), dim3(256), 0, s, a);
+        else if (ta == 's') hipLaunchKernelGGL((clip_sum_kernel<float>), dim3(blocks), dim3(256), 0, s, a);
+        else if (ta == 'd') hipLaunchKernelGGL((clip_sum_kernel<double>), dim3(blocks), dim3(256), 0, s, a);
+        else throw std::invalid_argument("clip_norm: bad element type");
+        HIP_LAUNCH_CHECK();
+    }
+    return done;
+}
+
+void clip_join(const double* part, int parts, double* out, hipStream_t s) {
+    hipLaunchKernelGGL(clip_join_kernel, dim3(1), dim3(256), 0, s, part, parts, out);
+    HIP_LAUNCH_CHECK();
+}
+
+void clip_scale(char ta, char tb, const ClipMat* v, int count, double limit, const double* part, int parts,
+                double* norm, bool scale, hipStream_t s) {
+    if (!scale) count = 0;
+    if (ta == 'b' && tb == 'b') clip_scale_run<__bf16, __bf16>(v, count, limit, part, parts, norm, s);
+    else if (ta == 'b' && tb == 's') clip_scale_run<__bf16, float>(v, count, limit, part, parts, norm, s);
+    else if (ta == 'h' && tb == 'h') clip_scale_run<_Float16, _Float16>(v, count, limit, part, parts, norm, s);
+    else if (ta == 'h' && tb == 's') clip_scale_run<_Float16, float>(v, count, limit, part, parts, norm, s);
+    else if (ta == 's' && tb == 's') clip_scale_run<float, float>(v, count, limit, part, parts, norm, s);
+    else if (ta == 'd' && tb == 'd') clip_scale_run<double, double>(v, count, limit, part, parts, norm, s);
+    else throw std::invalid_argument("clip_norm: bad element types");
+}
+
+}  // namespace slate_hip

@@ -1,0 +1,493 @@
+// Matrix products with a fused epilogue for gfx950 (bf16, f16, f32, f64):
+//
+//   plain   Z = alpha sum_p op(A_p) op(B_p) + bias,  C = act(Z) + beta R
+//   gated   Z_i = op(A_i) op(B),                     C = act(Z_1) o Z_2
+//   pair    C_i = alpha op(A_i) op(B_i)              (two products, one launch)
+//
+// Sums are kept in 32 bits (64 for f64) in the MFMA accumulators and rounded
+// once, when C (and Z) are stored.
+//
+// Every operand is staged into LDS as slabs of 128 bytes of K per row
+// (KB = 64 / 32 / 16 elements) by global_load_lds_dwordx4, 1 KiB per wave and
+// instruction, written lane-linear.  The bank swizzle therefore sits on the
+// source address and on the read:
+//  * KC, source contiguous along k (element (r, k) at X[k + r ld]):
+//    image [r][8 chunks of 16 bytes], chunk c of row r at c ^ ((r >> 1) & 7):
+//    the 16 rows of a fragment read one chunk column from 16 distinct
+//    16-byte slots of the 256-byte bank row.  One ds_read_b128 per fragment.
+//  * MN, source contiguous along the tile's rows (X[r + k ld]): image
+//    [k][R], the 16-row segment s of row k at s ^ swz(k).  16-bit types read
+//    it with ds_read_b64_tr_b16 (a 4 x 16 block arrives transposed: each lane
+//    gets four k of its row), 32- and 64-bit types with one read per element.
+// A fragment is 16 bytes per lane in either case: lane l holds row l & 15 and
+// the E = 8 / 4 / 2 consecutive k of chunk (l >> 4); A and B use the same
+// k order, so one, four or two MFMAs multiply it.
+#pragma once
+#include "ffn.hpp"
+
+namespace slate_hip {
+
+typedef int i4v __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+typedef _Float16 hf8v __attribute__((ext_vector_type(8)));
+
+template <typename T> struct ga_traits;
+template <> struct ga_traits<__bf16> {
+    using acc = float; using acc4 = f4;
+    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c,
+                                                       0, 0, 0);
+    }
+};
+template <> struct ga_traits<_Float16> {
+    using acc = float; using acc4 = f4;
+    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8v, a), __builtin_bit_cast(hf8v, b), c,
+                                                      0, 0, 0);
+    }
+};
+template <> struct ga_traits<float> {
+    using acc = float; using acc4 = f4;
+    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c) {
+        const f4 x = __builtin_bit_cast(f4, a), y = __builtin_bit_cast(f4, b);
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+        return c;
+    }
+};
+template <> struct ga_traits<double> {
+    using acc = double; using acc4 = d4;
+    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c) {
+        const d2 x = __builtin_bit_cast(d2, a), y = __builtin_bit_cast(d2, b);
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) c = __builtin_amdgcn_mfma_f64_16x16x4f64(x[j], y[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// ------------------------------------------------------------- activations
+// 16-bit results round to 2^-9 at best, so their exponential is the hardware
+// one (a few 2^-24 times the argument); 32- and 64-bit results call exp.
+template <bool FAST> __device__ inline float ga_exp(float x) { return FAST ? __expf(x) : expf(x); }
+template <bool FAST> __device__ inline double ga_exp(double x) { return exp(x); }
+template <bool FAST> __device__ inline float ga_div(float a, float b) {
+    return FAST ? a * __builtin_amdgcn_rcpf(b) : a / b;
+}
+template <bool FAST> __device__ inline double ga_div(double a, double b) { return a / b; }
+__device__ inline float ga_erfc(float x) { return erfcf(x); }
+__device__ inline double ga_erfc(double x) { return erfc(x); }
+
+// Beyond GA_FLAT the smooth activations are 0 (left) or z itself (right) in
+// their type: arguments are held inside it, which keeps 0 * inf out.
+template <typename R> __device__ constexpr R ga_flat() { return sizeof(R) == 4 ? R(120) : R(800); }
+
+template <bool FAST, typename R> __device__ inline R ga_act(int act, R z) {
+    if (act == ACT_IDENTITY) return z;
+    if (act == ACT_RELU) return z < R(0) ? R(0) : z;                             // a NaN stays one
+    z = z < -ga_flat<R>() ? -ga_flat<R>() : z;
+    if (act == ACT_GELU) return R(0.5) * z * ga_erfc(z * R(-0.70710678118654752440));
+    if (act == ACT_GELU_TANH) {                                                  // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
+        const R u2 = R(1.59576912160573071176) * (z + R(0.044715) * z * z * z);
+        return ga_div<FAST>(z, R(1) + ga_exp<FAST>(-u2));
+    }
+    return ga_div<FAST>(z, R(1) + ga_exp<FAST>(-z));
+}
+// value and slope at once (the backward pass of a gated product needs both)
+template <bool FAST, typename R> __device__ inline void ga_act_grad(int act, R z, R& v, R& d) {
+    if (act == ACT_IDENTITY) { v = z; d = R(1); return; }
+    if (act == ACT_RELU) { v = z < R(0) ? R(0) : z; d = z > R(0) ? R(1) : (z <= R(0) ? R(0) : z); return; }
+    const R L = ga_flat<R>(), x = z < -L ? -L : (z > L ? L : z);
+    R p, e;                                                                      // v = x p, d = p + x e
+    if (act == ACT_GELU) {
+        p = R(0.5) * ga_erfc(x * R(-0.70710678118654752440));
+        e = R(0.39894228040143267794) * ga_exp<FAST>(R(-0.5) * x * x);
+    } else if (act == ACT_GELU_TANH) {
+        const R u2 = R(1.59576912160573071176) * (x + R(0.044715) * x * x * x);
+        p = ga_div<FAST>(R(1), R(1) + ga_exp<FAST>(-u2));
+        e = p * (R(1) - p) * R(1.59576912160573071176) * (R(1) + R(0.134145) * x * x);
+    } else {
+        p = ga_div<FAST>(R(1), R(1) + ga_exp<FAST>(-x));
+        e = p * (R(1) - p);
+    }
+    v = z > L ? z : x * p;
+    d = p + x * e;
+}
+
+// V rows of column n: the epilogue on finished sums
+template <typename T, int V, bool GATED>
+__device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, const typename ga_traits<T>::acc* s1,
+                                 const typename ga_traits<T>::acc* s2) {
+    using R = typename ga_traits<T>::acc;
+    constexpr bool FAST = sizeof(T) == 2;
+    typedef T vT __attribute__((ext_vector_type(V)));
+    if (n >= a.n || m >= a.m) return;
+    const bool whole = V == 1 || m + V <= a.m;
+    const int left = (int)min((i64)V, a.m - m);
+    T* C = static_cast<T*>(a.C[pair]) + m + n * a.ldc[pair];
+    R z[V], y[V];
+    if constexpr (GATED) {
+        #pragma unroll
+        for (int r = 0; r < V; ++r) { z[r] = s1[r]; y[r] = ga_act<FAST>(a.act, s1[r]) * s2[r]; }
+    } else {
+        const R alpha = (R)a.alpha;
+        #pragma unroll
+        for (int r = 0; r < V; ++r) z[r] = alpha * s1[r];
+        if (a.bias_mode == 1) {
+            const T* b = static_cast<const T*>(a.bias);
+            if (whole && (a.vec & 8)) {
+                const vT x = *reinterpret_cast<const vT*>(b + m);
+                #pragma unroll
+                for (int r = 0; r < V; ++r) z[r] += (R)x[r];
+            } else {
+                #pragma unroll
+                for (int r = 0; r < V; ++r) if (r < left) z[r] += (R)b[(m + r) * a.incb];
+            }
+        } else if (a.bias_mode == 2) {
+            const R x = (R) static_cast<const T*>(a.bias)[n * a.incb];
+            #pragma unroll
+            for (int r = 0; r < V; ++r) z[r] += x;
+        }
+        #pragma unroll
+        for (int r = 0; r < V; ++r) y[r] = ga_act<FAST>(a.act, z[r]);
+        if (a.R) {
+            const T* X = static_cast<const T*>(a.R) + m + n * a.ldr;
+            const R beta = (R)a.beta;
+            if (whole && (a.vec & 2)) {
+                const vT x = *reinterpret_cast<const vT*>(X);
+                #pragma unroll
+                for (int r = 0; r < V; ++r) y[r] += beta * (R)x[r];
+            } else {
+                #pragma unroll
+                for (int r = 0; r < V; ++r) if (r < left) y[r] += beta * (R)X[r];
+            }
+        }
+    }
+    auto put = [&](T* p, const R* v, bool wide) {
+        if (wide) {
+            vT x;
+            #pragma unroll
+            for (int r = 0; r < V; ++r) x[r] = (T)v[r];
+            *reinterpret_cast<vT*>(p) = x;
+        } else {
+            #pragma unroll
+            for (int r = 0; r < V; ++r) if (r < left) p[r] = (T)v[r];
+        }
+    };
+    put(C, y, whole && (a.vec & 1));
+    if (a.Z[0]) put(static_cast<T*>(a.Z[0]) + m + n * a.ldz[0], z, whole && (a.vec & 4));
+    if constexpr (GATED)
+        if (a.Z[1]) put(static_cast<T*>(a.Z[1]) + m + n * a.ldz[1], s2, whole && (a.vec & 4));
+}
+
+// ------------------------------------------------------------- LDS images
+template <typename T, int R, bool KC> struct GaImg {
+    static constexpr int ES = sizeof(T), E = 16 / ES, KB = 128 / ES;
+    static constexpr int BYTES = R * 128, CHUNKS = BYTES / 1024;
+    static constexpr int ROWB = R * ES;                       // MN: bytes per k
+    static constexpr int SEGB = 16 * ES;                      // MN: bytes of a 16-row segment
+    static constexpr int NSEG = R / 16;
+    // MN: which segments the k rows that one read touches together go to
+    __device__ static constexpr int swz(int k) {
+        if constexpr (ES == 2) return ((k & 3) | ((k >> 1) & 4)) & (NSEG - 1);
+        else if constexpr (ES == 4) return (k >> 2) & 3 & (NSEG - 1);
+        else return (k >> 1) & 1 & (NSEG - 1);
+    }
+    // row and k of the first element of 16-byte slot q
+    __device__ static inline void src_of(int q, int& r, int& k) {
+        if constexpr (KC) {
+            r = q >> 3;
+            k = ((q & 7) ^ ((r >> 1) & 7)) * E;
+        } else {
+            const int p = q * 16;
+            k = p / ROWB;
+            r = ((p % ROWB) ^ (swz(k) * SEGB)) / ES;
+        }
+    }
+    // this lane's fragment: rows r0..r0+15, chunk half kk
+    __device__ static inline i4v frag(const char* img, int r0, int kk, int lane) {
+        const int l = lane & 15, g = lane >> 4;
+        if constexpr (KC) {
+            const int r = r0 + l;
+            return *reinterpret_cast<const i4v*>(img + r * 128 + (((kk * 4 + g) ^ ((r >> 1) & 7)) << 4));
+        } else if constexpr (ES == 2) {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef int i2 __attribute__((ext_vector_type(2)));
+            const int k = kk * 32 + g * 8 + (l >> 2);
+            const char* p = img + k * ROWB + (((r0 >> 4) ^ swz(k)) * SEGB) + (l & 3) * 8;
+            using lds_s4 = __attribute__((address_space(3))) s4;
+            const i2 x = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p));
+            const i2 y = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 4 * ROWB)));
+            return i4v{x[0], x[1], y[0], y[1]};
+        } else {
+            T v[E];
+            #pragma unroll
+            for (int j = 0; j < E; ++j) {
+                const int k = (kk * 4 + g) * E + j;
+                v[j] = *reinterpret_cast<const T*>(img + k * ROWB + (((r0 >> 4) ^ swz(k)) * SEGB) + l * ES);
+            }
+            if constexpr (ES == 4) return __builtin_bit_cast(i4v, f4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]});
+            else return __builtin_bit_cast(i4v, d2{(double)v[0], (double)v[1]});
+        }
+    }
+    // bytes from the slab's first element that lane `lane` of chunk c stages;
+    // rows past the matrix read a row that exists and feed no stored output
+    __device__ static inline uint32_t offset(int c, int lane, i64 ld, i64 rows) {
+        int r, k;
+        src_of(c * 64 + lane, r, k);
+        if constexpr (KC) {
+            const i64 rr = r < rows ? r : rows - 1;
+            return (uint32_t)((rr * ld + k) * ES);
+        } else {
+            const i64 rr = r < rows ? r : 0;
+            return (uint32_t)((k * ld + rr) * ES);
+        }
+    }
+    // the slab through registers: any alignment, zeros past the matrix
+    template <int NT>
+    __device__ static inline void stage(const T* X, i64 ld, i64 rows, i64 kleft, char* img, int tid) {
+        for (int q = tid; q < BYTES / 16; q += NT) {
+            int r, k;
+            src_of(q, r, k);
+            T v[E];
+            #pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int rr = KC ? r : r + e, kx = KC ? k + e : k;
+                v[e] = (T)0;
+                if (rr < rows && kx < kleft) v[e] = KC ? X[rr * ld + kx] : X[kx * ld + rr];
+            }
+            typedef T vE __attribute__((ext_vector_type(E)));
+            vE w;
+            #pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = v[e];
+            *reinterpret_cast<vE*>(img + q * 16) = w;
+        }
+    }
+};
+
+// The epilogue turns the accumulators through LDS, a wave's columns NJ
+// fragments at a time, so that stores (and the loads of bias and residual) run
+// along the rows in 16-byte accesses and the activation appears in the code
+// once: unrolled over the 32 fragments of a wave it is 16 000 instructions.
+template <typename T, int BM, int BN, int WVM, int WVN> struct GaEpi {
+    static constexpr int AS = sizeof(typename ga_traits<T>::acc), NW = WVM * WVN, NI = BN / WVN / 16;
+    static constexpr int LDR = BM / WVM + 16 / AS;                    // rows of a column, and 16 bytes against conflicts
+    static constexpr int RING = 2 * (BM + BN) * 128, MOST = RING > 131071 ? 163840 : (RING > 65535 ? 81920 : RING);
+    static constexpr int bytes(int nj) { return NW * LDR * 16 * nj * AS; }
+    static constexpr int pick() { int nj = NI; while (nj > 1 && bytes(nj) > MOST) nj /= 2; return nj; }
+    static constexpr int NJ = pick();
+    static constexpr int LDS = RING > bytes(NJ) ? RING : bytes(NJ);
+    static_assert(LDS <= 163840, "tile does not fit the LDS");
+};
+
+// ------------------------------------------------------------------ kernel
+template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, bool GATED>
+__global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a) {
+    using TR = ga_traits<T>;
+    using acc4 = typename TR::acc4;
+    using R = typename TR::acc;
+    constexpr int NW = WVM * WVN, NT = 64 * NW, NA = GATED ? 2 : 1, BMI = BM / NA;
+    constexpr int WM = BM / WVM, WN = BN / WVN, MI = WM / 16, NI = WN / 16, KB = 128 / (int)sizeof(T);
+    using IA = GaImg<T, BMI, AKC>;
+    using IB = GaImg<T, BN, BKC>;
+    constexpr int SLOT = (BM + BN) * 128;
+    constexpr int PA = (IA::CHUNKS + NW - 1) / NW, PB = (IB::CHUNKS + NW - 1) / NW;
+    static_assert(MI % NA == 0, "gated tiles pair their fragments");
+    extern __shared__ __align__(16) char smem[];
+
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int gm = (int)((a.m + BMI - 1) / BMI), gn = (int)((a.n + BN - 1) / BN), nblk = gm * gn;
+    // blocks b and b + 8 share an XCD: consecutive tiles of one group there
+    const int lin = xcd_remap(blockIdx.x, nblk);
+    const int G = a.group_m, grp = lin / (G * gn), first = grp * G, gsz = min(gm - first, G);
+    const int inner = lin - grp * G * gn;
+    const i64 m0 = (i64)(first + inner % gsz) * BMI, n0 = (i64)(inner / gsz) * BN;
+    const int pair = a.mode == GA_PAIR ? blockIdx.z : 0;
+    const int total = a.nsteps * (a.mode == GA_SUM ? 2 : 1);
+    const int s0 = a.splits > 1 ? (int)blockIdx.y * a.per_split : 0;
+    const int s1 = a.splits > 1 ? min(total, s0 + a.per_split) : total;
+
+    uint32_t offA[NA][PA], offB[PB];
+    const i64 rowsA = a.m - m0, rowsB = a.n - n0;
+    const bool sum = a.mode == GA_SUM;
+    auto offsets = [&](int p) {
+        #pragma unroll
+        for (int h = 0; h < NA; ++h)
+            #pragma unroll
+            for (int i = 0; i < PA; ++i)
+                offA[h][i] = IA::offset(min(wid + i * NW, IA::CHUNKS - 1), lane, a.lda[GATED ? h : p], rowsA);
+        #pragma unroll
+        for (int i = 0; i < PB; ++i)
+            offB[i] = IB::offset(min(wid + i * NW, IB::CHUNKS - 1), lane, a.ldb[p], rowsB);
+    };
+    int curp = sum ? (s0 >= a.nsteps ? 1 : 0) : pair;
+    offsets(curp);
+
+    using gptr = const __attribute__((address_space(1))) void*;
+    using lptr = __attribute__((address_space(3))) void*;
+    auto issue = [&](int s) {
+        int kt = s, p = pair;
+        if (sum && s >= a.nsteps) { kt = s - a.nsteps; p = 1; }
+        if (sum && p != curp) { curp = p; offsets(p); }
+        char* slot = smem + (s & 1) * SLOT;
+        const i64 k0 = (i64)kt * KB;
+        if (kt < a.nfull) {
+            #pragma unroll
+            for (int h = 0; h < NA; ++h) {
+                const int q = GATED ? h : p;
+                const char* X = static_cast<const char*>(a.A[q]) +
+                                (AKC ? m0 * a.lda[q] + k0 : m0 + k0 * a.lda[q]) * (i64)sizeof(T);
+                #pragma unroll
+                for (int i = 0; i < PA; ++i) {
+                    const int c = min(wid + i * NW, IA::CHUNKS - 1);
+                    __builtin_amdgcn_global_load_lds((gptr)(X + offA[h][i]),
+                                                     (lptr)(slot + h * IA::BYTES + c * 1024), 16, 0, 0);
+                }
+            }
+            const char* Y = static_cast<const char*>(a.B[p]) +
+                            (BKC ? n0 * a.ldb[p] + k0 : n0 + k0 * a.ldb[p]) * (i64)sizeof(T);
+            #pragma unroll
+            for (int i = 0; i < PB; ++i) {
+                const int c = min(wid + i * NW, IB::CHUNKS - 1);
+                __builtin_amdgcn_global_load_lds((gptr)(Y + offB[i]), (lptr)(slot + BM * 128 + c * 1024), 16, 0, 0);
+            }
+        } else {
+            #pragma unroll
+            for (int h = 0; h < NA; ++h) {
+                const int q = GATED ? h : p;
+                IA::template stage<NT>(static_cast<const T*>(a.A[q]) + (AKC ? m0 * a.lda[q] + k0 : m0 + k0 * a.lda[q]),
+                                       a.lda[q], rowsA, a.k - k0, slot + h * IA::BYTES, tid);
+            }
+            IB::template stage<NT>(static_cast<const T*>(a.B[p]) + (BKC ? n0 * a.ldb[p] + k0 : n0 + k0 * a.ldb[p]),
+                                   a.ldb[p], rowsB, a.k - k0, slot + BM * 128, tid);
+        }
+    };
+
+    const int wm = wid / WVN, wn = wid % WVN;
+    acc4 acc[MI][NI];
+    #pragma unroll
+    for (int i = 0; i < MI; ++i)
+        #pragma unroll
+        for (int j = 0; j < NI; ++j)
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = R(0);
+
+    if (s0 < s1) issue(s0);
+    for (int s = s0; s < s1; ++s) {
+        // my part of step s has landed ...
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        // ... and everyone's, and everyone has read step s - 1's slot
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + 1 < s1) issue(s + 1);
+        const char* la = smem + (s & 1) * SLOT;
+        const char* lb = la + BM * 128;
+        #pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            i4v fa[MI], fb[NI];
+            #pragma unroll
+            for (int j = 0; j < NI; ++j) fb[j] = IB::frag(lb, wn * WN + j * 16, kk, lane);
+            #pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                constexpr int H = MI / NA;
+                fa[i] = IA::frag(la + (i / H) * IA::BYTES, wm * (WM / NA) + (i % H) * 16, kk, lane);
+            }
+            #pragma unroll
+            for (int i = 0; i < MI; ++i)
+                #pragma unroll
+                for (int j = 0; j < NI; ++j) {
+                    // D's four registers run along the rows of the first operand:
+                    // rows of C for f32 sums; for f64 they are 4 apart, and the
+                    // columns take them so that lanes run along the rows
+                    if constexpr (sizeof(R) == 4) acc[i][j] = TR::mma(fa[i], fb[j], acc[i][j]);
+                    else acc[i][j] = TR::mma(fb[j], fa[i], acc[i][j]);
+                }
+        }
+    }
+
+    constexpr int H = MI / NA, WH = WM / NA;
+    const i64 mw = m0 + wm * WH, nw = n0 + wn * WN;
+    // row and column, inside the wave's tile, of register r of fragment (i, j)
+    auto row_of = [&](int i, int r) { return i * 16 + (sizeof(R) == 4 ? (lane >> 4) * 4 + r : (lane & 15)); };
+    auto col_of = [&](int j, int r) { return j * 16 + (sizeof(R) == 4 ? (lane & 15) : (lane >> 4) + 4 * r); };
+    if (a.splits > 1) {
+        const int planes = GATED ? 2 : (int)gridDim.z;
+        #pragma unroll
+        for (int i = 0; i < MI; ++i)
+            #pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const i64 plane = (i64)blockIdx.y * planes + (GATED ? i / H : pair);
+                if constexpr (sizeof(R) == 4) {
+                    const i64 m = mw + row_of(i % H, 0), n = nw + col_of(j, 0);
+                    if (m < a.m && n < a.n)
+                        *reinterpret_cast<f4*>(static_cast<float*>(a.part) + (plane * a.n + n) * a.ldp + m) = acc[i][j];
+                } else {
+                    #pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const i64 m = mw + row_of(i % H, r), n = nw + col_of(j, r);
+                        if (m < a.m && n < a.n) static_cast<R*>(a.part)[(plane * a.n + n) * a.ldp + m] = acc[i][j][r];
+                    }
+                }
+            }
+        return;
+    }
+    using EP = GaEpi<T, BM, BN, WVM, WVN>;
+    constexpr int NJ = EP::NJ, LDR = EP::LDR, V = 16 / (int)sizeof(T);
+    R* img = reinterpret_cast<R*>(smem) + wid * (LDR * 16 * NJ);
+    __syncthreads();                                 // every wave has read its last slab
+    #pragma unroll 1
+    for (int pass = 0; pass < NI / NJ; ++pass) {
+        #pragma unroll
+        for (int q = 0; q < NI / NJ; ++q)
+            if (q == pass) {
+                #pragma unroll
+                for (int i = 0; i < MI; ++i)
+                    #pragma unroll
+                    for (int jj = 0; jj < NJ; ++jj)
+                        #pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            img[col_of(jj, r) * LDR + (i / H) * WH + row_of(i % H, r)] = acc[i][q * NJ + jj][r];
+            }
+        // a wave reads what it wrote itself: its LDS accesses complete in order
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        #pragma unroll 1
+        for (int t = lane; t < (WH / V) * 16 * NJ; t += 64) {
+            const int rr = (t % (WH / V)) * V, cc = t / (WH / V);
+            R x[V], y[V];
+            #pragma unroll
+            for (int r = 0; r < V; ++r) {
+                x[r] = img[cc * LDR + rr + r];
+                if constexpr (GATED) y[r] = img[cc * LDR + WH + rr + r];
+            }
+            ga_finish<T, V, GATED>(a, pair, mw + rr, nw + pass * (16 * NJ) + cc, x, y);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+// adds the partial sums in the order of their splits and finishes them
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(256) gemm_act_join_kernel(GemmActArgs a) {
+    using R = typename ga_traits<T>::acc;
+    constexpr int V = 16 / (int)sizeof(T);
+    typedef R vR __attribute__((ext_vector_type(V)));
+    const i64 mv = (a.m + V - 1) / V;
+    const i64 t = (i64)blockIdx.x * 256 + threadIdx.x;
+    if (t >= mv * a.n) return;
+    const i64 n = t / mv, m = (t - n * mv) * V;
+    const int planes = a.mode == GA_PAIR || GATED ? 2 : 1, pair = GATED ? 0 : (int)blockIdx.z;
+    R x[2][V];
+    #pragma unroll
+    for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+        #pragma unroll
+        for (int r = 0; r < V; ++r) x[h][r] = R(0);
+        const R* P = static_cast<const R*>(a.part) + ((i64)(GATED ? h : pair) * a.n + n) * a.ldp + m;
+        for (int s = 0; s < a.splits; ++s) {
+            const vR v = *reinterpret_cast<const vR*>(P + (i64)s * planes * a.n * a.ldp);
+            #pragma unroll
+            for (int r = 0; r < V; ++r) x[h][r] += v[r];
+        }
+    }
+    ga_finish<T, V, GATED>(a, pair, m, n, x[0], x[GATED ? 1 : 0]);
+}
+
+}  // namespace slate_hip

@@ -1,0 +1,4 @@
+#include "gemm_act_launch.hpp"
+namespace slate_hip {
+template void gemm_act<__bf16>(GemmActArgs, char, char, const GemmActPlan&, hipStream_t);
+}

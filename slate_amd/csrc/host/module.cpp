@@ -6,6 +6,7 @@ void register_runtime(py::module& m);
 void register_tile_kernels(py::module& m);
 void register_matgen(py::module& m);
 void register_eig(py::module& m);
+void register_ffn(py::module& m);
 }
 PYBIND11_MODULE(_host, m) {
     m.doc() = "slate_amd native host runtime (MOSI table, slab pool, trace, host tile kernels, matgen)";
@@ -13,4 +14,5 @@ PYBIND11_MODULE(_host, m) {
     slate_host::register_tile_kernels(m);
     slate_host::register_matgen(m);
     slate_host::register_eig(m);
+    slate_host::register_ffn(m);
 }

@@ -56,6 +56,7 @@ public:
     // others Shared (MatrixStorage.hh:1107-1109).
     void insert(int64_t i, int64_t j, int slot, int kind, bool origin) {
         std::lock_guard<std::mutex> g(mu_);
+        ++version_;
         Node& n = nodes_[key(i, j)];
         check_slot(slot);
         Instance& in = n.inst[slot];
@@ -92,6 +93,7 @@ public:
     // dst Modified and every other instance Invalid; with hold, OnHold.
     int acquire(int64_t i, int64_t j, int dst, bool modify, bool hold) {
         std::lock_guard<std::mutex> g(mu_);
+        ++version_;
         Node& n = node(i, j);
         check_slot(dst);
         Instance& d = n.inst[dst];
@@ -127,6 +129,7 @@ public:
     // tileModified (BaseMatrix.hh:1719-1740)
     void modified(int64_t i, int64_t j, int slot, bool permissive) {
         std::lock_guard<std::mutex> g(mu_);
+        ++version_;
         Node& n = node(i, j);
         check_slot(slot);
         if (!n.inst[slot].exists) throw std::runtime_error("tileModified: missing instance");
@@ -140,12 +143,14 @@ public:
     }
     void set_state(int64_t i, int64_t j, int slot, int st) {
         std::lock_guard<std::mutex> g(mu_);
+        ++version_;
         Instance& in = node(i, j).inst[slot];
         in.state = st & 0x111;
         in.hold = (st & OnHold) != 0;
     }
     void unhold(int64_t i, int64_t j, int slot) {
         std::lock_guard<std::mutex> g(mu_);
+        ++version_;
         node(i, j).inst[slot].hold = false;
     }
     // Release a workspace instance if it is neither OnHold nor the last
@@ -153,6 +158,7 @@ public:
     // Returns true when the instance was erased (caller frees the buffer).
     bool release(int64_t i, int64_t j, int slot) {
         std::lock_guard<std::mutex> g(mu_);
+        ++version_;
         auto it = nodes_.find(key(i, j));
         if (it == nodes_.end()) return false;
         Node& n = it->second;
@@ -172,6 +178,7 @@ public:
     }
     void erase(int64_t i, int64_t j, int slot) {
         std::lock_guard<std::mutex> g(mu_);
+        ++version_;
         auto it = nodes_.find(key(i, j));
         if (it == nodes_.end()) return;
         if (slot < 0) { nodes_.erase(it); return; }
@@ -183,6 +190,7 @@ public:
     // Slot holding the latest data (for origin update): -1 if origin valid.
     int update_origin_source(int64_t i, int64_t j) {
         std::lock_guard<std::mutex> g(mu_);
+        ++version_;
         Node& n = node(i, j);
         if (n.origin < 0) return -1;
         if (n.inst[n.origin].state != Invalid) return -1;
@@ -210,6 +218,7 @@ public:
     // kernel or copy).  Returns number of tiles touched.
     int64_t mark_all(int slot, int st) {
         std::lock_guard<std::mutex> g(mu_);
+        ++version_;
         int64_t c = 0;
         for (auto& kv : nodes_) {
             Node& n = kv.second;
@@ -231,9 +240,13 @@ public:
                     out.emplace_back(kv.first.first, kv.first.second, s);
         return out;
     }
+    // Grows with every call that may change a state: a caller that checked the
+    // whole table at one version need not check it again at the same one.
+    int64_t version() const { std::lock_guard<std::mutex> g(mu_); return version_; }
     size_t size() const { std::lock_guard<std::mutex> g(mu_); return nodes_.size(); }
     void clear_workspace() {
         std::lock_guard<std::mutex> g(mu_);
+        ++version_;
         for (auto it = nodes_.begin(); it != nodes_.end();) {
             Node& n = it->second;
             bool any = false;
@@ -268,6 +281,7 @@ private:
         check_slot(slot);
         return it->second.inst[slot];
     }
+    int64_t version_ = 0;
     mutable std::mutex mu_;
     std::unordered_map<std::pair<int64_t, int64_t>, Node, PairHash> nodes_;
 };
@@ -385,6 +399,7 @@ void register_runtime(py::module& m) {
         .def("mark_all", &TileTable::mark_all)
         .def("instances", &TileTable::instances)
         .def("clear_workspace", &TileTable::clear_workspace)
+        .def("version", &TileTable::version)
         .def("__len__", &TileTable::size);
     py::class_<SlabPool>(m, "SlabPool")
         .def(py::init<int64_t, int64_t>())

@@ -17,10 +17,11 @@ from __future__ import annotations
 import torch
 
 from .. import _native
-from .._native import code, kmod, stream
+from .._native import REAL_CODE, code, kmod, stream
 from ..core.exceptions import SlateError
 
 _WORK = {}
+_HALF = (torch.bfloat16, torch.float16)
 _FLOPS = None     # [count] while a flop_counter() is active
 
 
@@ -547,7 +548,12 @@ def gecopy(A, B, uplo='G', trans='N'):
     """B = op(A) with precision conversion (B is m x n)."""
     _chk(A); _chk(B, "B")
     m, n = B.shape
-    if m and n:
+    if m and n and (A.dtype in _HALF or B.dtype in _HALF):
+        if A.dtype not in REAL_CODE or B.dtype not in REAL_CODE:
+            raise SlateError(f"no copy from {A.dtype} to {B.dtype}")
+        kmod(B).gecopy16(REAL_CODE[A.dtype], REAL_CODE[B.dtype], _ch(uplo), _ch(trans), m, n, A.data_ptr(), ld(A),
+                         B.data_ptr(), ld(B), stream(B))
+    elif m and n:
         kmod(B).gecopy(code(A.dtype), code(B.dtype), _ch(uplo), _ch(trans), m, n, A.data_ptr(), ld(A),
                        B.data_ptr(), ld(B), stream(B))
     return B

@@ -1,0 +1,797 @@
+"""Fused feed-forward products, their gradients, and gradient clipping against
+plain formulas in 64 bits, on the host path and (``gpu``) on the gfx950
+kernels.
+
+Tolerances come from the arithmetic.  With u = eps / 2 of the stored type and
+w = 2^-24 (2^-53) of the sums', an element of a product over k terms is off by
+at most (k + 4) w S, S the sum of the terms' sizes (bias among them), in any
+order of the sums; an activation (slope at most 1.13) passes that on and adds
+a few w relative to its argument, 16 w (1 + |z|) |z| with the exponential's
+error; the store adds u of the value.  Where dZ is rounded between two
+products it is off by u + 32 w relative, which the second product's terms
+carry."""
+import math
+
+import pytest
+import torch
+
+import slate_amd as sl
+from slate_amd import ops
+from slate_amd.core.exceptions import SlateError
+
+DEVS = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+TYPES = [torch.bfloat16, torch.float16, torch.float32, torch.float64]
+ACTS = ["identity", "relu", "gelu", "gelu_tanh", "silu"]
+HALF = (torch.bfloat16, torch.float16)
+
+
+def u_of(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def w_of(dt):
+    return 2.0 ** -53 if dt == torch.float64 else 2.0 ** -24
+
+
+def tiny(dt):
+    """Half the distance of the smallest subnormal numbers."""
+    return torch.finfo(dt).tiny * torch.finfo(dt).eps / 2
+
+
+def cm(m, n, dt, seed, dev, std=1.0, pad=0, off=0):
+    """m x n column-major tensor, leading dimension m + pad, first element off."""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(n, m, generator=g, dtype=torch.float64) * std).to(dt).to(dev)
+    buf = torch.full((off + n * (m + pad),), float("nan"), dtype=dt, device=dev)
+    y = buf[off:].view(n, m + pad)[:, :m].t()
+    y.copy_(x.t())
+    return y
+
+
+def mat(t, trans=False, nb=64):
+    M = sl.Matrix.fromLAPACK(t.shape[0], t.shape[1], t, nb=nb)
+    return M.transpose() if trans else M
+
+
+def act64(name, z):
+    if name == "relu":
+        return z.clamp(min=0), (z > 0).double()
+    if name == "gelu":
+        p = 0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+        return z * p, p + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if name == "gelu_tanh":
+        c = math.sqrt(2 / math.pi)
+        h = torch.tanh(c * (z + 0.044715 * z ** 3))
+        return 0.5 * z * (1 + h), 0.5 * (1 + h) + 0.5 * z * (1 - h * h) * c * (1 + 3 * 0.044715 * z * z)
+    if name == "silu":
+        p = torch.sigmoid(z)
+        return z * p, p * (1 + z * (1 - p))
+    return z, torch.ones_like(z)
+
+
+def within(got, want, bound):
+    g = got.double()
+    bad = ~((g - want).abs() <= bound)
+    assert not bad.any(), (int(bad.sum()), float(((g - want).abs() / bound).nan_to_num(1e9).max()))
+
+
+def act_bound(z, w):
+    return 16 * w * (1 + z.abs()) * z.abs()
+
+
+class Product:
+    """Operands, call and oracle of gemm_bias_act."""
+
+    def __init__(self, dt, dev, m, n, k, ta="T", tb="N", bias=1, act="gelu", res=True, keep=True, alpha=0.75, beta=0.5,
+                 pad=0, off=0, seed=0, cpad=0):
+        self.dt, self.dev, self.m, self.n, self.k, self.act, self.alpha, self.beta = dt, dev, m, n, k, act, alpha, beta
+        std = 1 / math.sqrt(max(k, 1))
+        self.A = cm(*((k, m) if ta == "T" else (m, k)), dt, seed + 1, dev, std, pad, off)
+        self.B = cm(*((n, k) if tb == "T" else (k, n)), dt, seed + 2, dev, 1.0, pad, off)
+        self.ta, self.tb = ta, tb
+        self.b = None if not bias else (cm(m, 1, dt, seed + 3, dev) if bias == 1 else cm(1, n, dt, seed + 3, dev))
+        self.R = cm(m, n, dt, seed + 4, dev, 1.0, pad, off) if res else None
+        self.C = cm(m, n, dt, seed + 5, dev, 1.0, cpad, off)
+        self.Z = cm(m, n, dt, seed + 6, dev, 1.0, cpad, off) if keep else None
+
+    def handles(self):
+        h = [mat(self.A, self.ta == "T"), mat(self.B, self.tb == "T")]
+        return h + [None if x is None else mat(x) for x in (self.b, self.R, self.C, self.Z)]
+
+    def want(self):
+        a, b = self.A.double(), self.B.double()
+        a, b = (a.t() if self.ta == "T" else a).contiguous(), (b.t() if self.tb == "T" else b).contiguous()
+        z, S = self.alpha * (a @ b), abs(self.alpha) * (a.abs() @ b.abs())
+        if self.b is not None:
+            z, S = z + self.b.double(), S + self.b.double().abs()
+        w, u = w_of(self.dt), u_of(self.dt)
+        ez = (self.k + 4) * w * S + tiny(self.dt)
+        y = act64(self.act, z)[0]
+        ey = 1.13 * ez + act_bound(z, w)
+        if self.R is not None:
+            y = y + self.beta * self.R.double()
+            ey = ey + 4 * w * (y.abs() + self.beta * self.R.double().abs())
+        return z, ez + u * (z.abs() + ez), y, ey + u * (y.abs() + ey)
+
+    def check(self):
+        z, ez, y, ey = self.want()
+        A, B, b, R, C, Z = self.handles()
+        sl.gemm_bias_act(self.alpha, A, B, b, self.act, self.beta, R, C, Z)
+        within(self.C, y, ey)
+        if self.Z is not None:
+            within(self.Z, z, ez)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT", "TT"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (64, 1, 128), (40, 5, 72), (131, 67, 203), (96, 130, 16)])
+def test_product(dev, dt, ta, tb, m, n, k):
+    Product(dt, dev, m, n, k, ta, tb).check()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("bias", [0, 1, 2])
+@pytest.mark.parametrize("res,keep", [(False, False), (True, False), (False, True)])
+def test_product_epilogue(dev, dt, act, bias, res, keep):
+    Product(dt, dev, 72, 20, 64, act=act, bias=bias, res=res, keep=keep).check()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT"])
+@pytest.mark.parametrize("pad,off,cpad", [(8, 0, 8), (3, 0, 0), (0, 1, 5), (24, 8, 24)])
+def test_product_strides(dev, dt, ta, tb, pad, off, cpad):
+    """Padded and offset storage: aligned and not; what lies beside it stays."""
+    p = Product(dt, dev, 70, 33, 130, ta, tb, pad=pad, off=off, cpad=cpad)
+    p.check()
+    if cpad:
+        assert torch.isnan(p.C.as_strided((cpad, 33), (1, 70 + cpad), p.C.storage_offset() + 70)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT", "TT"])
+@pytest.mark.parametrize("m,n,k", [(3601, 3700, 200), (4096, 4096, 256), (1100, 1300, 520), (260, 300, 1000),
+                                   (2100, 17, 4100), (513, 16, 8200), (5000, 1, 640), (8, 3000, 72)])
+def test_product_sizes(dt, ta, tb, m, n, k):
+    """Every tile, whole and ragged, with K in one piece and in several."""
+    if dt == torch.float64 and m * n * k > 2e9:
+        k = 64 + k % 8
+    Product(dt, "cuda", m, n, k, ta, tb, act="silu", alpha=1.0, beta=1.0).check()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_product_transposed_output(dev, dt):
+    p = Product(dt, dev, 66, 41, 80, bias=1)
+    z, ez, y, ey = p.want()
+    Ct, Zt, Rt = (torch.empty(66, 41, dtype=dt, device=dev).t() for _ in range(3))        # 41 x 66 column-major
+    Rt.copy_(p.R.t())
+    A, B, b, R, C, Z = p.handles()
+    sl.gemm_bias_act(p.alpha, A, B, b, p.act, p.beta, R, mat(Ct, True), mat(Zt, True))
+    within(Ct.t(), y, ey)
+    within(Zt.t(), z, ez)
+    sl.gemm_bias_act(p.alpha, A, B, b, p.act, p.beta, mat(Rt, True), C, mat(Zt, True))
+    within(p.C, y, ey)
+    within(Zt.t(), z, ez)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+def test_product_edges(dev, dt):
+    nan = float("nan")
+    # the residual's own matrix as output
+    p = Product(dt, dev, 40, 24, 32, keep=False)
+    _, _, y, ey = p.want()
+    A, B, b, R, C, _ = p.handles()
+    sl.gemm_bias_act(p.alpha, A, B, b, p.act, p.beta, R, R)
+    within(p.R, y, ey)
+    # beta = 0 reads no residual, alpha = 0 no operand, k = 0 has none
+    p = Product(dt, dev, 40, 24, 32, keep=False, beta=0.0)
+    p.R.fill_(nan)
+    A, B, b, R, C, _ = p.handles()
+    sl.gemm_bias_act(p.alpha, A, B, b, p.act, 0.0, R, C)
+    assert torch.isfinite(p.C).all()
+    p.A.fill_(nan)
+    sl.gemm_bias_act(0.0, A, B, b, "identity", 0.0, None, C)
+    assert torch.equal(p.C, p.b.expand(40, 24))
+    e = torch.empty(0, 40, dtype=dt, device=dev).t()
+    f = torch.empty(24, 0, dtype=dt, device=dev).t()
+    sl.gemm_bias_act(1.0, mat(e), mat(f), b, "identity", 0.0, None, C)
+    assert torch.equal(p.C, p.b.expand(40, 24))
+    # no column, no row
+    g = torch.empty(0, 32, dtype=dt, device=dev).t()
+    h = torch.empty(0, 40, dtype=dt, device=dev).t()
+    sl.gemm_bias_act(1.0, A, mat(g), b, "relu", 0.0, None, mat(h))
+    # a NaN or an infinity reaches its own column, and no other
+    q = Product(dt, dev, 40, 24, 32, keep=False, act="relu", res=False)
+    q.B[3, 5] = nan
+    q.B[7, 9] = float("inf")
+    A, B, b, _, C, _ = q.handles()
+    sl.gemm_bias_act(1.0, A, B, b, "relu", 0.0, None, C)
+    assert torch.isnan(q.C[:, 5]).all()
+    assert (q.C[:, 9].isinf() | (q.C[:, 9] == 0) | q.C[:, 9].isnan()).all()
+    rest = [j for j in range(24) if j not in (5, 9)]
+    assert torch.isfinite(q.C[:, rest]).all()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_activation_far(dev, dt, act):
+    """Far arguments: 0 on the left and z on the right, infinities included, no 0 inf."""
+    big = float("inf")
+    z = torch.tensor([-big, -6e4, -1e3, -130.0, 0.0, 130.0, 1e3, 6e4, big], dtype=torch.float64)
+    one = torch.ones(1, 1, dtype=dt, device=dev)
+    Z = z.to(dt).to(dev)[:, None]
+    C = torch.empty(1, 9, dtype=dt, device=dev).t()
+    sl.gemm_bias_act(0.0, mat(Z), mat(one), mat(Z), act, 0.0, None, mat(C))
+    want = Z.double().cpu() if act == "identity" else Z.double().cpu().clamp(min=0)
+    # at -130 the largest left tail is silu's, 130 e^-130 = 4.6e-55, which float64 still holds
+    assert torch.allclose(C.double().cpu(), want, rtol=0, atol=1e-54)
+    D = torch.empty(1, 9, dtype=dt, device=dev).t()
+    G = torch.ones(1, 9, dtype=dt, device=dev).t()
+    sl.gemm_bias_act_grad(1.0, mat(Z), mat(one), act, mat(Z), mat(G), mat(D), None, None)
+    slope = torch.ones(9, 1) if act == "identity" else (Z.cpu() > 0).double()
+    keep = [i for i in range(9) if i != 4]
+    assert torch.allclose(D.double().cpu()[keep], slope.double()[keep], rtol=0, atol=1e-54)
+
+
+# ---------------------------------------------------------------- gradients
+def grad_call(p, act, which="ABb", bias=1, swap=False, dev_t=lambda t: t):
+    """gemm_bias_act_grad on Product p's operands with its Z and R as Z and dC."""
+    dt, dev, m, n, k = p.dt, p.dev, p.m, p.n, p.k
+    dA = cm(*p.A.shape, dt, 9, dev) if "A" in which else None
+    dB = cm(*p.B.shape, dt, 9, dev) if "B" in which else None
+    db = (cm(m, 1, dt, 9, dev) if bias == 1 else cm(1, n, dt, 9, dev)) if "b" in which else None
+    A, B, _, G, _, Z = p.handles()
+    sl.gemm_bias_act_grad(p.alpha, A, B, act, Z, G, None if dA is None else mat(dA, p.ta == "T"),
+                          None if dB is None else mat(dB, p.tb == "T"), None if db is None else mat(db))
+    a, b, g, z = (x.double() for x in (p.A, p.B, p.R, p.Z))
+    a, b = (a.t() if p.ta == "T" else a), (b.t() if p.tb == "T" else b)
+    dz = g * act64(act, z)[1]
+    u, w = u_of(dt), w_of(dt)
+    # a slope is a sum p + z p' of terms of up to 1 + |z|, each off by a few w of
+    # itself: the sum passes 0, its error does not, so that it counts relative to
+    # the terms; the rounding of dZ to the type counts relative to dZ
+    own = 32 * w * (1 + z.abs()) * g.abs() * (act != "identity") + tiny(dt)
+    f = own + (0 if act == "identity" else u) * dz.abs()
+    al = abs(p.alpha)
+    if dA is not None:
+        bt = b.t().contiguous()
+        want, e = p.alpha * (dz @ bt), al * (f @ bt.abs() + (n + 4) * w * (dz.abs() @ bt.abs())) + tiny(dt)
+        within(dA.t() if p.ta == "T" else dA, want, e + u * (want.abs() + e))
+    if dB is not None:
+        at = a.t().contiguous()
+        want, e = p.alpha * (at @ dz), al * (at.abs() @ f + (m + 4) * w * (at.abs() @ dz.abs())) + tiny(dt)
+        within(dB.t() if p.tb == "T" else dB, want, e + u * (want.abs() + e))
+    if db is not None:
+        d = 1 if bias == 1 else 0
+        want = dz.sum(d, keepdim=True)
+        e = own.sum(d, keepdim=True) + (n if d else m) * w * dz.abs().sum(d, keepdim=True) + tiny(dt)
+        within(db, want, e + u * (want.abs() + e))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT"])
+def test_product_grad(dev, dt, act, ta, tb):
+    for (m, n, k) in [(1, 1, 1), (48, 1, 40), (70, 33, 50)]:
+        grad_call(Product(dt, dev, m, n, k, ta, tb), act)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("which", ["A", "B", "b", "Bb"])
+@pytest.mark.parametrize("bias", [1, 2])
+def test_product_grad_parts(dev, dt, which, bias):
+    for act in ("identity", "gelu"):
+        grad_call(Product(dt, dev, 72, 520, 24, pad=3), act, which, bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1503, 777, 1001), (1024, 2048, 512), (4000, 3, 640), (600, 5000, 128)])
+def test_product_grad_sizes(dt, m, n, k):
+    grad_call(Product(dt, "cuda", m, n, k), "gelu_tanh")
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_product_grad_no_tokens(dev):
+    """A batch without tokens: zero gradients of weight and bias."""
+    dt = torch.bfloat16
+    A, dA = cm(32, 16, dt, 1, dev), cm(32, 16, dt, 2, dev)
+    B, Z = torch.empty(0, 32, dtype=dt, device=dev).t(), torch.empty(0, 16, dtype=dt, device=dev).t()
+    db, dB = cm(16, 1, dt, 3, dev), torch.empty_like(B)
+    sl.gemm_bias_act_grad(1.0, mat(A, True), mat(B), "gelu", mat(Z), mat(Z.clone()), mat(dA, True), mat(dB), mat(db))
+    assert (dA == 0).all() and (db == 0).all()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_grad_differences(dev, act):
+    """Both backward passes against central differences of the forward calls:
+    with h = 1e-4 those are off by h^2 f''' / 6 and 2^-52 f / h, far below 1e-6."""
+    dt = torch.float64
+    m, n, k, h = 12, 7, 9, 1e-4
+    t = {x: cm(*s, dt, i, dev) for i, (x, s) in enumerate(dict(
+        A=(k, m), A2=(k, m), B=(k, n), b=(m, 1), G=(m, n), R=(m, n)).items())}
+    C, Z1, Z2 = (cm(m, n, dt, 50 + i, dev) for i in range(3))
+    M = {x: mat(v, x in ("A", "A2")) for x, v in t.items()}
+
+    def plain():
+        sl.gemm_bias_act(0.7, M["A"], M["B"], M["b"], act, 0.5, M["R"], mat(C), mat(Z1))
+        return float((C * t["G"]).sum())
+
+    def gated():
+        sl.gemm_gated(M["A"], M["A2"], M["B"], act, mat(C), mat(Z1), mat(Z2))
+        return float((C * t["G"]).sum())
+
+    def slope(f, x, i, j):
+        v = float(t[x][i, j])
+        t[x][i, j] = v + h
+        up = f()
+        t[x][i, j] = v - h
+        down = f()
+        t[x][i, j] = v
+        return (up - down) / (2 * h)
+
+    d = {x: cm(*t[x].shape, dt, 60, dev) for x in ("A", "A2", "B", "b")}
+    plain()
+    sl.gemm_bias_act_grad(0.7, M["A"], M["B"], act, mat(Z1), M["G"], mat(d["A"], True), mat(d["B"]), mat(d["b"]))
+    for x in ("A", "B", "b"):
+        for (i, j) in [(0, 0), (t[x].shape[0] - 1, t[x].shape[1] - 1), (t[x].shape[0] // 2, 0)]:
+            assert abs(slope(plain, x, i, j) - float(d[x][i, j])) < 1e-6
+    gated()
+    sl.gemm_gated_grad(M["A"], M["A2"], M["B"], act, mat(Z1), mat(Z2), M["G"], mat(d["A"], True), mat(d["A2"], True),
+                       mat(d["B"]))
+    for x in ("A", "A2", "B"):
+        for (i, j) in [(0, 0), (t[x].shape[0] - 1, t[x].shape[1] - 1), (t[x].shape[0] // 2, 0)]:
+            assert abs(slope(gated, x, i, j) - float(d[x][i, j])) < 1e-6
+
+
+# -------------------------------------------------------------------- gated
+class Gated:
+    def __init__(self, dt, dev, m, n, k, ta="T", tb="N", act="silu", pad=0, off=0):
+        self.dt, self.dev, self.m, self.n, self.k, self.ta, self.tb, self.act = dt, dev, m, n, k, ta, tb, act
+        std = 1 / math.sqrt(max(k, 1))
+        shape = (k, m) if ta == "T" else (m, k)
+        self.A1, self.A2 = cm(*shape, dt, 1, dev, std, pad, off), cm(*shape, dt, 2, dev, std, pad, off)
+        self.B = cm(*((n, k) if tb == "T" else (k, n)), dt, 3, dev, 1.0, pad, off)
+        self.C, self.Z1, self.Z2 = (cm(m, n, dt, 4 + i, dev, 1.0, pad, off) for i in range(3))
+        self.G = cm(m, n, dt, 7, dev, 1.0, pad, off)
+
+    def dense(self):
+        a1, a2, b = self.A1.double(), self.A2.double(), self.B.double()
+        if self.ta == "T":
+            a1, a2 = a1.t().contiguous(), a2.t().contiguous()
+        return a1, a2, (b.t().contiguous() if self.tb == "T" else b)
+
+    def handles(self):
+        return [mat(self.A1, self.ta == "T"), mat(self.A2, self.ta == "T"), mat(self.B, self.tb == "T")]
+
+    def want(self):
+        a1, a2, b = self.dense()
+        w, u = w_of(self.dt), u_of(self.dt)
+        z1, z2 = a1 @ b, a2 @ b
+        e1, e2 = ((self.k + 4) * w * (a.abs() @ b.abs()) + tiny(self.dt) for a in (a1, a2))
+        v = act64(self.act, z1)[0]
+        ev = 1.13 * e1 + act_bound(z1, w)
+        y = v * z2
+        ey = ev * z2.abs() + e2 * v.abs() + ev * e2 + 2 * w * y.abs() + tiny(self.dt)
+        return [(z1, e1 + u * (z1.abs() + e1)), (z2, e2 + u * (z2.abs() + e2)), (y, ey + u * (y.abs() + ey))]
+
+    def check(self):
+        (z1, e1), (z2, e2), (y, ey) = self.want()
+        sl.gemm_gated(*self.handles(), self.act, mat(self.C), mat(self.Z1), mat(self.Z2))
+        within(self.C, y, ey)
+        within(self.Z1, z1, e1)
+        within(self.Z2, z2, e2)
+        self.C.fill_(0)
+        sl.gemm_gated(*self.handles(), self.act, mat(self.C))
+        within(self.C, y, ey)
+
+    def check_grad(self, which=("A1", "A2", "B")):
+        dt, u, w = self.dt, u_of(self.dt), w_of(self.dt)
+        a1, a2, b = self.dense()
+        z1, z2, g = self.Z1.double(), self.Z2.double(), self.G.double()
+        d = {x: cm(*getattr(self, x).shape, dt, 9, self.dev) if x in which else None for x in ("A1", "A2", "B")}
+        t = {"A1": self.ta == "T", "A2": self.ta == "T", "B": self.tb == "T"}
+        sl.gemm_gated_grad(*self.handles(), self.act, mat(self.Z1), mat(self.Z2), mat(self.G),
+                           *(None if d[x] is None else mat(d[x], t[x]) for x in ("A1", "A2", "B")))
+        v, s = act64(self.act, z1)
+        d1, d2 = g * z2 * s, g * v
+        one = u + 32 * w * (1 + z1.abs().max())
+        bt = b.t().contiguous()
+        # a slope's own error is relative to 1, not to itself (it passes 0)
+        f1, f2 = one * d1.abs() + 32 * w * (g * z2).abs() + tiny(dt), one * d2.abs() + 32 * w * (g * z1).abs() + tiny(dt)
+        wants = {"A1": (d1 @ bt, f1 @ bt.abs() + (self.n + 4) * w * (d1.abs() @ bt.abs())),
+                 "A2": (d2 @ bt, f2 @ bt.abs() + (self.n + 4) * w * (d2.abs() @ bt.abs())),
+                 "B": (a1.t().contiguous() @ d1 + a2.t().contiguous() @ d2,
+                       sum(a.abs().t().contiguous() @ f + (2 * self.m + 4) * w * (a.abs().t().contiguous() @ x.abs())
+                           for a, x, f in ((a1, d1, f1), (a2, d2, f2))))}
+        for x in which:
+            want, e = wants[x]
+            e = e + tiny(dt)
+            within(d[x].t() if t[x] else d[x], want, e + u * (want.abs() + e))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT", "TT"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (64, 1, 128), (131, 67, 75)])
+def test_gated(dev, dt, ta, tb, m, n, k):
+    Gated(dt, dev, m, n, k, ta, tb).check()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("pad,off", [(0, 0), (8, 8), (3, 1)])
+def test_gated_strides(dev, dt, act, pad, off):
+    g = Gated(dt, dev, 70, 33, 66, act=act, pad=pad, off=off)
+    g.check_grad()
+    g.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN"])
+@pytest.mark.parametrize("m,n,k", [(1801, 3700, 200), (2048, 4096, 256), (700, 1300, 520), (2100, 17, 4100), (5000, 1, 640)])
+def test_gated_sizes(dt, ta, tb, m, n, k):
+    Gated(dt, "cuda", m, n, k, ta, tb).check()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT"])
+def test_gated_grad(dev, dt, ta, tb):
+    for (m, n, k) in [(1, 1, 1), (48, 1, 40), (70, 33, 50)]:
+        Gated(dt, dev, m, n, k, ta, tb).check_grad()
+    for which in (("A1",), ("A2",), ("B",), ("A1", "B")):
+        Gated(dt, dev, 33, 20, 40, ta, tb).check_grad(which)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1503, 777, 500), (1024, 2048, 512), (2560, 515, 1024), (3000, 2, 640)])
+def test_gated_grad_sizes(dt, m, n, k):
+    Gated(dt, "cuda", m, n, k, act="gelu").check_grad()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", [torch.float16, torch.float32])
+def test_gated_mixed_orientation(dev, dt):
+    """Operands, outputs and stored products of either orientation."""
+    g = Gated(dt, dev, 40, 24, 32)
+    (z1, e1), (z2, e2), (y, ey) = g.want()
+    turn = lambda x: torch.empty(x.shape[0], x.shape[1], dtype=dt, device=dev).t()      # noqa: E731
+    Ct, Z1t, A2t = turn(g.C), turn(g.Z1), turn(g.A2)
+    A2t.copy_(g.A2.t())
+    A1, A2, B = g.handles()
+    sl.gemm_gated(A1, mat(A2t), B, g.act, mat(Ct, True), mat(Z1t, True), mat(g.Z2))
+    within(Ct.t(), y, ey)
+    within(Z1t.t(), z1, e1)
+    within(g.Z2, z2, e2)
+    # the backward pass from a transposed Z1 is that from Z1
+    g.Z1.copy_(Z1t.t())
+    d = [[torch.empty_like(x) for x in (g.A1, g.A2, g.B)] for _ in range(2)]
+    for k, (z, a2) in enumerate(((mat(Z1t, True), mat(A2t)), (mat(g.Z1), A2))):
+        sl.gemm_gated_grad(A1, a2, B, g.act, z, mat(g.Z2), mat(g.G), mat(d[k][0], True), mat(d[k][1], True), mat(d[k][2]))
+    for x, v in zip(*d):
+        assert torch.equal(x, v)
+
+
+# ----------------------------------------------------------------- clipping
+def clip_case(dt, dev, shapes, std=0.02, pad=0, off=0):
+    return [cm(m, n, dt, 100 + i, dev, std, pad, off) for i, (m, n) in enumerate(shapes)]
+
+
+def clip_want(xs, limit):
+    wide = lambda x: torch.view_as_real(x.contiguous()).double() if x.is_complex() else x.double()      # noqa: E731
+    s = math.sqrt(math.fsum(float((wide(x) ** 2).sum()) for x in xs))
+    return s, min(1.0, limit / s) if s else 1.0
+
+
+CLIP_TYPES = [(torch.bfloat16,) * 2, (torch.bfloat16, torch.float32), (torch.float16,) * 2, (torch.float16, torch.float32),
+              (torch.float32,) * 2, (torch.float64,) * 2, (torch.complex64,) * 2, (torch.complex128,) * 2]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt,out", CLIP_TYPES)
+@pytest.mark.parametrize("pad,off", [(0, 0), (3, 1), (8, 0)])
+@pytest.mark.parametrize("limit", [0.25, 1e6, 0.0])
+def test_clip(dev, dt, out, pad, off, limit):
+    if dt.is_complex:
+        mk = lambda i, m, n: torch.complex(cm(m, n, dt.to_real(), i, dev, .02), cm(m, n, dt.to_real(), i + 50, dev, .02))  # noqa: E731
+        xs = [mk(i, m, n).t().contiguous().t() for i, (m, n) in enumerate([(30, 20), (1, 7), (200, 1)])]
+    else:
+        xs = clip_case(dt, dev, [(300, 200), (1, 17), (65, 1), (33, 130), (1, 1)], pad=pad, off=off)
+    ys = [cm(*x.shape, out.to_real() if out.is_complex else out, 1, dev, 1.0, pad) for x in xs]
+    if out.is_complex:
+        ys = [torch.zeros_like(x) for x in xs]
+    s, f = clip_want(xs, limit)
+    got = sl.clip_norm(limit, [mat(x) for x in xs], [mat(y) for y in ys])
+    n = sum(x.numel() for x in xs)
+    assert got.dtype == torch.float64 and abs(float(got) - s) <= (n + 4) * 2.0 ** -53 * s
+    # the factor is rounded to the sums' type, the product again, then the store
+    rt = out.to_real() if out.is_complex else out
+    rel = u_of(rt) + 3 * w_of(rt) + (n + 4) * 2.0 ** -53
+    for x, y in zip(xs, ys):
+        a, b = (torch.view_as_real(v.contiguous()).double() if v.is_complex() else v.double() for v in (x, y))
+        assert ((b - a * f).abs() <= rel * (a * f).abs() + tiny(rt)).all()
+        if limit == 1e6 and dt == out:
+            assert torch.equal(x, y)
+    # in place, the same values
+    if dt == out:
+        sl.clip_norm(limit, [mat(x) for x in xs])
+        for x, y in zip(xs, ys):
+            assert torch.equal(x, y)
+            if pad and x.shape[1] > 1 and not dt.is_complex:
+                m = x.shape[0]
+                assert torch.isnan(x.as_strided((pad, x.shape[1]), (1, m + pad), x.storage_offset() + m)).all()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("count", [0, 1, 48, 49, 200])
+def test_clip_many(dev, count):
+    """More matrices than one launch describes, empty ones among them."""
+    xs = clip_case(torch.float32, dev, [((7 * i) % 23 if i % 9 else 0, 1 + i % 11) for i in range(count)], 1.0)
+    s, f = clip_want(xs, 2.0)
+    want = [x.double() * f for x in xs]
+    got = sl.clip_norm(2.0, [mat(x) for x in xs])
+    assert abs(float(got) - s) <= 1e-12 * max(s, 1)
+    for x, w in zip(xs, want):
+        assert ((x.double() - w).abs() <= 2.0 ** -22 * w.abs()).all()
+    assert abs(sl.global_norm([mat(x) for x in xs]) - min(s, 2.0)) <= 1e-6 * max(1, s)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_clip_extremes(dev):
+    """Squares outside a type's range, and norms that are not finite."""
+    for dt, v in ((torch.float32, 1e30), (torch.float32, 1e-30), (torch.float64, 1e300), (torch.float64, 1e-300),
+                  (torch.float64, 1e140), (torch.float64, 5e-324)):
+        x = torch.full((1000,), v, dtype=dt, device=dev)[:, None]
+        want = float(x[0, 0]) * math.sqrt(1000)
+        assert abs(sl.global_norm([mat(x)]) - want) <= 1e-12 * want
+    x = torch.tensor([3e200, 4e200, 1.0, 1e-200], dtype=torch.float64, device=dev)[:, None]
+    assert abs(sl.global_norm([mat(x)]) - 5e200) <= 1e188
+    x = torch.tensor([3e-170, 4e-170, 1e-300], dtype=torch.float64, device=dev)[:, None]
+    assert abs(sl.global_norm([mat(x)]) - 5e-170) <= 1e-182
+    for bad in (float("inf"), float("nan")):
+        for dt in (torch.float32, torch.bfloat16, torch.float64):
+            x = cm(64, 40, dt, 1, dev)
+            x[5, 6] = bad
+            y, z = x.clone(), cm(64, 40, dt, 2, dev)
+            s = float(sl.clip_norm(1.0, [mat(x)]))
+            assert (s != s) if bad != bad else s == bad
+            assert torch.equal(x.view(torch.uint8) if False else x.nan_to_num(7.0), y.nan_to_num(7.0))
+            sl.clip_norm(1.0, [mat(x)], [mat(z)])
+            assert torch.equal(z.nan_to_num(7.0), y.nan_to_num(7.0))
+    z = torch.zeros(16, 16, device=dev).t()
+    assert float(sl.clip_norm(0.0, [mat(z)])) == 0.0 and (z == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32, torch.float64])
+def test_clip_sizes(dt):
+    xs = clip_case(dt, "cuda", [(4096, 1024), (4099, 513), (100003, 1), (5, 50000)])
+    s, f = clip_want(xs, 1.0)
+    want = [x.double() * f for x in xs]
+    got = sl.clip_norm(1.0, [mat(x) for x in xs])
+    assert abs(float(got) - s) <= 1e-9 * s
+    for x, w in zip(xs, want):
+        assert ((x.double() - w).abs() <= (u_of(dt) + 4 * w_of(dt) + 1e-9 * (dt == torch.float64)) * w.abs() + tiny(dt)).all()
+
+
+# ------------------------------------------------------------------- copies
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("src", TYPES)
+@pytest.mark.parametrize("dst", TYPES)
+@pytest.mark.parametrize("trans", "NT")
+def test_copy_half(dev, src, dst, trans):
+    """Precision conversion of sl.copy to and from the 16-bit types, ties to even."""
+    if src not in HALF and dst not in HALF:
+        pytest.skip("the other kernels")
+    x = cm(67, 45, src, 3, dev)
+    x[0, :6] = torch.tensor([1 + 2.0 ** -9, 1 + 3 * 2.0 ** -9, 1 + 2.0 ** -12, 65519.0, 1e-7, -0.0], dtype=torch.float64).to(src)
+    y = cm(*((67, 45) if trans == "N" else (45, 67)), dst, 4, dev)
+    ops.gecopy(x, y, trans=trans)
+    want = x if trans == "N" else x.t()
+    assert torch.equal(y.cpu(), want.cpu().to(dst))
+    if trans == "N":
+        A, B = mat(x), mat(cm(67, 45, dst, 5, dev))
+        sl.copy(A, B)
+        assert torch.equal(B.to_dense().cpu(), x.cpu().to(dst))
+
+
+# ----------------------------------------------------------------- refusals
+@pytest.mark.parametrize("dev", DEVS)
+def test_refusals(dev):
+    f = torch.float32
+    A, B, C = (mat(cm(m, n, f, 1, dev)) for (m, n) in ((16, 8), (8, 12), (16, 12)))
+    b, R = mat(cm(16, 1, f, 2, dev)), mat(cm(16, 12, f, 3, dev))
+    ok = lambda **k: sl.gemm_bias_act(*[{**dict(alpha=1.0, A=A, B=B, bias=b, act="relu", beta=1.0, R=R, C=C), **k}[x]  # noqa: E731
+                                        for x in ("alpha", "A", "B", "bias", "act", "beta", "R", "C")])
+    ok()
+    for bad in (dict(A=mat(cm(16, 9, f, 1, dev))), dict(B=mat(cm(8, 11, f, 1, dev))), dict(R=mat(cm(16, 11, f, 1, dev))),
+                dict(bias=mat(cm(12, 1, f, 1, dev))), dict(bias=mat(cm(16, 2, f, 1, dev))), dict(act="tanh"), dict(act=None),
+                dict(A=mat(cm(16, 8, torch.float64, 1, dev))), dict(R=mat(cm(16, 12, torch.bfloat16, 1, dev))),
+                dict(C=A), dict(R=C.transpose())):
+        with pytest.raises(SlateError):
+            ok(**bad)
+    with pytest.raises(SlateError):
+        sl.gemm_bias_act(1.0, A, B, b, "relu", 1.0, R, C, C)
+    square = mat(cm(8, 8, f, 1, dev))
+    for call in (lambda: sl.gemm_bias_act(1.0, square, square, None, "relu", 0.0, None, square),
+                 lambda: sl.gemm_gated(square, square, square, "relu", square),
+                 lambda: sl.gemm_gated(A, A, B, "relu", C, R, R),
+                 lambda: sl.gemm_gated_grad(A, A, B, "relu", None, R, C, None, None, None),
+                 lambda: sl.gemm_bias_act_grad(1.0, A, B, "relu", None, C, mat(cm(16, 8, f, 1, dev)), None, None),
+                 lambda: sl.gemm_bias_act_grad(1.0, A, B, "relu", R, C, A, None, None)):
+        with pytest.raises(SlateError):
+            call()
+    z = [mat(torch.zeros(4, 4, dtype=torch.complex64, device=dev).t()) for _ in range(3)]
+    with pytest.raises(SlateError):
+        sl.gemm_bias_act(1.0, z[0], z[1], None, "relu", 0.0, None, z[2])
+    H = sl.HermitianMatrix.fromLAPACK(sl.Uplo.Lower, 8, cm(8, 8, f, 1, dev))
+    with pytest.raises(SlateError):
+        sl.gemm_bias_act(1.0, H, square, None, "relu", 0.0, None, mat(cm(8, 8, f, 2, dev)))
+    spread = torch.zeros(8, 1, dtype=f, device=dev).expand(8, 4)
+    with pytest.raises(SlateError):
+        sl.gemm_bias_act(1.0, square, sl.Matrix.fromLAPACK(8, 4, spread.as_strided((8, 4), (1, 0)), nb=8), None, "relu", 0.0,
+                         None, mat(cm(8, 4, f, 2, dev)))
+    for call in (lambda: sl.clip_norm(-1.0, [A]), lambda: sl.clip_norm(float("nan"), [A]), lambda: sl.clip_norm(1.0, A),
+                 lambda: sl.clip_norm(1.0, [A, A]), lambda: sl.clip_norm(1.0, [A, B], [A]),
+                 lambda: sl.clip_norm(1.0, [A], [B]), lambda: sl.clip_norm(1.0, [A, mat(cm(4, 4, torch.float64, 1, dev))]),
+                 lambda: sl.clip_norm(1.0, [mat(cm(4, 4, torch.float64, 1, dev))], [mat(cm(4, 4, f, 1, dev))]),
+                 lambda: sl.clip_norm(1.0, [H]), lambda: sl.clip_norm(1.0, [A], [B.transpose()])):
+        with pytest.raises(SlateError):
+            call()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_blocks_of_one_matrix(dev):
+    """Disjoint blocks of one storage are operands and outputs of one call."""
+    big = torch.zeros(40, 64, dtype=torch.float32, device=dev).t()
+    big.copy_(torch.randn(64, 40, generator=torch.Generator().manual_seed(1)).to(dev))
+    M = sl.Matrix.fromLAPACK(64, 40, big, nb=8)
+    A, B, C = M.slice(0, 31, 0, 15), M.slice(32, 47, 0, 23), M.slice(32, 63, 16, 39)
+    with pytest.raises(SlateError):                      # B's columns 16.. lie in C
+        sl.gemm_bias_act(1.0, A, B, None, "relu", 0.0, None, C)
+    B = M.slice(0, 15, 16, 39)
+    keep = big.clone()
+    sl.gemm_bias_act(1.0, A, B, None, "relu", 0.0, None, C)
+    want = (keep[:32, :16].double() @ keep[:16, 16:].double()).clamp(min=0)
+    S = keep[:32, :16].double().abs() @ keep[:16, 16:].double().abs()
+    within(big[32:, 16:], want, 24 * 2.0 ** -24 * S + 2.0 ** -24 * want)
+    assert torch.equal(big[:32], keep[:32]) and torch.equal(big[32:, :16], keep[32:, :16])
+
+
+# ------------------------------------------------------------------ together
+def block(dt, dev, t=45, d=72, f=104, seed=0):
+    """One feed-forward block's step: gated projection, projection back onto
+    the residual, both backward passes, and the clipping of all gradients."""
+    s = dict(x=cm(d, t, dt, seed + 1, dev), wg=cm(d, f, dt, seed + 2, dev, d ** -.5), wu=cm(d, f, dt, seed + 3, dev, d ** -.5),
+             wd=cm(f, d, dt, seed + 4, dev, f ** -.5), b=cm(d, 1, dt, seed + 5, dev), g=cm(d, t, dt, seed + 6, dev))
+    for n, (a, b) in dict(h=(f, t), z1=(f, t), z2=(f, t), y=(d, t), dh=(f, t), dx=(d, t)).items():
+        s[n] = cm(a, b, dt, 20, dev)
+    for n in ("wg", "wu", "wd", "b"):
+        s["d" + n] = torch.empty_like(s[n])
+    H = {n: mat(v, n in ("wg", "wu", "wd", "dwg", "dwu", "dwd")) for n, v in s.items()}
+
+    def step():
+        sl.gemm_gated(H["wg"], H["wu"], H["x"], "silu", H["h"], H["z1"], H["z2"])
+        sl.gemm_bias_act(1.0, H["wd"], H["h"], H["b"], "identity", 1.0, H["x"], H["y"])
+        sl.gemm_bias_act_grad(1.0, H["wd"], H["h"], "identity", None, H["g"], H["dwd"], H["dh"], H["db"])
+        sl.gemm_gated_grad(H["wg"], H["wu"], H["x"], "silu", H["z1"], H["z2"], H["dh"], H["dwg"], H["dwu"], H["dx"])
+        return sl.clip_norm(0.5, [H[n] for n in ("dwg", "dwu", "dwd", "db")])
+
+    return s, step
+
+
+OUT = ("y", "dx", "dwg", "dwu", "dwd", "db")
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+def test_block(dev, dt):
+    s, step = block(dt, dev)
+    norm = step()
+    v = {n: x.double().detach().clone().requires_grad_(n in ("x", "wg", "wu", "wd", "b"))
+         for n, x in s.items() if n in ("x", "wg", "wu", "wd", "b", "g")}
+    x = v["x"]
+    h = torch.nn.functional.silu(v["wg"].t() @ x) * (v["wu"].t() @ x)
+    y = v["wd"].t() @ h + v["b"] + x
+    (y * v["g"]).sum().backward()
+    want = dict(y=y.detach(), dwg=v["wg"].grad, dwu=v["wu"].grad, dwd=v["wd"].grad, db=v["b"].grad, dx=x.grad - v["g"])
+    total = math.sqrt(sum(float((want[n] ** 2).sum()) for n in ("dwg", "dwu", "dwd", "db")))
+    # at most six roundings to the type (h, z1, z2, dh, dz, the gradient) and the
+    # sums' own errors lie on a path, each of relative 2-norm at most u (w (k + 4))
+    tol = 8 * u_of(dt) + 8 * (104 + 4) * w_of(dt)
+    assert abs(float(norm) - total) <= tol * total
+    for n in OUT:
+        ref = want[n] * (min(1, 0.5 / total) if n in ("dwg", "dwu", "dwd", "db") else 1)
+        assert float((s[n].double() - ref).norm()) <= 2 * tol * float(ref.norm()), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_block_stream_and_repeat(dt):
+    """Another stream, and the same bits on every run."""
+    s, step = block(dt, "cuda", 300, 256, 520)
+    n0 = step()
+    first = {n: s[n].clone() for n in OUT}
+    side = torch.cuda.Stream()
+    for n in OUT:
+        s[n].fill_(0)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        n1 = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert float(n0) == float(n1)
+    for n in OUT:
+        assert torch.equal(s[n], first[n]), n
+
+
+@pytest.mark.gpu
+def test_block_two_streams():
+    """Two steps at once on two streams, each with its own workspaces."""
+    a, b = block(torch.bfloat16, "cuda", 300, 256, 520), block(torch.bfloat16, "cuda", 300, 256, 520, seed=40)
+    want = []
+    for s, step in (a, b):
+        step()
+        want.append({n: s[n].clone() for n in OUT})
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for (s, step), st in zip((a, b), sides):
+            with torch.cuda.stream(st):
+                step()
+    torch.cuda.synchronize()
+    for (s, _), w in zip((a, b), want):
+        for n in OUT:
+            assert torch.equal(s[n], w[n]), n
+
+
+@pytest.mark.gpu
+def test_block_graphs():
+    """Two captured steps that share a pool, replayed with eager work between."""
+    a, b = block(torch.bfloat16, "cuda", 1, 256, 520), block(torch.bfloat16, "cuda", 77, 256, 520, seed=40)
+    want = []
+    for s, step in (a, b):
+        step()
+        want.append({n: s[n].clone() for n in OUT})
+    torch.cuda.synchronize()
+    graphs, pool = [], torch.cuda.graph_pool_handle()
+    for s, step in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            step()
+        graphs.append(g)
+    for _ in range(3):
+        for (s, step), g, w in zip((a, b), graphs, want):
+            for n in OUT:
+                s[n].fill_(float("nan"))
+            g.replay()
+            torch.cuda.synchronize()
+            for n in OUT:
+                assert torch.equal(s[n], w[n]), n
+        a[1]()
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_no_host_sync():
+    s, step = block(torch.bfloat16, "cuda", 300, 256, 520)
+    step()
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        step()
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
