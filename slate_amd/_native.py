@@ -76,9 +76,14 @@ def code(dtype) -> str:
 REAL_CODE = {torch.bfloat16: 'b', torch.float16: 'h', torch.float32: 's', torch.float64: 'd'}
 
 
+# torch's own lookup of the handle (a Stream object costs ten times as much)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def raw_stream(t: torch.Tensor) -> int:
     """The current stream of t's own device (0 for host tensors)."""
-    return torch.cuda.current_stream(t.device).cuda_stream if t.is_cuda else 0
+    return _raw_stream(t.device.index) if t.is_cuda else 0
 
 
 def hip_available() -> bool:

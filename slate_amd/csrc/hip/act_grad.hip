@@ -16,16 +16,16 @@ constexpr int AG_WAVES = 4;
 
 // grid.x: blocks of 64 E rows (bias_mode 0, 1); grid.y: chunks of columns
 template <typename T, bool GATED>
-__global__ void __launch_bounds__(64 * AG_WAVES) act_grad_rows_kernel(ActGradArgs a, i64 cols, bool vec) {
+__global__ void __launch_bounds__(64 * AG_WAVES) act_grad_rows_kernel(ActGradArgs a, i64 cols) {
     using R = typename ga_traits<T>::acc;
     constexpr int E = 16 / sizeof(T);
     constexpr bool FAST = sizeof(T) == 2;
-    typedef T vE __attribute__((ext_vector_type(E)));
+    using vE = ga_vec<T, E>;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const i64 m = ((i64)blockIdx.x * 64 + lane) * E;
     const int left = (int)max((i64)0, min((i64)E, a.m - m));
     const i64 n0 = (i64)blockIdx.y * cols, n1 = min(a.n, n0 + cols);
-    const bool wide = vec && left == E;
+    const bool wide = left == E;
     R sum[E];
     #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = R(0);
@@ -52,24 +52,43 @@ __global__ void __launch_bounds__(64 * AG_WAVES) act_grad_rows_kernel(ActGradArg
             for (int e = 0; e < E; ++e) if (e < left) x[e] = (T)v[e];
         }
     };
+    // UN columns' loads are in flight per wave
+    constexpr int UN = GATED ? 2 : 4;
+    auto column = [&](i64 n, const T* c, const T* z1, const T* z2) {
+        R d1[E], d2[E];
+        #pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const R g = (R)c[e];
+            R v = R(0), d = R(1);
+            if (a.Z1) ga_act_grad<FAST>(a.act, (R)z1[e], v, d);
+            if constexpr (GATED) { d1[e] = g * (R)z2[e] * d; d2[e] = g * v; }
+            else { d1[e] = g * d; d2[e] = R(0); }
+            sum[e] += d1[e];
+        }
+        if (a.dZ1) put(a.dZ1, n, d1);
+        if constexpr (GATED) put(a.dZ2, n, d2);
+    };
     if (left > 0)
-        for (i64 n = n0 + w; n < n1; n += AG_WAVES) {
-            T c[E], z1[E], z2[E];
-            R d1[E], d2[E];
-            get(a.dC, a.lddc, n, c);
-            if (a.Z1) get(a.Z1, a.ldz1, n, z1);
-            if constexpr (GATED) get(a.Z2, a.ldz2, n, z2);
+        for (i64 n = n0 + w; n < n1; n += AG_WAVES * UN) {
+            T c[UN][E], z1[UN][E], z2[UN][E];
             #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const R g = (R)c[e];
-                R v = R(0), d = R(1);
-                if (a.Z1) ga_act_grad<FAST>(a.act, (R)z1[e], v, d);
-                if constexpr (GATED) { d1[e] = g * (R)z2[e] * d; d2[e] = g * v; }
-                else { d1[e] = g * d; d2[e] = R(0); }
-                sum[e] += d1[e];
+            for (int u = 0; u < UN; ++u) {
+                const i64 nu = min(n + u * AG_WAVES, n1 - 1);
+                get(a.dC, a.lddc, nu, c[u]);
+                if (a.Z1) get(a.Z1, a.ldz1, nu, z1[u]);
+                if constexpr (GATED) get(a.Z2, a.ldz2, nu, z2[u]);
             }
-            if (a.dZ1) put(a.dZ1, n, d1);
-            if constexpr (GATED) put(a.dZ2, n, d2);
+            #pragma unroll 1
+            for (int u = 0; u < UN; ++u) {
+                // (one copy of the activations in the code: the vectors are picked by u)
+                T cu[E], zu[E], wu[E];
+                #pragma unroll
+                for (int q = 0; q < UN; ++q)
+                    if (q == u)
+                        #pragma unroll
+                        for (int e = 0; e < E; ++e) { cu[e] = c[q][e]; zu[e] = z1[q][e]; wu[e] = z2[q][e]; }
+                if (n + u * AG_WAVES < n1) column(n + u * AG_WAVES, cu, zu, wu);
+            }
         }
     if (a.bias_mode == 1) {
         __shared__ R red[AG_WAVES][64 * E];
@@ -107,14 +126,24 @@ __global__ void __launch_bounds__(256) act_grad_cols_kernel(ActGradArgs a, i64 r
     if (lane == 0) static_cast<R*>(a.part)[blockIdx.y * a.n + n] = s;
 }
 
+// 32 sums per workgroup, 8 threads along the chunks of each
 template <typename T>
 __global__ void __launch_bounds__(256) act_grad_join_kernel(const typename ga_traits<T>::acc* part, i64 len, int chunks,
                                                             void* db, i64 incb, bool wide) {
     using R = typename ga_traits<T>::acc;
-    const i64 i = (i64)blockIdx.x * 256 + threadIdx.x;
-    if (i >= len) return;
+    __shared__ R red[8][32];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const i64 i = (i64)blockIdx.x * 32 + x;
     R s = R(0);
-    for (int c = 0; c < chunks; ++c) s += part[c * len + i];
+    if (i < len) {
+        #pragma unroll 4
+        for (int c = y; c < chunks; c += 8) s += part[c * len + i];
+    }
+    red[y][x] = s;
+    __syncthreads();
+    if (y || i >= len) return;
+    #pragma unroll
+    for (int q = 1; q < 8; ++q) s += red[q][x];
     if (wide) static_cast<R*>(db)[i * incb] = s;
     else static_cast<T*>(db)[i * incb] = (T)s;
 }
@@ -126,27 +155,25 @@ __global__ void __launch_bounds__(256) act_grad_join_kernel(const typename ga_tr
 int act_grad_chunks(int bias_mode, int es, i64 m, i64 n) {
     const i64 other = bias_mode == 2 ? (n + 3) / 4 : (m + 64 * (16 / es) - 1) / (64 * (16 / es));
     const i64 most = bias_mode == 2 ? (m + 511) / 512 : (n + 15) / 16;
-    return (int)std::max<i64>(1, std::min<i64>(most, (2048 + other - 1) / std::max<i64>(1, other)));
+    return (int)std::max<i64>(1, std::min<i64>(most, (1024 + other - 1) / std::max<i64>(1, other)));
 }
 
 template <typename T> void act_grad(ActGradArgs a, hipStream_t s) {
     if (a.m <= 0 || a.n <= 0) return;
     const int ES = sizeof(T), chunks = act_grad_chunks(a.bias_mode, ES, a.m, a.n);
-    auto on = [&](const void* p, i64 ld) { return !p || ((uintptr_t)p % 16 == 0 && (ld * ES) % 16 == 0); };
-    const bool vec = on(a.dC, a.lddc) && on(a.Z1, a.ldz1) && on(a.Z2, a.ldz2) && on(a.dZ1, a.lddz) && on(a.dZ2, a.lddz);
     if (a.bias_mode == 2) {
         const i64 rows = (a.m + chunks - 1) / chunks;
         hipLaunchKernelGGL((act_grad_cols_kernel<T>), dim3((unsigned)((a.n + 3) / 4), chunks), dim3(256), 0, s, a, rows);
     } else {
         const i64 cols = (a.n + chunks - 1) / chunks, rb = 64 * (16 / ES);
         const dim3 grid((unsigned)((a.m + rb - 1) / rb), chunks);
-        if (a.Z2) hipLaunchKernelGGL((act_grad_rows_kernel<T, true>), grid, dim3(64 * AG_WAVES), 0, s, a, cols, vec);
-        else hipLaunchKernelGGL((act_grad_rows_kernel<T, false>), grid, dim3(64 * AG_WAVES), 0, s, a, cols, vec);
+        if (a.Z2) hipLaunchKernelGGL((act_grad_rows_kernel<T, true>), grid, dim3(64 * AG_WAVES), 0, s, a, cols);
+        else hipLaunchKernelGGL((act_grad_rows_kernel<T, false>), grid, dim3(64 * AG_WAVES), 0, s, a, cols);
     }
     HIP_LAUNCH_CHECK();
     if (a.bias_mode) {
         const i64 len = a.bias_mode == 1 ? a.m : a.n;
-        hipLaunchKernelGGL((act_grad_join_kernel<T>), dim3((unsigned)((len + 255) / 256)), dim3(256), 0, s,
+        hipLaunchKernelGGL((act_grad_join_kernel<T>), dim3((unsigned)((len + 31) / 32)), dim3(256), 0, s,
                            static_cast<const typename ga_traits<T>::acc*>(a.part), len, chunks, a.db, a.incb, a.wide);
         HIP_LAUNCH_CHECK();
     }
@@ -156,30 +183,5 @@ template void act_grad<__bf16>(ActGradArgs, hipStream_t);
 template void act_grad<_Float16>(ActGradArgs, hipStream_t);
 template void act_grad<float>(ActGradArgs, hipStream_t);
 template void act_grad<double>(ActGradArgs, hipStream_t);
-
-// The tile and the number of pieces of K, from sizes alone.
-GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k) {
-    if (m <= 0 || n <= 0) return {};
-    GemmActPlan p;
-    const i64 rows = mode == GA_GATED ? 2 * m : m, pairs = mode == GA_PAIR ? 2 : 1;
-    const int steps = (int)((k * es + 127) / 128) * (mode == GA_SUM ? 2 : 1);
-    auto tiles = [&](i64 bm, i64 bn) { return ((rows + bm - 1) / bm) * ((n + bn - 1) / bn) * pairs; };
-    i64 t;
-    if (n <= 16) { p.tile = 3; t = tiles(128, 16); }
-    else if (es == 2 && tiles(256, 256) >= 192) { p.tile = 0; t = tiles(256, 256); }
-    else if (tiles(128, 128) >= 128) { p.tile = 1; t = tiles(128, 128); }
-    else { p.tile = 2; t = tiles(64, 64); }
-    const i64 want = p.tile == 3 ? 1024 : 512;
-    if (t < want / 2 && steps >= 8) {
-        p.splits = (int)std::min<i64>(steps / 4, want / t);
-        p.per_split = (steps + p.splits - 1) / p.splits;
-        p.splits = (steps + p.per_split - 1) / p.per_split;
-    }
-    if (p.splits > 1) {
-        p.ldp = (m + 7) / 8 * 8;
-        p.bytes = (i64)p.splits * (mode == GA_GATED || mode == GA_PAIR ? 2 : 1) * n * p.ldp * (es == 8 ? 8 : 4);
-    }
-    return p;
-}
 
 }  // namespace slate_hip

@@ -35,7 +35,8 @@ std::vector<ClipMat> mats(const Mats& v) {
 }  // namespace
 
 void register_ffn(py::module& m) {
-    m.def("gemm_act_ws", [](int es, int mode, i64 mm, i64 n, i64 k) { return gemm_act_plan(es, mode, mm, n, k).bytes; });
+    // Launches and returns 0, or returns the bytes of workspace that the call
+    // wants where ws is 0 (nothing is launched then).
     m.def("gemm_act", [](char dt, int mode, char ta, char tb, i64 mm, i64 n, i64 k, double alpha,
                          uintptr_t A0, i64 lda0, uintptr_t A1, i64 lda1, uintptr_t B0, i64 ldb0, uintptr_t B1, i64 ldb1,
                          uintptr_t C0, i64 ldc0, uintptr_t C1, i64 ldc1, uintptr_t bias, i64 incb, int bias_mode,
@@ -51,12 +52,12 @@ void register_ffn(py::module& m) {
         a.bias = P(bias); a.incb = incb; a.bias_mode = bias_mode;
         a.R = P(R); a.ldr = ldr;
         a.part = W(ws);
+        i64 bytes = 0;
         real_dispatch(dt, [&](auto z) {
             using T = decltype(z);
-            const GemmActPlan p = gemm_act_plan(sizeof(T), mode, mm, n, k);
-            if (p.bytes && !ws) throw std::invalid_argument("gemm_act: workspace missing");
-            gemm_act<T>(a, ta, tb, p, S(st));
+            bytes = gemm_act<T>(a, ta, tb, S(st));
         });
+        return bytes;
     });
     m.def("act_grad_ws", [](char dt, int bias_mode, i64 mm, i64 n) {
         i64 bytes = 0;
@@ -78,7 +79,7 @@ void register_ffn(py::module& m) {
         if (bias_mode && !ws) throw std::invalid_argument("act_grad: workspace missing");
         real_dispatch(dt, [&](auto z) { act_grad<decltype(z)>(a, S(st)); });
     });
-    m.def("clip_ws", [](const Mats& v) { const auto c = mats(v); return clip_parts(c.data(), (int)c.size()); });
+    m.def("clip_ws", [](char ta, const Mats& v) { const auto c = mats(v); return clip_parts(ta, c.data(), (int)c.size()); });
     m.def("clip_sum", [](char ta, const Mats& v, uintptr_t part, uintptr_t st) {
         const auto c = mats(v);
         return (i64)clip_sum(ta, c.data(), (int)c.size(), (double*)W(part), S(st));

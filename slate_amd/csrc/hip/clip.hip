@@ -15,7 +15,9 @@ namespace slate_hip {
 
 namespace {
 
-constexpr int CLIP_MATS = 48, CLIP_UNIT = 16384, CLIP_BLOCKS = 1024;
+constexpr int CLIP_MATS = 72, CLIP_BLOCKS = 1024;
+// a unit of work: 32 KiB of a matrix
+template <typename T> constexpr int clip_unit() { return 32768 / (int)sizeof(T); }
 
 struct ClipArgs {
     ClipMat v[CLIP_MATS];
@@ -50,19 +52,33 @@ __device__ inline double clip_block_sum(double x, double* lds) {
     return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-// f(i, j, vector): thread's share of unit u of matrix v, E rows at a time
-template <int E, typename F> __device__ inline void clip_walk(i64 m, i64 n, i64 u, bool flat, F&& f) {
-    const i64 total = m * n, lo = u * CLIP_UNIT, hi = min(total, lo + CLIP_UNIT);
+// This thread's share of unit u of an m x n matrix: whole(i, j) for E rows at
+// (i, j), one(i, j) for one.  Vectors need no alignment, but cross no column's
+// end: the columns are one (flat), or their length is a multiple of E.
+template <int E, int UNIT, typename F, typename G>
+__device__ inline void clip_walk(i64 m, i64 n, i64 u, bool flat, F&& whole, G&& one) {
+    const i64 total = m * n, lo = u * UNIT, hi = min(total, lo + UNIT);
     if (flat) {
-        for (i64 q = lo + threadIdx.x * E; q < hi; q += 256 * E) f(q, (i64)0);
+        constexpr int N = UNIT / (256 * E), B = N < 4 ? N : 4;
+        if (hi - lo == UNIT) {
+            #pragma unroll 1
+            for (int b = 0; b < N; b += B) whole(lo + (b * 256 + (i64)threadIdx.x) * E, (i64)0, std::integral_constant<int, B>());
+            return;
+        }
+        i64 q = lo + threadIdx.x * E;
+        for (; q + E <= hi; q += 256 * E) whole(q, (i64)0, std::integral_constant<int, 1>());
+        for (; q < hi; ++q) one(q, (i64)0);
         return;
     }
-    i64 q = lo + threadIdx.x * E;
+    const bool vec = m % E == 0;
+    const int w = vec ? E : 1;
+    i64 q = lo + threadIdx.x * w;
     if (q >= hi) return;
     i64 j = q / m, i = q - j * m;
-    const i64 dj = 256 * E / m, di = 256 * E - dj * m;
-    for (; q < hi; q += 256 * E) {
-        f(i, j);
+    const i64 dj = 256 * w / m, di = 256 * w - dj * m;
+    for (; q < hi; q += 256 * w) {
+        if (vec) whole(i, j, std::integral_constant<int, 1>());
+        else one(i, j);
         i += di;
         j += dj;
         if (i >= m) { i -= m; ++j; }
@@ -81,7 +97,7 @@ __device__ inline int clip_find(const ClipArgs& a, int u) {
 template <typename T>
 __global__ void __launch_bounds__(256) clip_sum_kernel(ClipArgs a) {
     constexpr int E = 16 / sizeof(T);
-    typedef T vE __attribute__((ext_vector_type(E)));
+    typedef T vE __attribute__((ext_vector_type(E), aligned(sizeof(T))));
     __shared__ double lds[4];
     double s[3] = {0, 0, 0};
     for (int u = blockIdx.x; u < a.first[a.count]; u += gridDim.x) {
@@ -90,16 +106,16 @@ __global__ void __launch_bounds__(256) clip_sum_kernel(ClipArgs a) {
         const T* A = static_cast<const T*>(v.A);
         const bool flat = v.lda == v.m || v.n == 1;
         const i64 uu = u - a.first[c];
-        // whole vectors: aligned, and no vector crosses a column's end
-        if ((uintptr_t)A % 16 == 0 && (flat ? (v.m * v.n) % E == 0 : (v.lda % E == 0 && v.m % E == 0))) {
-            clip_walk<E>(v.m, v.n, uu, flat, [&](i64 i, i64 j) {
-                const vE x = *reinterpret_cast<const vE*>(A + i + j * v.lda);
+        clip_walk<E, clip_unit<T>()>(v.m, v.n, uu, flat, [&](i64 i, i64 j, auto count) {
+            constexpr int B = decltype(count)::value;
+            vE x[B];
+            #pragma unroll
+            for (int b = 0; b < B; ++b) x[b] = *reinterpret_cast<const vE*>(A + i + b * (256 * E) + j * v.lda);
+            #pragma unroll
+            for (int b = 0; b < B; ++b)
                 #pragma unroll
-                for (int e = 0; e < E; ++e) clip_add(s, (T)x[e]);
-            });
-        } else {
-            clip_walk<1>(v.m, v.n, uu, flat, [&](i64 i, i64 j) { clip_add(s, A[i + j * v.lda]); });
-        }
+                for (int e = 0; e < E; ++e) clip_add(s, (T)x[b][e]);
+        }, [&](i64 i, i64 j) { clip_add(s, A[i + j * v.lda]); });
     }
     #pragma unroll
     for (int h = 0; h < 3; ++h) {
@@ -127,14 +143,15 @@ template <typename TA, typename TB>
 __global__ void __launch_bounds__(256) clip_scale_kernel(ClipArgs a) {
     using R = std::conditional_t<sizeof(TA) == 8, double, float>;
     constexpr int E = 16 / sizeof(TA);
-    typedef TA vA __attribute__((ext_vector_type(E)));
-    typedef TB vB __attribute__((ext_vector_type(E)));
+    typedef TA vA __attribute__((ext_vector_type(E), aligned(sizeof(TA))));
+    typedef TB vB __attribute__((ext_vector_type(E), aligned(sizeof(TB))));
     __shared__ double lds[4];
     const double norm = clip_norm_of(a, lds);
     if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
     const bool cut = norm > a.limit && norm < __builtin_huge_val();
     const R f = cut ? (R)(a.limit / norm) : R(1);
-    for (int u = blockIdx.x; u < a.first[a.count]; u += gridDim.x) {
+    // backwards: what the first pass read last is still in the cache
+    for (int u = a.first[a.count] - 1 - (int)blockIdx.x; u >= 0; u -= gridDim.x) {
         const int c = clip_find(a, u);
         const ClipMat v = a.v[c];
         const TA* A = static_cast<const TA*>(v.A);
@@ -142,21 +159,22 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(ClipArgs a) {
         if (!cut && v.A == v.B) continue;
         const bool flat = (v.lda == v.m && v.ldb == v.m) || v.n == 1;
         const i64 uu = u - a.first[c];
-        if ((uintptr_t)A % 16 == 0 && (uintptr_t)B % sizeof(vB) == 0 &&
-            (flat ? (v.m * v.n) % E == 0 : (v.lda % E == 0 && v.ldb % E == 0 && v.m % E == 0))) {
-            clip_walk<E>(v.m, v.n, uu, flat, [&](i64 i, i64 j) {
-                const vA x = *reinterpret_cast<const vA*>(A + i + j * v.lda);
+        clip_walk<E, clip_unit<TA>()>(v.m, v.n, uu, flat, [&](i64 i, i64 j, auto count) {
+            constexpr int N = decltype(count)::value;
+            vA x[N];
+            #pragma unroll
+            for (int b = 0; b < N; ++b) x[b] = *reinterpret_cast<const vA*>(A + i + b * (256 * E) + j * v.lda);
+            #pragma unroll
+            for (int b = 0; b < N; ++b) {
                 vB y;
                 #pragma unroll
-                for (int e = 0; e < E; ++e) y[e] = (TB)(cut ? (R)x[e] * f : (R)x[e]);
-                *reinterpret_cast<vB*>(B + i + j * v.ldb) = y;
-            });
-        } else {
-            clip_walk<1>(v.m, v.n, uu, flat, [&](i64 i, i64 j) {
-                const R x = (R)A[i + j * v.lda];
-                B[i + j * v.ldb] = (TB)(cut ? x * f : x);
-            });
-        }
+                for (int e = 0; e < E; ++e) y[e] = (TB)(cut ? (R)x[b][e] * f : (R)x[b][e]);
+                *reinterpret_cast<vB*>(B + i + b * (256 * E) + j * v.ldb) = y;
+            }
+        }, [&](i64 i, i64 j) {
+            const R x = (R)A[i + j * v.lda];
+            B[i + j * v.ldb] = (TB)(cut ? x * f : x);
+        });
     }
 }
 
@@ -172,21 +190,21 @@ __global__ void __launch_bounds__(256) clip_join_kernel(const double* part, int 
 }
 
 // the matrices [at, at + CLIP_MATS) as one launch's arguments; -> its units
-int clip_fill(ClipArgs& a, const ClipMat* v, int count, int at) {
+int clip_fill(ClipArgs& a, const ClipMat* v, int count, int at, int unit) {
     a.count = std::max(0, std::min(CLIP_MATS, count - at));
     a.first[0] = 0;
     for (int i = 0; i < a.count; ++i) {
         a.v[i] = v[at + i];
-        a.first[i + 1] = a.first[i] + (int)((a.v[i].m * a.v[i].n + CLIP_UNIT - 1) / CLIP_UNIT);
+        a.first[i + 1] = a.first[i] + (int)((a.v[i].m * a.v[i].n + unit - 1) / unit);
     }
     return a.first[a.count];
 }
 
 template <typename TA, typename TB>
 void clip_scale_run(const ClipMat* v, int count, double limit, const double* part, int parts, double* norm, hipStream_t s) {
-    for (int at = 0; at == 0 || at < count; at += CLIP_MATS) {
+    for (int at = count ? (count - 1) / CLIP_MATS * CLIP_MATS : 0; at >= 0; at -= CLIP_MATS) {
         ClipArgs a;
-        const int blocks = std::min(CLIP_BLOCKS, clip_fill(a, v, count, at));
+        const int blocks = std::min(CLIP_BLOCKS, clip_fill(a, v, count, at, clip_unit<TA>()));
         a.limit = limit;
         a.all = part;
         a.parts = parts;
@@ -198,12 +216,15 @@ void clip_scale_run(const ClipMat* v, int count, double limit, const double* par
 
 }  // namespace
 
-i64 clip_parts(const ClipMat* v, int count) {
+static int clip_unit_of(char t) { return t == 'd' ? clip_unit<double>() : t == 's' ? clip_unit<float>() : clip_unit<__bf16>(); }
+
+i64 clip_parts(char ta, const ClipMat* v, int count) {
+    const i64 unit = clip_unit_of(ta);
     i64 parts = 0;
     for (int at = 0; at < count; at += CLIP_MATS) {
         i64 units = 0;
         for (int i = at; i < std::min(count, at + CLIP_MATS); ++i) {
-            const i64 u = (v[i].m * v[i].n + CLIP_UNIT - 1) / CLIP_UNIT;
+            const i64 u = (v[i].m * v[i].n + unit - 1) / unit;
             if (u + units > 0x7fffffff) throw std::invalid_argument("clip_norm: matrices too large for one call");
             units += u;
         }
@@ -216,7 +237,7 @@ int clip_sum(char ta, const ClipMat* v, int count, double* part, hipStream_t s) 
     int done = 0;
     for (int at = 0; at < count; at += CLIP_MATS) {
         ClipArgs a;
-        const int blocks = std::min(CLIP_BLOCKS, clip_fill(a, v, count, at));
+        const int blocks = std::min(CLIP_BLOCKS, clip_fill(a, v, count, at, clip_unit_of(ta)));
         a.part = part + 3 * (i64)done;
         done += blocks;
         if (ta == 'b') hipLaunchKernelGGL((clip_sum_kernel<__bf16>), dim3(blocks), dim3(256), 0, s, a);

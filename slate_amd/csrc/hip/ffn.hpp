@@ -24,8 +24,7 @@ struct GemmActArgs {
     int bias_mode = 0;      // 0 none, 1 one value per row of C, 2 one per column
     int act = ACT_IDENTITY;
     // filled by the launcher
-    int vec = 0;            // bit 0 C, 1 R, 2 Z, 3 bias: 16 bytes of rows in one access
-    int nfull = 0;          // K steps per product that LDS-DMA may stage (0: all through registers)
+    i64 kfull = 0;          // first k that LDS-DMA does not stage
     int nsteps = 0;         // K steps per product
     int group_m = 8;
     int splits = 1, per_split = 0;
@@ -33,11 +32,12 @@ struct GemmActArgs {
     i64 ldp = 0;
 };
 
-// Which tile, and in how many pieces K: made from sizes and the element size
-// alone, so that the caller can give the workspace (bytes) with the call.
+// Which kernel, and in how many pieces K: from sizes, types and alignment alone.
+// tile -1: the kernel for few columns; bytes: workspace.
 struct GemmActPlan { int tile = 0, splits = 1, per_split = 0; i64 ldp = 0, bytes = 0; };
-GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k);
-template <typename T> void gemm_act(GemmActArgs a, char ta, char tb, const GemmActPlan& p, hipStream_t s);
+GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool bkc, bool dma);
+// Launches and returns 0, or returns the workspace wanted where part is null.
+template <typename T> i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s);
 
 // dZ = dC o act'(Z) (dZ1 = dC o Z2 o act'(Z1), dZ2 = dC o act(Z1) where Z2 is
 // given), and the sums of dZ over the columns (bias_mode 1) or rows (2)
@@ -59,7 +59,7 @@ template <typename T> void act_grad(ActGradArgs a, hipStream_t s);
 // number of matrices.  part: clip_parts() doubles, three (sums of squares of
 // small, ordinary and large elements) per block of the first pass.
 struct ClipMat { const void* A; void* B; i64 m, n, lda, ldb; };
-i64 clip_parts(const ClipMat* v, int count);
+i64 clip_parts(char ta, const ClipMat* v, int count);
 int clip_sum(char ta, const ClipMat* v, int count, double* part, hipStream_t s);          // -> partial sums written
 void clip_join(const double* part, int parts, double* out, hipStream_t s);                // all of them as one
 void clip_scale(char ta, char tb, const ClipMat* v, int count, double limit, const double* part, int parts,

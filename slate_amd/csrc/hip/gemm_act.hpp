@@ -31,6 +31,12 @@ typedef int i4v __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
 typedef _Float16 hf8v __attribute__((ext_vector_type(8)));
 
+// V elements as one access.  Rows need not lie on 16 bytes: the type claims the
+// element's alignment only, and the hardware takes such addresses (a vector
+// that straddles a cache line costs a second access, not V of them).
+template <typename T, int V> struct ga_vec_of { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
+template <typename T, int V> using ga_vec = typename ga_vec_of<T, V>::type;
+
 template <typename T> struct ga_traits;
 template <> struct ga_traits<__bf16> {
     using acc = float; using acc4 = f4;
@@ -119,7 +125,7 @@ __device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, c
                                  const typename ga_traits<T>::acc* s2) {
     using R = typename ga_traits<T>::acc;
     constexpr bool FAST = sizeof(T) == 2;
-    typedef T vT __attribute__((ext_vector_type(V)));
+    using vT = ga_vec<T, V>;
     if (n >= a.n || m >= a.m) return;
     const bool whole = V == 1 || m + V <= a.m;
     const int left = (int)min((i64)V, a.m - m);
@@ -134,7 +140,7 @@ __device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, c
         for (int r = 0; r < V; ++r) z[r] = alpha * s1[r];
         if (a.bias_mode == 1) {
             const T* b = static_cast<const T*>(a.bias);
-            if (whole && (a.vec & 8)) {
+            if (whole && a.incb == 1) {
                 const vT x = *reinterpret_cast<const vT*>(b + m);
                 #pragma unroll
                 for (int r = 0; r < V; ++r) z[r] += (R)x[r];
@@ -152,7 +158,7 @@ __device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, c
         if (a.R) {
             const T* X = static_cast<const T*>(a.R) + m + n * a.ldr;
             const R beta = (R)a.beta;
-            if (whole && (a.vec & 2)) {
+            if (whole) {
                 const vT x = *reinterpret_cast<const vT*>(X);
                 #pragma unroll
                 for (int r = 0; r < V; ++r) y[r] += beta * (R)x[r];
@@ -173,10 +179,10 @@ __device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, c
             for (int r = 0; r < V; ++r) if (r < left) p[r] = (T)v[r];
         }
     };
-    put(C, y, whole && (a.vec & 1));
-    if (a.Z[0]) put(static_cast<T*>(a.Z[0]) + m + n * a.ldz[0], z, whole && (a.vec & 4));
+    put(C, y, whole);
+    if (a.Z[0]) put(static_cast<T*>(a.Z[0]) + m + n * a.ldz[0], z, whole);
     if constexpr (GATED)
-        if (a.Z[1]) put(static_cast<T*>(a.Z[1]) + m + n * a.ldz[1], s2, whole && (a.vec & 4));
+        if (a.Z[1]) put(static_cast<T*>(a.Z[1]) + m + n * a.ldz[1], s2, whole);
 }
 
 // ------------------------------------------------------------- LDS images
@@ -242,25 +248,32 @@ template <typename T, int R, bool KC> struct GaImg {
             return (uint32_t)((k * ld + rr) * ES);
         }
     }
-    // the slab through registers: any alignment, zeros past the matrix
+    // 16-byte slot q of the slab at X, off elements from X, at any alignment; zeros
+    // past the matrix in k, anything in rows that do not exist
+    __device__ static inline i64 element(int q, i64 ld, i64 rows) {
+        int r, k;
+        src_of(q, r, k);
+        if constexpr (KC) return (r < rows ? r : rows - 1) * ld + k;
+        else return k * ld + r;
+    }
+    __device__ static inline i4v fetch(const T* X, i64 off, int q, i64 ld, i64 rows, i64 kleft, bool inside) {
+        using vE = ga_vec<T, E>;
+        int r, k;
+        src_of(q, r, k);
+        if (inside || (KC ? kleft - k >= E : k < kleft && rows - r >= E))
+            return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(X + off));
+        vE w;
+        #pragma unroll
+        for (int e = 0; e < E; ++e) {
+            w[e] = (T)0;
+            if (KC ? k + e < kleft : k < kleft && r + e < rows) w[e] = X[off + e];
+        }
+        return __builtin_bit_cast(i4v, w);
+    }
     template <int NT>
     __device__ static inline void stage(const T* X, i64 ld, i64 rows, i64 kleft, char* img, int tid) {
-        for (int q = tid; q < BYTES / 16; q += NT) {
-            int r, k;
-            src_of(q, r, k);
-            T v[E];
-            #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int rr = KC ? r : r + e, kx = KC ? k + e : k;
-                v[e] = (T)0;
-                if (rr < rows && kx < kleft) v[e] = KC ? X[rr * ld + kx] : X[kx * ld + rr];
-            }
-            typedef T vE __attribute__((ext_vector_type(E)));
-            vE w;
-            #pragma unroll
-            for (int e = 0; e < E; ++e) w[e] = v[e];
-            *reinterpret_cast<vE*>(img + q * 16) = w;
-        }
+        for (int q = tid; q < BYTES / 16; q += NT)
+            *reinterpret_cast<i4v*>(img + q * 16) = fetch(X, element(q, ld, rows), q, ld, rows, kleft, false);
     }
 };
 
@@ -280,7 +293,10 @@ template <typename T, int BM, int BN, int WVM, int WVN> struct GaEpi {
 };
 
 // ------------------------------------------------------------------ kernel
-template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, bool GATED>
+// DMA: operands on 16 bytes, staged by LDS-DMA (the ragged end of K through
+// registers).  Otherwise every slab goes through registers, fetched before the
+// products of the slab ahead of it and written to LDS after them.
+template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, bool GATED, bool DMA>
 __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a) {
     using TR = ga_traits<T>;
     using acc4 = typename TR::acc4;
@@ -306,9 +322,19 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
     const int s0 = a.splits > 1 ? (int)blockIdx.y * a.per_split : 0;
     const int s1 = a.splits > 1 ? min(total, s0 + a.per_split) : total;
 
-    uint32_t offA[NA][PA], offB[PB];
     const i64 rowsA = a.m - m0, rowsB = a.n - n0;
     const bool sum = a.mode == GA_SUM;
+    // product and first k of step s
+    auto step = [&](int s, int& p, i64& k0) {
+        p = pair;
+        if (sum && s >= a.nsteps) { s -= a.nsteps; p = 1; }
+        k0 = (i64)s * KB;
+    };
+    auto slabA = [&](int q, i64 k0) { return static_cast<const T*>(a.A[q]) + (AKC ? m0 * a.lda[q] + k0 : m0 + k0 * a.lda[q]); };
+    auto slabB = [&](int q, i64 k0) { return static_cast<const T*>(a.B[q]) + (BKC ? n0 * a.ldb[q] + k0 : n0 + k0 * a.ldb[q]); };
+
+    // LDS-DMA
+    uint32_t offA[NA][PA], offB[PB];
     auto offsets = [&](int p) {
         #pragma unroll
         for (int h = 0; h < NA; ++h)
@@ -320,46 +346,79 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             offB[i] = IB::offset(min(wid + i * NW, IB::CHUNKS - 1), lane, a.ldb[p], rowsB);
     };
     int curp = sum ? (s0 >= a.nsteps ? 1 : 0) : pair;
-    offsets(curp);
+    if constexpr (DMA) offsets(curp);
 
     using gptr = const __attribute__((address_space(1))) void*;
     using lptr = __attribute__((address_space(3))) void*;
     auto issue = [&](int s) {
-        int kt = s, p = pair;
-        if (sum && s >= a.nsteps) { kt = s - a.nsteps; p = 1; }
+        int p;
+        i64 k0;
+        step(s, p, k0);
         if (sum && p != curp) { curp = p; offsets(p); }
         char* slot = smem + (s & 1) * SLOT;
-        const i64 k0 = (i64)kt * KB;
-        if (kt < a.nfull) {
+        if (k0 < a.kfull) {
             #pragma unroll
             for (int h = 0; h < NA; ++h) {
-                const int q = GATED ? h : p;
-                const char* X = static_cast<const char*>(a.A[q]) +
-                                (AKC ? m0 * a.lda[q] + k0 : m0 + k0 * a.lda[q]) * (i64)sizeof(T);
+                const char* X = reinterpret_cast<const char*>(slabA(GATED ? h : p, k0));
                 #pragma unroll
-                for (int i = 0; i < PA; ++i) {
-                    const int c = min(wid + i * NW, IA::CHUNKS - 1);
-                    __builtin_amdgcn_global_load_lds((gptr)(X + offA[h][i]),
-                                                     (lptr)(slot + h * IA::BYTES + c * 1024), 16, 0, 0);
-                }
+                for (int i = 0; i < PA; ++i)
+                    __builtin_amdgcn_global_load_lds(
+                        (gptr)(X + offA[h][i]),
+                        (lptr)(slot + h * IA::BYTES + min(wid + i * NW, IA::CHUNKS - 1) * 1024), 16, 0, 0);
             }
-            const char* Y = static_cast<const char*>(a.B[p]) +
-                            (BKC ? n0 * a.ldb[p] + k0 : n0 + k0 * a.ldb[p]) * (i64)sizeof(T);
+            const char* Y = reinterpret_cast<const char*>(slabB(p, k0));
             #pragma unroll
-            for (int i = 0; i < PB; ++i) {
-                const int c = min(wid + i * NW, IB::CHUNKS - 1);
-                __builtin_amdgcn_global_load_lds((gptr)(Y + offB[i]), (lptr)(slot + BM * 128 + c * 1024), 16, 0, 0);
-            }
+            for (int i = 0; i < PB; ++i)
+                __builtin_amdgcn_global_load_lds((gptr)(Y + offB[i]),
+                                                 (lptr)(slot + BM * 128 + min(wid + i * NW, IB::CHUNKS - 1) * 1024), 16, 0, 0);
         } else {
             #pragma unroll
-            for (int h = 0; h < NA; ++h) {
-                const int q = GATED ? h : p;
-                IA::template stage<NT>(static_cast<const T*>(a.A[q]) + (AKC ? m0 * a.lda[q] + k0 : m0 + k0 * a.lda[q]),
-                                       a.lda[q], rowsA, a.k - k0, slot + h * IA::BYTES, tid);
-            }
-            IB::template stage<NT>(static_cast<const T*>(a.B[p]) + (BKC ? n0 * a.ldb[p] + k0 : n0 + k0 * a.ldb[p]),
-                                   a.ldb[p], rowsB, a.k - k0, slot + BM * 128, tid);
+            for (int h = 0; h < NA; ++h)
+                IA::template stage<NT>(slabA(GATED ? h : p, k0), a.lda[GATED ? h : p], rowsA, a.k - k0,
+                                       slot + h * IA::BYTES, tid);
+            IB::template stage<NT>(slabB(p, k0), a.ldb[p], rowsB, a.k - k0, slot + BM * 128, tid);
         }
+    };
+
+    // through registers
+    constexpr int QA = IA::BYTES / 16, QB = IB::BYTES / 16, CA = DMA ? 1 : (QA + NT - 1) / NT, CB = DMA ? 1 : (QB + NT - 1) / NT;
+    i4v ra[NA][CA], rb[CB];
+    i64 elA[NA][CA], elB[CB];
+    auto elements = [&](int p) {
+        #pragma unroll
+        for (int h = 0; h < NA; ++h)
+            #pragma unroll
+            for (int i = 0; i < CA; ++i) elA[h][i] = IA::element(min(tid + i * NT, QA - 1), a.lda[GATED ? h : p], rowsA);
+        #pragma unroll
+        for (int i = 0; i < CB; ++i) elB[i] = IB::element(min(tid + i * NT, QB - 1), a.ldb[p], rowsB);
+    };
+    if constexpr (!DMA) elements(curp);
+    auto fetch = [&](int s) {
+        int p;
+        i64 k0;
+        step(s, p, k0);
+        if (sum && p != curp) { curp = p; elements(p); }
+        const i64 left = a.k - k0;
+        const bool inA = left >= KB && (AKC || rowsA >= BMI), inB = left >= KB && (BKC || rowsB >= BN);
+        #pragma unroll
+        for (int h = 0; h < NA; ++h)
+            #pragma unroll
+            for (int i = 0; i < CA; ++i)
+                ra[h][i] = IA::fetch(slabA(GATED ? h : p, k0), elA[h][i], min(tid + i * NT, QA - 1), a.lda[GATED ? h : p],
+                                     rowsA, left, inA);
+        #pragma unroll
+        for (int i = 0; i < CB; ++i)
+            rb[i] = IB::fetch(slabB(p, k0), elB[i], min(tid + i * NT, QB - 1), a.ldb[p], rowsB, left, inB);
+    };
+    auto write = [&](int s) {
+        char* slot = smem + (s & 1) * SLOT;
+        #pragma unroll
+        for (int h = 0; h < NA; ++h)
+            #pragma unroll
+            for (int i = 0; i < CA; ++i)
+                *reinterpret_cast<i4v*>(slot + h * IA::BYTES + min(tid + i * NT, QA - 1) * 16) = ra[h][i];
+        #pragma unroll
+        for (int i = 0; i < CB; ++i) *reinterpret_cast<i4v*>(slot + BM * 128 + min(tid + i * NT, QB - 1) * 16) = rb[i];
     };
 
     const int wm = wid / WVN, wn = wid % WVN;
@@ -371,14 +430,20 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             #pragma unroll
             for (int r = 0; r < 4; ++r) acc[i][j][r] = R(0);
 
-    if (s0 < s1) issue(s0);
+    if (s0 < s1) {
+        if constexpr (DMA) issue(s0);
+        else { fetch(s0); write(s0); }
+    }
     for (int s = s0; s < s1; ++s) {
         // my part of step s has landed ...
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         // ... and everyone's, and everyone has read step s - 1's slot
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + 1 < s1) issue(s + 1);
+        if (s + 1 < s1) {
+            if constexpr (DMA) issue(s + 1);
+            else fetch(s + 1);
+        }
         const char* la = smem + (s & 1) * SLOT;
         const char* lb = la + BM * 128;
         #pragma unroll
@@ -402,6 +467,8 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
                     else acc[i][j] = TR::mma(fb[j], fa[i], acc[i][j]);
                 }
         }
+        if constexpr (!DMA)
+            if (s + 1 < s1) write(s + 1);
     }
 
     constexpr int H = MI / NA, WH = WM / NA;
@@ -464,30 +531,141 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
     }
 }
 
-// adds the partial sums in the order of their splits and finishes them
+// ------------------------------------------------------------ few columns
+// C of up to 16 NF columns (tokens), both operands contiguous along k: bound by
+// reading op(A) once.  A workgroup takes 16 rows and all of K, its NW waves
+// interleaved slabs of 128 bytes per row, fragments straight from memory to
+// registers with 2 U of them in flight per wave and operand (no LDS, no
+// barrier in the loop); the waves' sums are added in LDS in their order.
+template <typename T, int NF, bool GATED, int NW>
+__global__ void __launch_bounds__(64 * NW) gemm_act_skinny_kernel(GemmActArgs a) {
+    using TR = ga_traits<T>;
+    using acc4 = typename TR::acc4;
+    using R = typename TR::acc;
+    constexpr int NA = GATED ? 2 : 1, E = 16 / (int)sizeof(T), KB = 8 * E, U = NF * NA <= 1 ? 4 : 2, LD = 16 + 16 / (int)sizeof(R);
+    __shared__ __align__(16) R red[NW][NA][NF][16 * LD];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
+    const i64 m0 = (i64)xcd_remap(blockIdx.x, gridDim.x) * 16;
+    // rows and columns past the matrix read one that exists and are not stored
+    const T* pa[NA];
+    const T* pb[NF];
+    #pragma unroll
+    for (int h = 0; h < NA; ++h) pa[h] = static_cast<const T*>(a.A[h]) + min(m0 + l, a.m - 1) * a.lda[h] + g * E;
+    #pragma unroll
+    for (int j = 0; j < NF; ++j) pb[j] = static_cast<const T*>(a.B[0]) + min((i64)(j * 16 + l), a.n - 1) * a.ldb[0] + g * E;
+    acc4 acc[NA][NF];
+    #pragma unroll
+    for (int h = 0; h < NA; ++h)
+        #pragma unroll
+        for (int j = 0; j < NF; ++j)
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) acc[h][j][r] = R(0);
+    auto mul = [&](const i4v (&fa)[NA], const i4v (&fb)[NF]) {
+        #pragma unroll
+        for (int h = 0; h < NA; ++h)
+            #pragma unroll
+            for (int j = 0; j < NF; ++j) {
+                if constexpr (sizeof(R) == 4) acc[h][j] = TR::mma(fa[h], fb[j], acc[h][j]);
+                else acc[h][j] = TR::mma(fb[j], fa[h], acc[h][j]);
+            }
+    };
+    const int slabs = (int)(a.k / KB);
+    int s = w;
+    for (; s + (U - 1) * NW < slabs; s += U * NW) {
+        i4v fa[2 * U][NA], fb[2 * U][NF];
+        #pragma unroll
+        for (int u = 0; u < 2 * U; ++u) {
+            const i64 k = (i64)(s + (u >> 1) * NW) * KB + (u & 1) * (4 * E);
+            #pragma unroll
+            for (int h = 0; h < NA; ++h)
+                fa[u][h] = __builtin_bit_cast(i4v, __builtin_nontemporal_load(reinterpret_cast<const ga_vec<T, E>*>(pa[h] + k)));
+            #pragma unroll
+            for (int j = 0; j < NF; ++j) fb[u][j] = __builtin_bit_cast(i4v, *reinterpret_cast<const ga_vec<T, E>*>(pb[j] + k));
+        }
+        #pragma unroll
+        for (int u = 0; u < 2 * U; ++u) mul(fa[u], fb[u]);
+    }
+    for (; s * KB < a.k; s += NW) {
+        #pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const i64 k = (i64)s * KB + kk * (4 * E);
+            const int left = (int)min((i64)E, a.k - k - g * E);
+            i4v fa[NA], fb[NF];
+            auto get = [&](const T* p) {
+                using vE = ga_vec<T, E>;
+                vE x;
+                if (left == E) return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(p + k));
+                #pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = e < left ? p[k + e] : (T)0;
+                return __builtin_bit_cast(i4v, x);
+            };
+            #pragma unroll
+            for (int h = 0; h < NA; ++h) fa[h] = get(pa[h]);
+            #pragma unroll
+            for (int j = 0; j < NF; ++j) fb[j] = get(pb[j]);
+            mul(fa, fb);
+        }
+    }
+    #pragma unroll
+    for (int h = 0; h < NA; ++h)
+        #pragma unroll
+        for (int j = 0; j < NF; ++j)
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = sizeof(R) == 4 ? g * 4 + r : l, col = sizeof(R) == 4 ? l : g + 4 * r;
+                red[w][h][j][col * LD + row] = acc[h][j][r];
+            }
+    __syncthreads();
+    for (int t = threadIdx.x; t < NF * 256; t += 64 * NW) {
+        const int j = t >> 8, col = (t >> 4) & 15, row = t & 15;
+        if (j * 16 + col >= a.n) break;
+        R x[NA];
+        #pragma unroll
+        for (int h = 0; h < NA; ++h) {
+            x[h] = red[0][h][j][col * LD + row];
+            #pragma unroll
+            for (int q = 1; q < NW; ++q) x[h] += red[q][h][j][col * LD + row];
+        }
+        ga_finish<T, 1, GATED>(a, 0, m0 + row, j * 16 + col, &x[0], &x[NA - 1]);
+    }
+}
+
+// Adds the partial sums and finishes them: 64 threads along the outputs, 4
+// along the pieces of K, so that small outputs (where K is split) keep enough
+// loads in flight; the order of the sums depends on the plan alone.
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(256) gemm_act_join_kernel(GemmActArgs a) {
     using R = typename ga_traits<T>::acc;
-    constexpr int V = 16 / (int)sizeof(T);
+    constexpr int V = 16 / (int)sizeof(R), NP = GATED ? 2 : 1;
     typedef R vR __attribute__((ext_vector_type(V)));
-    const i64 mv = (a.m + V - 1) / V;
-    const i64 t = (i64)blockIdx.x * 256 + threadIdx.x;
-    if (t >= mv * a.n) return;
-    const i64 n = t / mv, m = (t - n * mv) * V;
+    __shared__ vR red[3][NP][64];
+    const i64 mv = (a.m + V - 1) / V, t = (i64)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int y = threadIdx.x >> 6;
+    const bool live = t < mv * a.n;
+    const i64 n = live ? t / mv : 0, m = live ? (t - n * mv) * V : 0;
     const int planes = a.mode == GA_PAIR || GATED ? 2 : 1, pair = GATED ? 0 : (int)blockIdx.z;
-    R x[2][V];
+    const i64 plane = a.n * a.ldp;
+    vR x[NP];
     #pragma unroll
-    for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+    for (int h = 0; h < NP; ++h) {
         #pragma unroll
         for (int r = 0; r < V; ++r) x[h][r] = R(0);
-        const R* P = static_cast<const R*>(a.part) + ((i64)(GATED ? h : pair) * a.n + n) * a.ldp + m;
-        for (int s = 0; s < a.splits; ++s) {
-            const vR v = *reinterpret_cast<const vR*>(P + (i64)s * planes * a.n * a.ldp);
-            #pragma unroll
-            for (int r = 0; r < V; ++r) x[h][r] += v[r];
-        }
+        const R* P = static_cast<const R*>(a.part) + (GATED ? h : pair) * plane + n * a.ldp + m;
+        #pragma unroll 4
+        for (int s = y; s < a.splits; s += 4) x[h] += *reinterpret_cast<const vR*>(P + (i64)s * planes * plane);
+        if (y) red[y - 1][h][threadIdx.x & 63] = x[h];
     }
-    ga_finish<T, V, GATED>(a, pair, m, n, x[0], x[GATED ? 1 : 0]);
+    __syncthreads();
+    if (y || !live) return;
+    R z[2][V];
+    #pragma unroll
+    for (int h = 0; h < NP; ++h) {
+        #pragma unroll
+        for (int q = 0; q < 3; ++q) x[h] += red[q][h][threadIdx.x];
+        #pragma unroll
+        for (int r = 0; r < V; ++r) z[h][r] = x[h][r];
+    }
+    ga_finish<T, V, GATED>(a, pair, m, n, z[0], z[NP - 1]);
 }
 
 }  // namespace slate_hip

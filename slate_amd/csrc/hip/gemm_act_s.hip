@@ -1,4 +1,4 @@
 #include "gemm_act_launch.hpp"
 namespace slate_hip {
-template void gemm_act<float>(GemmActArgs, char, char, const GemmActPlan&, hipStream_t);
+template i64 gemm_act<float>(GemmActArgs, char, char, hipStream_t);
 }

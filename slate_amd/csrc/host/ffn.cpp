@@ -139,7 +139,6 @@ void multiply(i64 m, i64 n, i64 k, const std::vector<double>& A, const std::vect
 }  // namespace
 
 void register_ffn(py::module& m) {
-    m.def("gemm_act_ws", [](int, int, i64, i64, i64) { return (i64)0; });
     m.def("gemm_act", [](char dt, int mode, char ta, char tb, i64 m, i64 n, i64 k, double alpha,
                          uintptr_t A0, i64 lda0, uintptr_t A1, i64 lda1, uintptr_t B0, i64 ldb0, uintptr_t B1, i64 ldb1,
                          uintptr_t C0, i64 ldc0, uintptr_t C1, i64 ldc1, uintptr_t bias, i64 incb, int bias_mode,
@@ -178,6 +177,7 @@ void register_ffn(py::module& m) {
                     }
                 }
         });
+        return (i64)0;                      // no workspace is wanted
     });
     m.def("act_grad_ws", [](char, int, i64, i64) { return (i64)0; });
     m.def("act_grad", [](char dt, i64 m, i64 n, int act, uintptr_t dC, i64 lddc, uintptr_t Z1, i64 ldz1, uintptr_t Z2,
@@ -206,7 +206,7 @@ void register_ffn(py::module& m) {
     // matrices: (A, lda, B, ldb, m, n); triple: the sums of squares of small,
     // ordinary and large elements (see csrc/hip/clip.hip)
     using Mats = std::vector<std::tuple<uintptr_t, i64, uintptr_t, i64, i64, i64>>;
-    m.def("clip_ws", [](const Mats&) { return (i64)3; });
+    m.def("clip_ws", [](char, const Mats&) { return (i64)3; });
     m.def("clip_sum", [](char ta, const Mats& v, uintptr_t part, uintptr_t) {
         double s[3] = {0, 0, 0};
         real_dispatch(ta, [&](auto z) {

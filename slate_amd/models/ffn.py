@@ -37,23 +37,26 @@ from ..core.storage import DEV
 from ..utils.trace import trace_block
 from ._panels import col_bcast, row_bcast
 from ._util import grid_of, tiles_local_before
-from .blas3 import _copy_in, _copy_out, _fresh, _single
+from .blas3 import _copy_out, _fresh
 
 PLAIN, GATED, SUM, PAIR = 0, 1, 2, 3
 _ACT = {a: i for i, a in enumerate(Activation)}
 _ACT.update({a.name.lower(): i for a, i in list(_ACT.items())})
-_BYTES = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4, torch.float64: 8}
+_BYTES = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4, torch.float64: 8, torch.complex64: 8, torch.complex128: 16}
 
 
 # ------------------------------------------------------------------ operands
 class _Opd:
-    """One rank's strided column-major operand: address, leading dimension,
-    stored shape, whether it enters transposed, and the tensor that owns it."""
+    """One rank's strided column-major operand: first and one past the last
+    address, leading dimension, stored and logical shape, whether it enters
+    transposed, and the tensor that owns it."""
 
-    __slots__ = ("ptr", "ld", "rows", "cols", "trans", "t")
+    __slots__ = ("ptr", "end", "ld", "rows", "cols", "m", "n", "trans", "t")
 
     def __init__(self, ptr, ld, rows, cols, trans, t):
         self.ptr, self.ld, self.rows, self.cols, self.trans, self.t = ptr, ld, rows, cols, trans, t
+        self.m, self.n = (cols, rows) if trans else (rows, cols)
+        self.end = ptr + ((cols - 1) * ld + rows) * _BYTES[t.dtype] if rows and cols else ptr
 
     @property
     def T(self):
@@ -63,35 +66,73 @@ class _Opd:
     def op(self):
         return 'T' if self.trans else 'N'
 
-    @property
-    def m(self):
-        return self.cols if self.trans else self.rows
-
-    @property
-    def n(self):
-        return self.rows if self.trans else self.cols
-
 
 _NONE = _Opd(0, 0, 0, 0, False, None)
 
 
 def _of_tensor(t, rows, cols, trans=False, name="matrix"):
-    ld = t.stride(1) if cols > 1 else -(-max(rows, 1) // 8) * 8
-    if cols > 1 and ld < rows:
-        raise SlateError(f"{name}: columns overlap (leading dimension {ld} < {rows} rows)")
+    if cols > 1:
+        ld = t.stride(1)
+        if ld < rows:
+            raise SlateError(f"{name}: columns overlap (leading dimension {ld} < {rows} rows)")
+    else:
+        ld = rows + 7 & -8 or 8            # of no meaning: any aligned one
     return _Opd(t.data_ptr(), ld, rows, cols, trans, t)
 
 
 def _opd(M, name="matrix"):
     """The (one) rank's operand of a view."""
     s = M.storage
-    if M._mt == s.mt and M._nt == s.nt and not (M.ioffset or M.joffset or M.row0_offset or M.col0_offset) \
-            and M.last_mb is None and M.last_nb is None and s.origin_slot is not None:
-        t, rows, cols = s.prepare_local(s.origin_slot), s.bc.mloc, s.bc.nloc
-    else:
-        t = M.local_block().data
-        rows, cols = t.shape
-    return _of_tensor(t, rows, cols, M._op != Op.NoTrans, name)
+    slot = s.origin_slot
+    if M._mt == s.mt and M._nt == s.nt and not (M.row0_offset or M.col0_offset) and M.last_mb is None \
+            and M.last_nb is None and slot is not None:
+        t = s.local[slot] if s._valid.get(slot) == s.table.version() else s.prepare_local(slot)
+        bc = s.bc
+        return _of_tensor(t, bc.mloc, bc.nloc, M._op is not Op.NoTrans, name)
+    t = M.local_block().data
+    return _of_tensor(t, t.shape[0], t.shape[1], M._op is not Op.NoTrans, name)
+
+
+def _operands(what, names, mats):
+    """Operands of a one-rank call's matrices (None stays none): one element
+    type, one device, general block-cyclic storage."""
+    out, first = [], None
+    for name, M in zip(names, mats):
+        if M is None:
+            out.append(_NONE)
+            continue
+        s = M.storage
+        if M._kind != "general" or s.bc is None:
+            raise SlateError(f"{what}: {name} must be a general block-cyclic matrix")
+        if s.origin_slot is None:
+            raise SlateError(f"{what}: {name} has no tiles (insertLocalTiles)")
+        x = _opd(M, name)
+        if first is None:
+            first = x.t
+            dt, dev = first.dtype, first.device
+            if dt not in REAL_CODE:
+                raise SlateError(f"{what}: element type {dt} (bfloat16, float16, float32 or float64 are wanted)")
+        elif x.t.dtype != dt:
+            raise SlateError(f"{what}: {name} has type {x.t.dtype}, the others {dt}")
+        elif x.t.device != dev:
+            raise SlateError(f"{what}: {name} is on {x.t.device}, the others on {dev}")
+        out.append(x)
+    return out
+
+
+def _one(mats):
+    """Is every matrix on one rank?"""
+    for M in mats:
+        if M is not None:
+            s = M.storage
+            if s.bc is None or (s.comm.size > 1 and s.bc.p * s.bc.q > 1):
+                return s.bc is None         # not block-cyclic: the checks refuse it
+    return True
+
+
+def _shape(what, name, x, m, n):
+    if x.t is not None and (x.m != m or x.n != n):
+        raise SlateError(f"{what}: {name} is {x.m} x {x.n}, {m} x {n} is wanted")
 
 
 def _t(M):
@@ -99,54 +140,50 @@ def _t(M):
     return None if M is None else M._clone(_op=Op.NoTrans if M._op != Op.NoTrans else Op.Trans)
 
 
-def _span(x):
-    return x.ptr, x.ptr + ((x.cols - 1) * x.ld + x.rows) * _BYTES[x.t.dtype] if x.rows and x.cols else x.ptr
-
-
 def _overlap(x, y):
     """Do two operands share elements?  Blocks of one leading dimension are
     compared as rectangles, others by their address ranges."""
-    (a0, a1), (b0, b1) = _span(x), _span(y)
-    if a1 <= b0 or b1 <= a0:
+    if x.end <= y.ptr or y.end <= x.ptr:
         return False
-    es = _BYTES[x.t.dtype]
-    if y.t.dtype != x.t.dtype or (b0 - a0) % es or (x.cols > 1 and y.cols > 1 and x.ld != y.ld):
+    es, off = _BYTES[x.t.dtype], y.ptr - x.ptr
+    if y.t.dtype != x.t.dtype or off % es or (x.cols > 1 and y.cols > 1 and x.ld != y.ld):
         return True
     ld = x.ld if x.cols > 1 else y.ld
     if x.rows > ld or y.rows > ld:
         return True
-    dc, dr = divmod((b0 - a0) // es, ld)
+    dc, dr = divmod(off // es, ld)
     for c, r in ((dc, dr), (dc + 1, dr - ld)):
         if r < x.rows and -r < y.rows and c < x.cols and -c < y.cols:
             return True
     return False
 
 
-def _outputs(outs, ins, names, in_names, same=()):
-    """Outputs share no element with each other or with inputs; ``same`` lists
-    (output, input) pairs that may be the same view (read, then written, by the
-    same thread)."""
-    for i, x in enumerate(outs):
+def _outputs(what, outs, ins, same=None):
+    """Outputs [(name, operand)] share no element with each other or with
+    inputs; ``same`` names an input that the first output may be (the same view:
+    each element is read, then written, by one thread)."""
+    for i, (nx, x) in enumerate(outs):
         if x.t is None:
             continue
-        for j, y in enumerate(ins):
-            if y.t is None or ((i, j) in same and (x.ptr, x.ld, x.trans, x.t.dtype) == (y.ptr, y.ld, y.trans, y.t.dtype)):
-                continue
-            if _overlap(x, y):
-                raise SlateError(f"output {names[i]} overlaps {in_names[j]}")
-        for j in range(i):
-            if outs[j].t is not None and _overlap(x, outs[j]):
-                raise SlateError(f"outputs {names[i]} and {names[j]} overlap")
+        lo, hi = x.ptr, x.end
+        for ny, y in ins:
+            if y.ptr < hi and lo < y.end and not (i == 0 and ny == same and (x.ptr, x.ld, x.trans) == (y.ptr, y.ld, y.trans)) \
+                    and _overlap(x, y):
+                raise SlateError(f"{what}: output {nx} overlaps {ny}")
+        for ny, y in outs[:i]:
+            if y.ptr < hi and lo < y.end and _overlap(x, y):
+                raise SlateError(f"{what}: outputs {nx} and {ny} overlap")
 
 
 def _act(act):
-    i = _ACT.get(act)
-    if i is None:
+    """Kernel code of an Activation, its name or its character."""
+    try:
+        return _ACT[act]
+    except (KeyError, TypeError):
         try:
             return _ACT[Activation.from_string(act)]
-        except (KeyError, ValueError):
+        except ValueError:
             raise SlateError(f"unknown activation {act!r}") from None
-    return i
 
 
 def _where(s):
@@ -179,15 +216,21 @@ def _check(mats, shapes, what):
     return first
 
 
-def _bias_shape(bias, m, n, what):
-    """(shape to check, mode): one value per row (m x 1) or per column (1 x n)."""
-    if bias is None:
-        return (m, 1), 0
-    if bias.n() == 1 and bias.m() == m:
-        return (m, 1), 1
-    if bias.m() == 1 and bias.n() == n:
-        return (1, n), 2
-    raise SlateError(f"{what}: bias is {bias.m()} x {bias.n()}, {m} x 1 or 1 x {n} is wanted")
+def _bias_mode(what, shape, m, n):
+    """1: one value per row (m x 1), 2: per column (1 x n), 0: no bias."""
+    if shape is None:
+        return 0
+    if shape == (m, 1):
+        return 1
+    if shape == (1, n):
+        return 2
+    raise SlateError(f"{what}: bias is {shape[0]} x {shape[1]}, {m} x 1 or 1 x {n} is wanted")
+
+
+def _bias_of(what, bias, m, n):
+    """(shape to check, mode) of a distributed bias."""
+    mode = _bias_mode(what, None if bias is None else (bias.m(), bias.n()), m, n)
+    return ((1, n) if mode == 2 else (m, 1)), mode
 
 
 def _inc(b):
@@ -212,28 +255,27 @@ class _on:
             self.ctx.__exit__(*e)
 
 
-def _launch(mode, alpha, A, B, C, bias=_NONE, bias_mode=0, act=0, beta=0.0, R=_NONE, Z=()):
-    """One rank's product(s): operands as lists of _Opd, C not transposed."""
-    t = C[0].t
-    m, n, k = C[0].rows, C[0].cols, A[0].n
+def _launch(mode, alpha, A1, A2, B1, B2, C1, C2, bias=_NONE, bias_mode=0, act=0, beta=0.0, R=_NONE, Z1=_NONE, Z2=_NONE):
+    """One rank's product(s); outputs, R and Z not transposed."""
+    t = C1.t
+    m, n, k = C1.rows, C1.cols, A1.n
     if m == 0 or n == 0:
         return
     if alpha == 0:
         k = 0                                   # op(A) op(B) is not read
     if beta == 0:
         R = _NONE
-    A, B, C = (list(x) + [_NONE] * (2 - len(x)) for x in (A, B, C))
-    Z = [z or _NONE for z in Z] + [_NONE] * (2 - len(Z))
     if ops._FLOPS is not None:
         ops._FLOPS[0] += 2 * m * n * k * (1 if mode == PLAIN else 2)
-    mod = kmod(t)
-    nbytes = mod.gemm_act_ws(_BYTES[t.dtype], mode, m, n, k)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
-    mod.gemm_act(REAL_CODE[t.dtype], mode, A[0].op, B[0].op, m, n, k, float(alpha),
-                 A[0].ptr, A[0].ld, A[1].ptr, A[1].ld, B[0].ptr, B[0].ld, B[1].ptr, B[1].ld,
-                 C[0].ptr, C[0].ld, C[1].ptr, C[1].ld, bias.ptr, _inc(bias), bias_mode, act, float(beta),
-                 R.ptr, R.ld, Z[0].ptr, Z[0].ld, Z[1].ptr, Z[1].ld,
-                 0 if ws is None else ws.data_ptr(), raw_stream(t))
+    call = kmod(t).gemm_act
+    args = (REAL_CODE[t.dtype], mode, A1.op, B1.op, m, n, k, alpha, A1.ptr, A1.ld, A2.ptr, A2.ld, B1.ptr, B1.ld,
+            B2.ptr, B2.ld, C1.ptr, C1.ld, C2.ptr, C2.ld, bias.ptr, _inc(bias), bias_mode, act, beta, R.ptr, R.ld,
+            Z1.ptr, Z1.ld, Z2.ptr, Z2.ld)
+    st = raw_stream(t)
+    nbytes = call(*args, 0, st)
+    if nbytes:                                  # few tiles: partial sums of pieces of k
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=t.device)
+        call(*args, ws.data_ptr(), st)
 
 
 def _like(x, rows, cols, trans=False):
@@ -347,8 +389,9 @@ def _run_dist(mode, alpha, A, B, C, bias=None, bias_mode=0, act=0, beta=0.0, R=N
         As, Bs = [_like(_opd(W[0]), lb.mloc, 0)], [_like(_opd(W[0]), 0, lb.nloc)]
     b = _NONE if bias is None else _vector(bias, bias_mode, W[0])
     if grid_rank:
-        _launch(mode, alpha, As, Bs, [_opd(w) for w in W], b, bias_mode, act, beta,
-                _NONE if Rw is None else _opd(Rw), [None if z is None else _opd(z) for z in Zw])
+        As, Bs, Ws = ((x + [_NONE])[:2] for x in (As, Bs, [_opd(w) for w in W]))
+        _launch(mode, alpha, *As, *Bs, *Ws, b, bias_mode, act, beta, _NONE if Rw is None else _opd(Rw),
+                *[_NONE if z is None else _opd(z) for z in Zw])
     _modified(*W, *Zw)
     for w, c in zip(list(W) + Zw, list(C) + list(Z)):
         if w is not None and w is not c:
@@ -370,23 +413,28 @@ def gemm_bias_act(alpha, A, B, bias, act, beta, R, C, Z=None, opts=None):
     if C._op != Op.NoTrans:
         gemm_bias_act(alpha, _t(B), _t(A), _t(bias), act, beta, _t(R), _t(C), _t(Z), opts)
         return C
-    m, n, k = C.m(), C.n(), A.n()
-    bshape, bmode = _bias_shape(bias, m, n, "gemm_bias_act")
-    mats = dict(A=A, B=B, bias=bias, R=R, C=C, Z=Z)
-    _check(mats, dict(A=(m, k), B=(k, n), bias=bshape, R=(m, n), C=(m, n), Z=(m, n)), "gemm_bias_act")
-    with trace_block("gemm_bias_act"):
-        if not _single(*(M for M in mats.values() if M is not None)):
+    what, mats = "gemm_bias_act", (A, B, bias, R, C, Z)
+    with trace_block(what):
+        if not _one(mats):
+            m, n, k = C.m(), C.n(), A.n()
+            bshape, bmode = _bias_of(what, bias, m, n)
+            _check(dict(A=A, B=B, bias=bias, R=R, C=C, Z=Z),
+                   dict(A=(m, k), B=(k, n), bias=bshape, R=(m, n), C=(m, n), Z=(m, n)), what)
             _run_dist(PLAIN, alpha, [A], [B], [C], bias, bmode, a, beta, R, (Z,))
             return C
-        oa, ob, oc = _opd(A, "A"), _opd(B, "B"), _opd(C, "C")
-        o1, orr = (_NONE if bias is None else _opd(bias, "bias")), (_NONE if R is None else _opd(R, "R"))
-        oz = _NONE if Z is None else _opd(Z, "Z")
-        _outputs([oc, oz], [oa, ob, o1, orr], ("C", "Z"), ("A", "B", "bias", "R"), {(0, 3)})
+        oa, ob, o1, orr, oc, oz = _operands(what, ("A", "B", "bias", "R", "C", "Z"), mats)
+        m, n, k = oc.m, oc.n, oa.n
+        _shape(what, "A", oa, m, k)
+        _shape(what, "B", ob, k, n)
+        _shape(what, "R", orr, m, n)
+        _shape(what, "Z", oz, m, n)
+        bmode = _bias_mode(what, None if bias is None else (o1.m, o1.n), m, n)
+        _outputs(what, (("C", oc), ("Z", oz)), (("A", oa), ("B", ob), ("bias", o1), ("R", orr)), "R")
         with _on(oc.t):
             # transposed views of R and Z go through workspace
-            r2 = orr if orr.t is None or beta == 0 else _turn(orr, False)
+            r2 = _turn(orr, False) if orr.trans and beta != 0 else orr
             z2 = _like(oz, m, n) if oz.trans else oz
-            _launch(PLAIN, alpha, [oa], [ob], [oc], o1, bmode, a, beta, r2, (z2 if z2.t is not None else None,))
+            _launch(PLAIN, alpha, oa, _NONE, ob, _NONE, oc, _NONE, o1, bmode, a, beta, r2, z2)
             if z2 is not oz:
                 _copy(z2.t[:m, :n], oz.t[:oz.rows, :oz.cols])
         _modified(C, Z)
@@ -402,26 +450,32 @@ def gemm_gated(A1, A2, B, act, C, Z1=None, Z2=None, opts=None):
     products, which :func:`gemm_gated_grad` takes.  C, Z1 and Z2 overlap no
     other matrix of the call."""
     a = _act(act)
-    m, n, k = C.m(), C.n(), A1.n()
-    mats = dict(A1=A1, A2=A2, B=B, C=C, Z1=Z1, Z2=Z2)
-    _check(mats, dict(A1=(m, k), A2=(m, k), B=(k, n), C=(m, n), Z1=(m, n), Z2=(m, n)), "gemm_gated")
-    with trace_block("gemm_gated"):
-        if not _single(*(M for M in mats.values() if M is not None)):
+    what, mats = "gemm_gated", (A1, A2, B, C, Z1, Z2)
+    with trace_block(what):
+        if not _one(mats):
+            m, n, k = C.m(), C.n(), A1.n()
+            _check(dict(A1=A1, A2=A2, B=B, C=C, Z1=Z1, Z2=Z2),
+                   dict(A1=(m, k), A2=(m, k), B=(k, n), C=(m, n), Z1=(m, n), Z2=(m, n)), what)
             outs = [M if M is None or M._op == Op.NoTrans else _grid_work(M, m, n) for M in (C, Z1, Z2)]
             _run_dist(GATED, 1.0, [A1, A2], [B], outs[:1], act=a, Z=tuple(outs[1:]))
             for w, M in zip(outs, (C, Z1, Z2)):
                 if w is not M:
                     _copy_out(w, M)
             return C
-        o1, o2, ob, oc = _opd(A1, "A1"), _opd(A2, "A2"), _opd(B, "B"), _opd(C, "C")
-        z1, z2 = (_NONE if Z is None else _opd(Z, "Z") for Z in (Z1, Z2))
-        _outputs([oc, z1, z2], [o1, o2, ob], ("C", "Z1", "Z2"), ("A1", "A2", "B"))
+        o1, o2, ob, oc, z1, z2 = _operands(what, ("A1", "A2", "B", "C", "Z1", "Z2"), mats)
+        m, n, k = oc.m, oc.n, o1.n
+        _shape(what, "A1", o1, m, k)
+        _shape(what, "A2", o2, m, k)
+        _shape(what, "B", ob, k, n)
+        _shape(what, "Z1", z1, m, n)
+        _shape(what, "Z2", z2, m, n)
+        _outputs(what, (("C", oc), ("Z1", z1), ("Z2", z2)), (("A1", o1), ("A2", o2), ("B", ob)))
         with _on(oc.t):
             if o1.trans != o2.trans:
                 o2 = _turn(o2, o1.trans)
             # a transposed output is made in workspace and copied
-            w = [x if x.t is None or not x.trans else _like(x, m, n) for x in (oc, z1, z2)]
-            _launch(GATED, 1.0, [o1, o2], [ob], w[:1], act=a, Z=[x if x.t is not None else None for x in w[1:]])
+            w = [_like(x, m, n) if x.trans else x for x in (oc, z1, z2)]
+            _launch(GATED, 1.0, o1, o2, ob, _NONE, w[0], _NONE, _NONE, 0, a, 0.0, _NONE, w[1], w[2])
             for x, y in zip(w, (oc, z1, z2)):
                 if x is not y:
                     _copy(x.t[:m, :n], y.t[:y.rows, :y.cols])
@@ -455,46 +509,49 @@ def gemm_bias_act_grad(alpha, A, B, act, Z, dC, dA, dB, dbias, opts=None):
     the forward pass stored (may be None for the identity).  The residual's
     gradient is beta dC.  dZ is rounded to the matrices' type between the two
     steps, the bias gradient is summed from its unrounded values."""
-    what = "gemm_bias_act_grad"
+    what, mats = "gemm_bias_act_grad", (A, B, Z, dC, dA, dB, dbias)
     a = _act(act)
-    m, n, k = dC.m(), dC.n(), A.n()
-    bshape, bmode = _bias_shape(dbias, m, n, what)
     if Z is None and a:
         raise SlateError(f"{what}: Z is wanted for activation {act}")
-    mats = dict(A=A, B=B, Z=Z, dC=dC, dA=dA, dB=dB, dbias=dbias)
-    _check(mats, dict(A=(m, k), B=(k, n), Z=(m, n), dC=(m, n), dA=(m, k), dB=(k, n), dbias=bshape), what)
-    Z = Z if a else None
     with trace_block(what):
-        if not _single(*(M for M in mats.values() if M is not None)):
-            dZ = _dz_dist(a, dC, (Z, None), dbias, bmode)[0]
+        if not _one(mats):
+            m, n, k = dC.m(), dC.n(), A.n()
+            bshape, bmode = _bias_of(what, dbias, m, n)
+            _check(dict(A=A, B=B, Z=Z, dC=dC, dA=dA, dB=dB, dbias=dbias),
+                   dict(A=(m, k), B=(k, n), Z=(m, n), dC=(m, n), dA=(m, k), dB=(k, n), dbias=bshape), what)
+            dZ = _dz_dist(a, dC, (Z if a else None, None), dbias, bmode)[0]
             if dA is not None:
                 _run_dist_any(PLAIN, alpha, [dZ], [_t(B)], [dA])
             if dB is not None:
                 _run_dist_any(PLAIN, alpha, [_t(A)], [dZ], [dB])
             return
-        oa, ob, oz, oc, ga, gb, gv = (_NONE if M is None else _opd(M, s) for M, s in
-                                      zip((A, B, Z, dC, dA, dB, dbias), ("A", "B", "Z", "dC", "dA", "dB", "dbias")))
-        _outputs([ga, gb, gv], [oa, ob, oz, oc], ("dA", "dB", "dbias"), ("A", "B", "Z", "dC"))
+        oa, ob, oz, oc, ga, gb, gv = _operands(what, ("A", "B", "Z", "dC", "dA", "dB", "dbias"), mats)
+        m, n, k = oc.m, oc.n, oa.n
+        for name, x, r, c in (("A", oa, m, k), ("B", ob, k, n), ("Z", oz, m, n), ("dA", ga, m, k), ("dB", gb, k, n)):
+            _shape(what, name, x, r, c)
+        mode = _bias_mode(what, None if dbias is None else (gv.m, gv.n), m, n)
+        _outputs(what, (("dA", ga), ("dB", gb), ("dbias", gv)), (("A", oa), ("B", ob), ("Z", oz), ("dC", oc)))
         with _on(oc.t):
             dZ = oc
-            if a or dbias is not None:
-                oz = oz if oz.t is None else _turn(oz, oc.trans)
-                dZ = _like(oc, oc.rows, oc.cols, oc.trans) if a and (dA is not None or dB is not None) else _NONE
-                mode = bmode if not oc.trans or not bmode else 3 - bmode
-                _act_grad(oc.rows, oc.cols, a, oc, oz, _NONE, dZ, _NONE, gv, mode)
-                dZ = dZ if a else oc
+            if a or mode:
+                oz = _NONE if not a else oz if oz.trans == oc.trans else _turn(oz, oc.trans)
+                if a and (dA is not None or dB is not None):
+                    dZ = _like(oc, oc.rows, oc.cols, oc.trans)
+                if mode and oc.trans:
+                    mode = 3 - mode
+                _act_grad(oc.rows, oc.cols, a, oc, oz, _NONE, _NONE if dZ is oc else dZ, _NONE, gv, mode)
             if dA is not None:
-                _product(PLAIN, alpha, [dZ], [ob.T], [ga])
+                _product(PLAIN, alpha, dZ, _NONE, ob.T, _NONE, ga, _NONE)
             if dB is not None:
-                _product(PLAIN, alpha, [oa.T], [dZ], [gb])
+                _product(PLAIN, alpha, oa.T, _NONE, dZ, _NONE, gb, _NONE)
         _modified(dA, dB, dbias)
 
 
-def _product(mode, alpha, A, B, C):
+def _product(mode, alpha, A1, A2, B1, B2, C1, C2):
     """One rank's product(s) into outputs of either orientation."""
-    if C[0].trans:
-        A, B, C = [x.T for x in B], [x.T for x in A], [x.T for x in C]
-    _launch(mode, alpha, A, B, C)
+    if C1.trans:
+        A1, A2, B1, B2, C1, C2 = (x if x is _NONE else x.T for x in (B1, B2, A1, A2, C1, C2))
+    _launch(mode, alpha, A1, A2, B1, B2, C1, C2)
 
 
 def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
@@ -506,16 +563,16 @@ def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
     with Z1, Z2 as the forward pass stored them; None leaves a gradient out.
     Both weight gradients are one launch, and dB is one sum over both products,
     rounded once."""
-    what = "gemm_gated_grad"
+    what, mats = "gemm_gated_grad", (A1, A2, B, Z1, Z2, dC, dA1, dA2, dB)
+    names = ("A1", "A2", "B", "Z1", "Z2", "dC", "dA1", "dA2", "dB")
     a = _act(act)
-    m, n, k = dC.m(), dC.n(), A1.n()
-    mats = dict(A1=A1, A2=A2, B=B, Z1=Z1, Z2=Z2, dC=dC, dA1=dA1, dA2=dA2, dB=dB)
     if Z1 is None or Z2 is None:
         raise SlateError(f"{what}: Z1 and Z2 are wanted")
-    w, z = (m, k), (m, n)
-    _check(mats, dict(A1=w, A2=w, B=(k, n), Z1=z, Z2=z, dC=z, dA1=w, dA2=w, dB=(k, n)), what)
     with trace_block(what):
-        if not _single(*(M for M in mats.values() if M is not None)):
+        if not _one(mats):
+            m, n, k = dC.m(), dC.n(), A1.n()
+            w, z = (m, k), (m, n)
+            _check(dict(zip(names, mats)), dict(zip(names, (w, w, (k, n), z, z, z, w, w, (k, n)))), what)
             dZ = _dz_dist(a, dC, (Z1, Z2), None, 0)
             for d, g in zip(dZ, (dA1, dA2)):
                 if g is not None:
@@ -523,20 +580,28 @@ def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
             if dB is not None:
                 _run_dist_any(SUM, 1.0, [_t(A1), _t(A2)], dZ, [dB])
             return
-        names = ("A1", "A2", "B", "Z1", "Z2", "dC", "dA1", "dA2", "dB")
-        o1, o2, ob, z1, z2, oc, g1, g2, gb = (_NONE if M is None else _opd(M, s) for M, s in zip(mats.values(), names))
-        _outputs([g1, g2, gb], [o1, o2, ob, z1, z2, oc], names[6:], names[:6])
+        o1, o2, ob, z1, z2, oc, g1, g2, gb = opds = _operands(what, names, mats)
+        m, n, k = oc.m, oc.n, o1.n
+        w, z = (m, k), (m, n)
+        for name, x, (r, c) in zip(names, opds, (w, w, (k, n), z, z, z, w, w, (k, n))):
+            _shape(what, name, x, r, c)
+        pairs = tuple(zip(names, opds))
+        _outputs(what, pairs[6:], pairs[:6])
         with _on(oc.t):
-            d1, d2 = _like(oc, oc.rows, oc.cols, oc.trans), _like(oc, oc.rows, oc.cols, oc.trans)
-            _act_grad(oc.rows, oc.cols, a, oc, _turn(z1, oc.trans), _turn(z2, oc.trans), d1, d2)
+            tr = oc.trans
+            d1, d2 = _like(oc, oc.rows, oc.cols, tr), _like(oc, oc.rows, oc.cols, tr)
+            _act_grad(oc.rows, oc.cols, a, oc, z1 if z1.trans == tr else _turn(z1, tr),
+                      z2 if z2.trans == tr else _turn(z2, tr), d1, d2)
             if dA1 is not None and dA2 is not None and g1.trans == g2.trans:
-                _product(PAIR, 1.0, [d1, d2], [ob.T, ob.T], [g1, g2])
+                _product(PAIR, 1.0, d1, d2, ob.T, ob.T, g1, g2)
             else:
                 for d, g in ((d1, g1), (d2, g2)):
                     if g.t is not None:
-                        _product(PLAIN, 1.0, [d], [ob.T], [g])
+                        _product(PLAIN, 1.0, d, _NONE, ob.T, _NONE, g, _NONE)
             if dB is not None:
-                _product(SUM, 1.0, [o1.T, (o2 if o2.trans == o1.trans else _turn(o2, o1.trans)).T], [d1, d2], [gb])
+                if o2.trans != o1.trans:
+                    o2 = _turn(o2, o1.trans)
+                _product(SUM, 1.0, o1.T, o2.T, d1, d2, gb, _NONE)
         _modified(dA1, dA2, dB)
 
 
@@ -587,24 +652,25 @@ def _dz_dist(act, dC, Z, dbias, bmode):
 
 # ------------------------------------------------------------------ clipping
 def _clip_views(mats, what):
+    """Operands of a list of matrices of one type, device and communicator."""
     if not isinstance(mats, (list, tuple)):
         raise SlateError(f"{what}: a list of matrices is wanted")
-    out, first = [], None
+    out, dt, dev, comm = [], None, None, None
     for M in mats:
         s = M.storage
-        if getattr(M, "_kind", "general") != "general" or s.bc is None:
+        if M._kind != "general" or s.bc is None:
             raise SlateError(f"{what}: general block-cyclic matrices are wanted")
         if s.origin_slot is None:
             raise SlateError(f"{what}: a matrix has no tiles (insertLocalTiles)")
-        if first is None:
-            first = s
-        elif s.dtype != first.dtype or _where(s) != _where(first):
-            raise SlateError(f"{what}: the matrices differ in type or device ({s.dtype} on {_where(s)}, "
-                             f"{first.dtype} on {_where(first)})")
-        elif s.comm is not first.comm and s.comm.ranks != first.comm.ranks:
+        x = _opd(M)
+        if dt is None:
+            dt, dev, comm = x.t.dtype, x.t.device, s.comm
+        elif x.t.dtype != dt or x.t.device != dev:
+            raise SlateError(f"{what}: the matrices differ in type or device ({x.t.dtype} on {x.t.device}, {dt} on {dev})")
+        elif s.comm is not comm and s.comm.ranks != comm.ranks:
             raise SlateError(f"{what}: the matrices differ in communicator")
-        out.append(_opd(M))
-    return out, first
+        out.append(x)
+    return out
 
 
 def clip_norm(max_norm, A, B=None, opts=None):
@@ -631,49 +697,46 @@ def global_norm(A, opts=None):
     return float(_clip("global_norm", None, A, A))
 
 
+_PARTS = {torch.complex64: torch.float32, torch.complex128: torch.float64}
+
+
 def _clip(what, limit, A, B):
-    va, s = _clip_views(A, what)
+    va = _clip_views(A, what)
     if not va:
         return torch.zeros((), dtype=torch.float64)
-    vb, sb = (va, s) if B is A else _clip_views(B, what)
-    cplx = {torch.complex64: torch.float32, torch.complex128: torch.float64}
-    ta, tb = cplx.get(s.dtype, s.dtype), cplx.get(sb.dtype, sb.dtype)
-    if ta not in REAL_CODE or not (s.dtype == sb.dtype or (_BYTES[ta] == 2 and sb.dtype == torch.float32)):
-        raise SlateError(f"{what}: no scaling from {s.dtype} to {sb.dtype}")
-    if len(vb) != len(va) or _where(sb) != _where(s):
-        raise SlateError(f"{what}: B has {len(vb)} matrices on {_where(sb)}, A has {len(va)} on {_where(s)}")
-    two = 2 if s.dtype in cplx else 1
+    vb = va if B is A else _clip_views(B, what)
+    t, comm = va[0].t, A[0].storage.comm
+    if len(vb) != len(va) or (vb is not va and vb[0].t.device != t.device):
+        raise SlateError(f"{what}: B has {len(vb)} matrices, A has {len(va)}, or they are on different devices")
+    ta, tb = t.dtype, vb[0].t.dtype
+    if _PARTS.get(ta, ta) not in REAL_CODE or not (ta == tb or (_BYTES[ta] == 2 and tb == torch.float32)):
+        raise SlateError(f"{what}: no scaling from {ta} to {tb}")
+    two = 2 if ta in _PARTS else 1
+    ca, cb = REAL_CODE[_PARTS.get(ta, ta)], REAL_CODE[_PARTS.get(tb, tb)]
     with trace_block(what):
         if vb is not va:
             for X, Y, x, y in zip(A, B, va, vb):
-                if X._op != Y._op or (x.rows, x.cols) != (y.rows, y.cols) or X.m() != Y.m() or X.n() != Y.n() or \
-                        (s.comm.size > 1 and not _same_place(X, Y)):
+                if x.trans != y.trans or x.rows != y.rows or x.cols != y.cols or \
+                        (comm.size > 1 and (X.m() != Y.m() or X.n() != Y.n() or not _same_place(X, Y))):
                     raise SlateError(f"{what}: B's matrices want the shapes, ops and distribution of A's")
-        if limit is not None:
-            seen = set()
-            for y in vb:
-                if y.rows and y.cols:
-                    if y.ptr in seen:
-                        raise SlateError(f"{what}: a matrix is in the list twice")
-                    seen.add(y.ptr)
-        t = va[0].t
+        if limit is not None and len({y.ptr for y in vb if y.end > y.ptr}) < sum([y.end > y.ptr for y in vb]):
+            raise SlateError(f"{what}: a matrix is in the list twice")
         mod, st = kmod(t), raw_stream(t)
-        list_ = [(x.ptr, x.ld * two, y.ptr, y.ld * two, x.rows * two, x.cols) for x, y in zip(va, vb)]
+        mats = [(x.ptr, x.ld * two, y.ptr, y.ld * two, x.rows * two, x.cols) for x, y in zip(va, vb)]
         with _on(t):
-            ws = torch.empty(mod.clip_ws(list_) + 4, dtype=torch.float64, device=t.device)
-            base = ws.data_ptr()
-            part = base + 32
-            norm = ws[0]
-            n = mod.clip_sum(REAL_CODE[ta], list_, part, st)
-            if s.comm.size > 1:
-                mod.clip_join(part, n, base + 8, st)
-                s.comm.allreduce(ws[1:4], "sum")
-                part, n = base + 8, 1
-            mod.clip_scale(REAL_CODE[ta], REAL_CODE[tb], list_, 0.0 if limit is None else limit, part, n, base,
-                           limit is not None, st)
+            # [norm, the ranks' common sums (3), partial sums]
+            ws = torch.empty(mod.clip_ws(ca, mats) + 4, dtype=torch.float64, device=t.device)
+            norm = ws.data_ptr()
+            part = norm + 32
+            n = mod.clip_sum(ca, mats, part, st)
+            if comm.size > 1:
+                mod.clip_join(part, n, norm + 8, st)
+                comm.allreduce(ws[1:4], "sum")
+                part, n = norm + 8, 1
+            mod.clip_scale(ca, cb, mats, 0.0 if limit is None else limit, part, n, norm, limit is not None, st)
         if limit is not None:
             _modified(*B)
-    return norm
+    return ws[0]
 
 
 def _same_place(X, Y):
