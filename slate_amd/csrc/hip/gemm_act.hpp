@@ -186,9 +186,9 @@ __device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, c
 }
 
 // ------------------------------------------------------------- LDS images
-template <typename T, int R, bool KC> struct GaImg {
-    static constexpr int ES = sizeof(T), E = 16 / ES, KB = 128 / ES;
-    static constexpr int BYTES = R * 128, CHUNKS = BYTES / 1024;
+template <typename T, int R, bool KC, int KBB> struct GaImg {
+    static constexpr int ES = sizeof(T), E = 16 / ES, KB = KBB / ES, NC = KBB / 16;
+    static constexpr int BYTES = R * KBB, CHUNKS = BYTES / 1024;
     static constexpr int ROWB = R * ES;                       // MN: bytes per k
     static constexpr int SEGB = 16 * ES;                      // MN: bytes of a 16-row segment
     static constexpr int NSEG = R / 16;
@@ -198,11 +198,13 @@ template <typename T, int R, bool KC> struct GaImg {
         else if constexpr (ES == 4) return (k >> 2) & 3 & (NSEG - 1);
         else return (k >> 1) & 1 & (NSEG - 1);
     }
+    // KC: 16 rows of one chunk column lie in 16 distinct 16-byte slots
+    __device__ static constexpr int turn(int r) { return NC == 8 ? (r >> 1) & 7 : (r >> 2) & 3; }
     // row and k of the first element of 16-byte slot q
     __device__ static inline void src_of(int q, int& r, int& k) {
         if constexpr (KC) {
-            r = q >> 3;
-            k = ((q & 7) ^ ((r >> 1) & 7)) * E;
+            r = q / NC;
+            k = ((q % NC) ^ turn(r)) * E;
         } else {
             const int p = q * 16;
             k = p / ROWB;
@@ -214,7 +216,7 @@ template <typename T, int R, bool KC> struct GaImg {
         const int l = lane & 15, g = lane >> 4;
         if constexpr (KC) {
             const int r = r0 + l;
-            return *reinterpret_cast<const i4v*>(img + r * 128 + (((kk * 4 + g) ^ ((r >> 1) & 7)) << 4));
+            return *reinterpret_cast<const i4v*>(img + r * KBB + (((kk * 4 + g) ^ turn(r)) << 4));
         } else if constexpr (ES == 2) {
             typedef short s4 __attribute__((ext_vector_type(4)));
             typedef int i2 __attribute__((ext_vector_type(2)));
@@ -256,7 +258,7 @@ template <typename T, int R, bool KC> struct GaImg {
         if constexpr (KC) return (r < rows ? r : rows - 1) * ld + k;
         else return k * ld + r;
     }
-    __device__ static inline i4v fetch(const T* X, i64 off, int q, i64 ld, i64 rows, i64 kleft, bool inside) {
+    __device__ static inline i4v fetch(const T* X, i64 off, int q, i64 rows, i64 kleft, bool inside) {
         using vE = ga_vec<T, E>;
         int r, k;
         src_of(q, r, k);
@@ -273,7 +275,7 @@ template <typename T, int R, bool KC> struct GaImg {
     template <int NT>
     __device__ static inline void stage(const T* X, i64 ld, i64 rows, i64 kleft, char* img, int tid) {
         for (int q = tid; q < BYTES / 16; q += NT)
-            *reinterpret_cast<i4v*>(img + q * 16) = fetch(X, element(q, ld, rows), q, ld, rows, kleft, false);
+            *reinterpret_cast<i4v*>(img + q * 16) = fetch(X, element(q, ld, rows), q, rows, kleft, false);
     }
 };
 
@@ -281,10 +283,10 @@ template <typename T, int R, bool KC> struct GaImg {
 // fragments at a time, so that stores (and the loads of bias and residual) run
 // along the rows in 16-byte accesses and the activation appears in the code
 // once: unrolled over the 32 fragments of a wave it is 16 000 instructions.
-template <typename T, int BM, int BN, int WVM, int WVN> struct GaEpi {
+template <typename T, int BM, int BN, int WVM, int WVN, int KBB, int S> struct GaEpi {
     static constexpr int AS = sizeof(typename ga_traits<T>::acc), NW = WVM * WVN, NI = BN / WVN / 16;
     static constexpr int LDR = BM / WVM + 16 / AS;                    // rows of a column, and 16 bytes against conflicts
-    static constexpr int RING = 2 * (BM + BN) * 128, MOST = RING > 131071 ? 163840 : (RING > 65535 ? 81920 : RING);
+    static constexpr int RING = S * (BM + BN) * KBB, MOST = RING > 131071 ? 163840 : (RING > 65535 ? 81920 : RING);
     static constexpr int bytes(int nj) { return NW * LDR * 16 * nj * AS; }
     static constexpr int pick() { int nj = NI; while (nj > 1 && bytes(nj) > MOST) nj /= 2; return nj; }
     static constexpr int NJ = pick();
@@ -296,18 +298,20 @@ template <typename T, int BM, int BN, int WVM, int WVN> struct GaEpi {
 // DMA: operands on 16 bytes, staged by LDS-DMA (the ragged end of K through
 // registers).  Otherwise every slab goes through registers, fetched before the
 // products of the slab ahead of it and written to LDS after them.
-template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, bool GATED, bool DMA>
+template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int KBB, int S, bool GATED, bool DMA>
 __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a) {
     using TR = ga_traits<T>;
     using acc4 = typename TR::acc4;
     using R = typename TR::acc;
     constexpr int NW = WVM * WVN, NT = 64 * NW, NA = GATED ? 2 : 1, BMI = BM / NA;
-    constexpr int WM = BM / WVM, WN = BN / WVN, MI = WM / 16, NI = WN / 16, KB = 128 / (int)sizeof(T);
-    using IA = GaImg<T, BMI, AKC>;
-    using IB = GaImg<T, BN, BKC>;
-    constexpr int SLOT = (BM + BN) * 128;
+    constexpr int WM = BM / WVM, WN = BN / WVN, MI = WM / 16, NI = WN / 16, KB = KBB / (int)sizeof(T);
+    using IA = GaImg<T, BMI, AKC, KBB>;
+    using IB = GaImg<T, BN, BKC, KBB>;
+    constexpr int SLOT = (BM + BN) * KBB;
     constexpr int PA = (IA::CHUNKS + NW - 1) / NW, PB = (IB::CHUNKS + NW - 1) / NW;
     static_assert(MI % NA == 0, "gated tiles pair their fragments");
+    static_assert(S == 2 || DMA, "registers hold one slab");
+    constexpr int LOADS = NA * PA + PB;              // DMA instructions of a wave's slab
     extern __shared__ __align__(16) char smem[];
 
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -324,59 +328,64 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
 
     const i64 rowsA = a.m - m0, rowsB = a.n - n0;
     const bool sum = a.mode == GA_SUM;
-    // product and first k of step s
-    auto step = [&](int s, int& p, i64& k0) {
-        p = pair;
-        if (sum && s >= a.nsteps) { s -= a.nsteps; p = 1; }
-        k0 = (i64)s * KB;
-    };
     auto slabA = [&](int q, i64 k0) { return static_cast<const T*>(a.A[q]) + (AKC ? m0 * a.lda[q] + k0 : m0 + k0 * a.lda[q]); };
     auto slabB = [&](int q, i64 k0) { return static_cast<const T*>(a.B[q]) + (BKC ? n0 * a.ldb[q] + k0 : n0 + k0 * a.ldb[q]); };
 
-    // LDS-DMA
+    // LDS-DMA: where the next slab starts, what a step adds, and the lanes' places
+    // in it.  (All of it in registers: an argument read again in the loop would
+    // cost a scalar load and its wait in every step.)
+    const i64 kfull = a.kfull;
+    const int nsteps = a.nsteps;
+    const char *xa[NA], *xb;
+    i64 da[NA], db;
     uint32_t offA[NA][PA], offB[PB];
-    auto offsets = [&](int p) {
+    auto aim = [&](int p, i64 k0) {
         #pragma unroll
-        for (int h = 0; h < NA; ++h)
+        for (int h = 0; h < NA; ++h) {
+            const int q = GATED ? h : p;
+            const i64 ld = a.lda[q];
+            xa[h] = reinterpret_cast<const char*>(slabA(q, k0));
+            da[h] = (AKC ? KB : KB * ld) * (i64)sizeof(T);
             #pragma unroll
-            for (int i = 0; i < PA; ++i)
-                offA[h][i] = IA::offset(min(wid + i * NW, IA::CHUNKS - 1), lane, a.lda[GATED ? h : p], rowsA);
+            for (int i = 0; i < PA; ++i) offA[h][i] = IA::offset(min(wid + i * NW, IA::CHUNKS - 1), lane, ld, rowsA);
+        }
+        const i64 ld = a.ldb[p];
+        xb = reinterpret_cast<const char*>(slabB(p, k0));
+        db = (BKC ? KB : KB * ld) * (i64)sizeof(T);
         #pragma unroll
-        for (int i = 0; i < PB; ++i)
-            offB[i] = IB::offset(min(wid + i * NW, IB::CHUNKS - 1), lane, a.ldb[p], rowsB);
+        for (int i = 0; i < PB; ++i) offB[i] = IB::offset(min(wid + i * NW, IB::CHUNKS - 1), lane, ld, rowsB);
     };
-    int curp = sum ? (s0 >= a.nsteps ? 1 : 0) : pair;
-    if constexpr (DMA) offsets(curp);
+    int curp = sum ? (s0 >= nsteps ? 1 : 0) : pair;
+    int kt = sum && s0 >= nsteps ? s0 - nsteps : s0;      // step of its product being staged
+    if constexpr (DMA) aim(curp, (i64)kt * KB);
 
     using gptr = const __attribute__((address_space(1))) void*;
     using lptr = __attribute__((address_space(3))) void*;
-    auto issue = [&](int s) {
-        int p;
-        i64 k0;
-        step(s, p, k0);
-        if (sum && p != curp) { curp = p; offsets(p); }
-        char* slot = smem + (s & 1) * SLOT;
-        if (k0 < a.kfull) {
+    // stages one step after the other
+    auto issue = [&](char* slot) {
+        if (sum && kt == nsteps) { kt = 0; curp = 1; aim(1, 0); }
+        const i64 k0 = (i64)kt++ * KB;
+        if (k0 < kfull) {
             #pragma unroll
             for (int h = 0; h < NA; ++h) {
-                const char* X = reinterpret_cast<const char*>(slabA(GATED ? h : p, k0));
                 #pragma unroll
                 for (int i = 0; i < PA; ++i)
                     __builtin_amdgcn_global_load_lds(
-                        (gptr)(X + offA[h][i]),
+                        (gptr)(xa[h] + offA[h][i]),
                         (lptr)(slot + h * IA::BYTES + min(wid + i * NW, IA::CHUNKS - 1) * 1024), 16, 0, 0);
+                xa[h] += da[h];
             }
-            const char* Y = reinterpret_cast<const char*>(slabB(p, k0));
             #pragma unroll
             for (int i = 0; i < PB; ++i)
-                __builtin_amdgcn_global_load_lds((gptr)(Y + offB[i]),
-                                                 (lptr)(slot + BM * 128 + min(wid + i * NW, IB::CHUNKS - 1) * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((gptr)(xb + offB[i]),
+                                                 (lptr)(slot + BM * KBB + min(wid + i * NW, IB::CHUNKS - 1) * 1024), 16, 0, 0);
+            xb += db;
         } else {
             #pragma unroll
             for (int h = 0; h < NA; ++h)
-                IA::template stage<NT>(slabA(GATED ? h : p, k0), a.lda[GATED ? h : p], rowsA, a.k - k0,
+                IA::template stage<NT>(slabA(GATED ? h : curp, k0), a.lda[GATED ? h : curp], rowsA, a.k - k0,
                                        slot + h * IA::BYTES, tid);
-            IB::template stage<NT>(slabB(p, k0), a.ldb[p], rowsB, a.k - k0, slot + BM * 128, tid);
+            IB::template stage<NT>(slabB(curp, k0), a.ldb[curp], rowsB, a.k - k0, slot + BM * KBB, tid);
         }
     };
 
@@ -392,33 +401,44 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
         #pragma unroll
         for (int i = 0; i < CB; ++i) elB[i] = IB::element(min(tid + i * NT, QB - 1), a.ldb[p], rowsB);
     };
-    if constexpr (!DMA) elements(curp);
-    auto fetch = [&](int s) {
-        int p;
-        i64 k0;
-        step(s, p, k0);
-        if (sum && p != curp) { curp = p; elements(p); }
-        const i64 left = a.k - k0;
+    const T *ya[NA], *yb;
+    i64 ea[NA], eb;
+    auto point = [&](int p, i64 k0) {
+        elements(p);
+        #pragma unroll
+        for (int h = 0; h < NA; ++h) {
+            ya[h] = slabA(GATED ? h : p, k0);
+            ea[h] = AKC ? KB : KB * a.lda[GATED ? h : p];
+        }
+        yb = slabB(p, k0);
+        eb = BKC ? KB : KB * a.ldb[p];
+    };
+    if constexpr (!DMA) point(curp, (i64)kt * KB);
+    const i64 kall = a.k;
+    auto fetch = [&]() {
+        if (sum && kt == nsteps) { kt = 0; curp = 1; point(1, 0); }
+        const i64 left = kall - (i64)kt++ * KB;
         const bool inA = left >= KB && (AKC || rowsA >= BMI), inB = left >= KB && (BKC || rowsB >= BN);
         #pragma unroll
         for (int h = 0; h < NA; ++h)
             #pragma unroll
             for (int i = 0; i < CA; ++i)
-                ra[h][i] = IA::fetch(slabA(GATED ? h : p, k0), elA[h][i], min(tid + i * NT, QA - 1), a.lda[GATED ? h : p],
-                                     rowsA, left, inA);
+                ra[h][i] = IA::fetch(ya[h], elA[h][i], min(tid + i * NT, QA - 1), rowsA, left, inA);
         #pragma unroll
-        for (int i = 0; i < CB; ++i)
-            rb[i] = IB::fetch(slabB(p, k0), elB[i], min(tid + i * NT, QB - 1), a.ldb[p], rowsB, left, inB);
+        for (int i = 0; i < CB; ++i) rb[i] = IB::fetch(yb, elB[i], min(tid + i * NT, QB - 1), rowsB, left, inB);
+        #pragma unroll
+        for (int h = 0; h < NA; ++h) ya[h] += ea[h];
+        yb += eb;
     };
     auto write = [&](int s) {
-        char* slot = smem + (s & 1) * SLOT;
+        char* slot = smem + (s % S) * SLOT;
         #pragma unroll
         for (int h = 0; h < NA; ++h)
             #pragma unroll
             for (int i = 0; i < CA; ++i)
                 *reinterpret_cast<i4v*>(slot + h * IA::BYTES + min(tid + i * NT, QA - 1) * 16) = ra[h][i];
         #pragma unroll
-        for (int i = 0; i < CB; ++i) *reinterpret_cast<i4v*>(slot + BM * 128 + min(tid + i * NT, QB - 1) * 16) = rb[i];
+        for (int i = 0; i < CB; ++i) *reinterpret_cast<i4v*>(slot + BM * KBB + min(tid + i * NT, QB - 1) * 16) = rb[i];
     };
 
     const int wm = wid / WVN, wn = wid % WVN;
@@ -431,42 +451,52 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             for (int r = 0; r < 4; ++r) acc[i][j][r] = R(0);
 
     if (s0 < s1) {
-        if constexpr (DMA) issue(s0);
-        else { fetch(s0); write(s0); }
+        if constexpr (DMA) {
+            #pragma unroll
+            for (int i = 0; i < S - 1; ++i)
+                if (s0 + i < s1) issue(smem + (s0 + i) % S * SLOT);
+        } else { fetch(); write(s0); }
     }
     for (int s = s0; s < s1; ++s) {
-        // my part of step s has landed ...
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        // my part of step s has landed (of the steps behind it, LOADS each are in
+        // flight; a step that went through registers waited for all before it) ...
+        if (S > 2 && s + S - 2 < s1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         // ... and everyone's, and everyone has read step s - 1's slot
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + 1 < s1) {
-            if constexpr (DMA) issue(s + 1);
-            else fetch(s + 1);
-        }
-        const char* la = smem + (s & 1) * SLOT;
-        const char* lb = la + BM * 128;
-        #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            i4v fa[MI], fb[NI];
-            #pragma unroll
-            for (int j = 0; j < NI; ++j) fb[j] = IB::frag(lb, wn * WN + j * 16, kk, lane);
-            #pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                constexpr int H = MI / NA;
-                fa[i] = IA::frag(la + (i / H) * IA::BYTES, wm * (WM / NA) + (i % H) * 16, kk, lane);
+        // the slab read and the one filled are different memory: said so, or the
+        // compiler waits for the DMA before each transposed read
+        auto work = [&](const char* __restrict la, char* __restrict fill) __attribute__((always_inline)) {
+            if constexpr (DMA) {
+                if (s + S - 1 < s1) issue(fill);
+            } else if (s + 1 < s1) {
+                fetch();
             }
+            const char* lb = la + BM * KBB;
             #pragma unroll
-            for (int i = 0; i < MI; ++i)
+            for (int kk = 0; kk < KBB / 64; ++kk) {
+                i4v fa[MI], fb[NI];
                 #pragma unroll
-                for (int j = 0; j < NI; ++j) {
-                    // D's four registers run along the rows of the first operand:
-                    // rows of C for f32 sums; for f64 they are 4 apart, and the
-                    // columns take them so that lanes run along the rows
-                    if constexpr (sizeof(R) == 4) acc[i][j] = TR::mma(fa[i], fb[j], acc[i][j]);
-                    else acc[i][j] = TR::mma(fb[j], fa[i], acc[i][j]);
+                for (int j = 0; j < NI; ++j) fb[j] = IB::frag(lb, wn * WN + j * 16, kk, lane);
+                #pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    constexpr int H = MI / NA;
+                    fa[i] = IA::frag(la + (i / H) * IA::BYTES, wm * (WM / NA) + (i % H) * 16, kk, lane);
                 }
-        }
+                #pragma unroll
+                for (int i = 0; i < MI; ++i)
+                    #pragma unroll
+                    for (int j = 0; j < NI; ++j) {
+                        // D's four registers run along the rows of the first operand:
+                        // rows of C for f32 sums; for f64 they are 4 apart, and the
+                        // columns take them so that lanes run along the rows
+                        if constexpr (sizeof(R) == 4) acc[i][j] = TR::mma(fa[i], fb[j], acc[i][j]);
+                        else acc[i][j] = TR::mma(fb[j], fa[i], acc[i][j]);
+                    }
+            }
+        };
+        work(smem + s % S * SLOT, smem + (s + S - 1) % S * SLOT);
         if constexpr (!DMA)
             if (s + 1 < s1) write(s + 1);
     }
@@ -497,7 +527,7 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             }
         return;
     }
-    using EP = GaEpi<T, BM, BN, WVM, WVN>;
+    using EP = GaEpi<T, BM, BN, WVM, WVN, KBB, S>;
     constexpr int NJ = EP::NJ, LDR = EP::LDR, V = 16 / (int)sizeof(T);
     R* img = reinterpret_cast<R*>(smem) + wid * (LDR * 16 * NJ);
     __syncthreads();                                 // every wave has read its last slab

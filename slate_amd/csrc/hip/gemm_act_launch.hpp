@@ -6,10 +6,10 @@ namespace slate_hip {
 
 namespace {
 
-template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, bool GATED, bool DMA>
+template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int KBB, int S, bool GATED, bool DMA>
 void ga_launch(const GemmActArgs& a, hipStream_t s) {
-    constexpr int BMI = GATED ? BM / 2 : BM, LDS = GaEpi<T, BM, BN, WVM, WVN>::LDS;
-    auto kern = gemm_act_kernel<T, AKC, BKC, BM, BN, WVM, WVN, GATED, DMA>;
+    constexpr int BMI = GATED ? BM / 2 : BM, LDS = GaEpi<T, BM, BN, WVM, WVN, KBB, S>::LDS;
+    auto kern = gemm_act_kernel<T, AKC, BKC, BM, BN, WVM, WVN, KBB, S, GATED, DMA>;
     if constexpr (LDS > 65536)
         HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                       LDS));
@@ -22,10 +22,10 @@ void ga_launch(const GemmActArgs& a, hipStream_t s) {
 template <typename T, bool AKC, bool BKC, bool GATED, bool DMA>
 void ga_tile(const GemmActArgs& a, int tile, hipStream_t s) {
     if constexpr (sizeof(T) == 2 && DMA)
-        if (tile == 0) return ga_launch<T, AKC, BKC, 256, 256, 2, 4, GATED, DMA>(a, s);
-    if (tile <= 1) return ga_launch<T, AKC, BKC, 128, 128, 2, 2, GATED, DMA>(a, s);
-    if (tile == 2) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, GATED, DMA>(a, s);
-    return ga_launch<T, AKC, BKC, 128, 16, 4, 1, GATED, DMA>(a, s);
+        if (tile == 0) return ga_launch<T, AKC, BKC, 256, 256, 2, 4, 128, 2, GATED, DMA>(a, s);
+    if (tile <= 1) return ga_launch<T, AKC, BKC, 128, 128, 2, 2, 128, 2, GATED, DMA>(a, s);
+    if (tile == 2) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 128, 2, GATED, DMA>(a, s);
+    return ga_launch<T, AKC, BKC, 128, 16, 4, 1, 128, 2, GATED, DMA>(a, s);
 }
 
 template <typename T, bool GATED, bool DMA>
@@ -54,7 +54,6 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
     // inside a tile; a slab whose last vector would pass the end of the last
     // column goes through registers, as the ragged end of K does
     bool dma = true;
-    a.nsteps = (int)((a.k + KB - 1) / KB);
     a.kfull = a.k / KB * KB;
     auto look = [&](const void* q, i64 ld, bool kc, i64 rows) {
         dma = dma && (uintptr_t)q % 16 == 0 && (ld * ES) % 16 == 0 && (kc ? 256 : KB) * ld * ES < (i64)1 << 31;
@@ -71,6 +70,7 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
     a.splits = p.splits;
     a.per_split = p.per_split;
     a.ldp = p.ldp;
+    a.nsteps = (int)((a.k + KB - 1) / KB);
     if (dma) gated ? ga_layout<T, true, true>(a, akc, bkc, p.tile, s) : ga_layout<T, false, true>(a, akc, bkc, p.tile, s);
     else gated ? ga_layout<T, true, false>(a, akc, bkc, p.tile, s) : ga_layout<T, false, false>(a, akc, bkc, p.tile, s);
     if (p.splits > 1) {

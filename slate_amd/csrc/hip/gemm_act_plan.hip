@@ -25,7 +25,7 @@ GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool 
     // 4096^3 2722 and 2851 us).
     i64 t;
     if (n <= 16) { p.tile = 3; t = tiles(128, 16); }
-    else if (es == 2 && dma && tiles(256, 256) >= 192) { p.tile = 0; t = tiles(256, 256); }
+    else if (es == 2 && dma && k >= 192 && tiles(256, 256) >= 192) { p.tile = 0; t = tiles(256, 256); }
     else if (es < 8 && tiles(128, 128) >= 768) { p.tile = 1; t = tiles(128, 128); }
     else { p.tile = 2; t = tiles(64, 64); }
     // Few tiles: K in pieces of at least 4 steps, up to two workgroups per CU
