@@ -55,14 +55,15 @@ __global__ void __launch_bounds__(64 * AG_WAVES) act_grad_rows_kernel(ActGradArg
     // UN columns' loads are in flight per wave
     constexpr int UN = GATED ? 2 : 4;
     auto column = [&](i64 n, const T* c, const T* z1, const T* z2) {
-        R d1[E], d2[E];
+        R d1[E], d2[E], z[E], v[E], d[E];
+        #pragma unroll
+        for (int e = 0; e < E; ++e) { z[e] = (R)z1[e]; v[e] = R(0); d[e] = R(1); }
+        if (a.Z1) ga_act_grad<FAST, E>(a.act, z, v, d);
         #pragma unroll
         for (int e = 0; e < E; ++e) {
             const R g = (R)c[e];
-            R v = R(0), d = R(1);
-            if (a.Z1) ga_act_grad<FAST>(a.act, (R)z1[e], v, d);
-            if constexpr (GATED) { d1[e] = g * (R)z2[e] * d; d2[e] = g * v; }
-            else { d1[e] = g * d; d2[e] = R(0); }
+            if constexpr (GATED) { d1[e] = g * (R)z2[e] * d[e]; d2[e] = g * v[e]; }
+            else { d1[e] = g * d[e]; d2[e] = R(0); }
             sum[e] += d1[e];
         }
         if (a.dZ1) put(a.dZ1, n, d1);
@@ -116,8 +117,11 @@ __global__ void __launch_bounds__(256) act_grad_cols_kernel(ActGradArgs a, i64 r
     const i64 m0 = (i64)blockIdx.y * rows, m1 = min(a.m, m0 + rows);
     R s = R(0);
     for (i64 m = m0 + lane; m < m1; m += 64) {
-        R v = R(0), d = R(1);
-        if (a.Z1) ga_act_grad<FAST>(a.act, (R) static_cast<const T*>(a.Z1)[m + n * a.ldz1], v, d);
+        R v, d = R(1);
+        if (a.Z1) {
+            const R z = (R) static_cast<const T*>(a.Z1)[m + n * a.ldz1];
+            ga_act_grad<FAST, 1>(a.act, &z, &v, &d);
+        }
         const R g = (R) static_cast<const T*>(a.dC)[m + n * a.lddc] * d;
         if (a.dZ1) static_cast<T*>(a.dZ1)[m + n * a.lddz] = (T)g;
         s += g;

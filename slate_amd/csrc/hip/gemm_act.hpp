@@ -72,51 +72,113 @@ template <> struct ga_traits<double> {
 };
 
 // ------------------------------------------------------------- activations
-// 16-bit results round to 2^-9 at best, so their exponential is the hardware
-// one (a few 2^-24 times the argument); 32- and 64-bit results call exp.
+// On V values at once, the choice of the function outside: V independent chains
+// hide each other's latency.  Results of 16 bits round to 2^-11 at best: their
+// exponential and reciprocal are the hardware's (a few 2^-24 of the argument),
+// 32- and 64-bit results call exp and divide.
 template <bool FAST> __device__ inline float ga_exp(float x) { return FAST ? __expf(x) : expf(x); }
 template <bool FAST> __device__ inline double ga_exp(double x) { return exp(x); }
-template <bool FAST> __device__ inline float ga_div(float a, float b) {
-    return FAST ? a * __builtin_amdgcn_rcpf(b) : a / b;
-}
-template <bool FAST> __device__ inline double ga_div(double a, double b) { return a / b; }
-__device__ inline float ga_erfc(float x) { return erfcf(x); }
-__device__ inline double ga_erfc(double x) { return erfc(x); }
+template <bool FAST> __device__ inline float ga_inv(float b) { return FAST ? __builtin_amdgcn_rcpf(b) : 1.f / b; }
+template <bool FAST> __device__ inline double ga_inv(double b) { return 1.0 / b; }
 
-// Beyond GA_FLAT the smooth activations are 0 (left) or z itself (right) in
+// The normal distribution's function P(z) and e = exp(-z^2 / 2).  For 16-bit
+// results P(-x sqrt 2) = exp(-x^2) f(1 / (1 + 0.43 x)) / 2 with a polynomial f
+// of degree 8 fitted to exp(x^2) erfc(x) on [0, 12] in the relative sense
+// (4.4e-7 in 32-bit arithmetic); P(z) = 1 - P(-z).
+template <bool FAST, typename R> __device__ inline R ga_phi(R z, R& e) {
+    e = ga_exp<FAST>(R(-0.5) * z * z);
+    if constexpr (FAST) {
+        const R t = ga_inv<FAST>(R(1) + R(0.43 * 0.70710678118654752440) * fabsf(z));
+        R f = R(0.0709153654);
+        f = f * t - R(0.299052681);
+        f = f * t + R(0.364768859);
+        f = f * t - R(0.0688474548);
+        f = f * t + R(0.238222132);
+        f = f * t + R(0.207465912);
+        f = f * t + R(0.243989002);
+        f = f * t + R(0.242538687);
+        f = f * t * e * R(0.5);
+        return z < R(0) ? f : R(1) - f;
+    } else if constexpr (sizeof(R) == 4) {
+        return R(0.5) * erfcf(z * R(-0.70710678118654752440));
+    } else {
+        return R(0.5) * erfc(z * R(-0.70710678118654752440));
+    }
+}
+
+// Beyond ga_flat the smooth activations are 0 (left) or z itself (right) in
 // their type: arguments are held inside it, which keeps 0 * inf out.
 template <typename R> __device__ constexpr R ga_flat() { return sizeof(R) == 4 ? R(120) : R(800); }
 
-template <bool FAST, typename R> __device__ inline R ga_act(int act, R z) {
-    if (act == ACT_IDENTITY) return z;
-    if (act == ACT_RELU) return z < R(0) ? R(0) : z;                             // a NaN stays one
-    z = z < -ga_flat<R>() ? -ga_flat<R>() : z;
-    if (act == ACT_GELU) return R(0.5) * z * ga_erfc(z * R(-0.70710678118654752440));
-    if (act == ACT_GELU_TANH) {                                                  // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
-        const R u2 = R(1.59576912160573071176) * (z + R(0.044715) * z * z * z);
-        return ga_div<FAST>(z, R(1) + ga_exp<FAST>(-u2));
-    }
-    return ga_div<FAST>(z, R(1) + ga_exp<FAST>(-z));
-}
-// value and slope at once (the backward pass of a gated product needs both)
-template <bool FAST, typename R> __device__ inline void ga_act_grad(int act, R z, R& v, R& d) {
-    if (act == ACT_IDENTITY) { v = z; d = R(1); return; }
-    if (act == ACT_RELU) { v = z < R(0) ? R(0) : z; d = z > R(0) ? R(1) : (z <= R(0) ? R(0) : z); return; }
-    const R L = ga_flat<R>(), x = z < -L ? -L : (z > L ? L : z);
-    R p, e;                                                                      // v = x p, d = p + x e
-    if (act == ACT_GELU) {
-        p = R(0.5) * ga_erfc(x * R(-0.70710678118654752440));
-        e = R(0.39894228040143267794) * ga_exp<FAST>(R(-0.5) * x * x);
-    } else if (act == ACT_GELU_TANH) {
-        const R u2 = R(1.59576912160573071176) * (x + R(0.044715) * x * x * x);
-        p = ga_div<FAST>(R(1), R(1) + ga_exp<FAST>(-u2));
-        e = p * (R(1) - p) * R(1.59576912160573071176) * (R(1) + R(0.134145) * x * x);
+template <bool FAST, int V, typename R> __device__ inline void ga_act(int act, const R* z, R* y) {
+    constexpr R L = ga_flat<R>();
+    if (act == ACT_IDENTITY) {
+        #pragma unroll
+        for (int r = 0; r < V; ++r) y[r] = z[r];
+    } else if (act == ACT_RELU) {
+        #pragma unroll
+        for (int r = 0; r < V; ++r) y[r] = z[r] < R(0) ? R(0) : z[r];                   // a NaN stays one
+    } else if (act == ACT_GELU) {
+        #pragma unroll
+        for (int r = 0; r < V; ++r) {
+            const R x = z[r] < -L ? -L : z[r];
+            R e;
+            y[r] = x * ga_phi<FAST>(x, e);
+        }
+    } else if (act == ACT_GELU_TANH) {                                                  // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
+        #pragma unroll
+        for (int r = 0; r < V; ++r) {
+            const R x = z[r] < -L ? -L : z[r], u2 = x * (R(1.59576912160573071176) + R(0.07135481627260024519) * x * x);
+            y[r] = x * ga_inv<FAST>(R(1) + ga_exp<FAST>(-u2));
+        }
     } else {
-        p = ga_div<FAST>(R(1), R(1) + ga_exp<FAST>(-x));
-        e = p * (R(1) - p);
+        #pragma unroll
+        for (int r = 0; r < V; ++r) {
+            const R x = z[r] < -L ? -L : z[r];
+            y[r] = x * ga_inv<FAST>(R(1) + ga_exp<FAST>(-x));
+        }
     }
-    v = z > L ? z : x * p;
-    d = p + x * e;
+}
+// values and slopes (the backward pass of a gated product needs both)
+template <bool FAST, int V, typename R> __device__ inline void ga_act_grad(int act, const R* z, R* v, R* d) {
+    constexpr R L = ga_flat<R>();
+    // v = x p, d = p + x e
+    auto put = [&](int r, R x, R p, R e) {
+        v[r] = z[r] > L ? z[r] : x * p;
+        d[r] = p + x * e;
+    };
+    auto in = [&](R x) { return x < -L ? -L : (x > L ? L : x); };
+    if (act == ACT_IDENTITY) {
+        #pragma unroll
+        for (int r = 0; r < V; ++r) { v[r] = z[r]; d[r] = R(1); }
+    } else if (act == ACT_RELU) {
+        #pragma unroll
+        for (int r = 0; r < V; ++r) {
+            v[r] = z[r] < R(0) ? R(0) : z[r];
+            d[r] = z[r] > R(0) ? R(1) : (z[r] <= R(0) ? R(0) : z[r]);
+        }
+    } else if (act == ACT_GELU) {
+        #pragma unroll
+        for (int r = 0; r < V; ++r) {
+            const R x = in(z[r]);
+            R e;
+            const R p = ga_phi<FAST>(x, e);
+            put(r, x, p, e * R(0.39894228040143267794));
+        }
+    } else if (act == ACT_GELU_TANH) {
+        #pragma unroll
+        for (int r = 0; r < V; ++r) {
+            const R x = in(z[r]), u2 = x * (R(1.59576912160573071176) + R(0.07135481627260024519) * x * x);
+            const R p = ga_inv<FAST>(R(1) + ga_exp<FAST>(-u2));
+            put(r, x, p, p * (R(1) - p) * (R(1.59576912160573071176) + R(0.21406444881780073557) * x * x));
+        }
+    } else {
+        #pragma unroll
+        for (int r = 0; r < V; ++r) {
+            const R x = in(z[r]), p = ga_inv<FAST>(R(1) + ga_exp<FAST>(-x));
+            put(r, x, p, p * (R(1) - p));
+        }
+    }
 }
 
 // V rows of column n: the epilogue on finished sums
@@ -133,7 +195,10 @@ __device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, c
     R z[V], y[V];
     if constexpr (GATED) {
         #pragma unroll
-        for (int r = 0; r < V; ++r) { z[r] = s1[r]; y[r] = ga_act<FAST>(a.act, s1[r]) * s2[r]; }
+        for (int r = 0; r < V; ++r) z[r] = s1[r];
+        ga_act<FAST, V>(a.act, z, y);
+        #pragma unroll
+        for (int r = 0; r < V; ++r) y[r] *= s2[r];
     } else {
         const R alpha = (R)a.alpha;
         #pragma unroll
@@ -153,8 +218,7 @@ __device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, c
             #pragma unroll
             for (int r = 0; r < V; ++r) z[r] += x;
         }
-        #pragma unroll
-        for (int r = 0; r < V; ++r) y[r] = ga_act<FAST>(a.act, z[r]);
+        ga_act<FAST, V>(a.act, z, y);
         if (a.R) {
             const T* X = static_cast<const T*>(a.R) + m + n * a.ldr;
             const R beta = (R)a.beta;
