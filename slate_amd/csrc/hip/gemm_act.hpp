@@ -521,48 +521,93 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
                 if (s0 + i < s1) issue(smem + (s0 + i) % S * SLOT);
         } else { fetch(); write(s0); }
     }
-    for (int s = s0; s < s1; ++s) {
-        // my part of step s has landed (of the steps behind it, LOADS each are in
-        // flight; a step that went through registers waited for all before it) ...
-        if (S > 2 && s + S - 2 < s1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * LOADS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        // ... and everyone's, and everyone has read step s - 1's slot
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        // the slab read and the one filled are different memory: said so, or the
-        // compiler waits for the DMA before each transposed read
-        auto work = [&](const char* __restrict la, char* __restrict fill) __attribute__((always_inline)) {
-            if constexpr (DMA) {
-                if (s + S - 1 < s1) issue(fill);
-            } else if (s + 1 < s1) {
-                fetch();
-            }
-            const char* lb = la + BM * KBB;
+    auto reads = [&](const char* la, int kk, i4v (&fa)[MI], i4v (&fb)[NI]) {
+        constexpr int H = MI / NA;
+        #pragma unroll
+        for (int j = 0; j < NI; ++j) fb[j] = IB::frag(la + BM * KBB, wn * WN + j * 16, kk, lane);
+        #pragma unroll
+        for (int i = 0; i < MI; ++i)
+            fa[i] = IA::frag(la + (i / H) * IA::BYTES, wm * (WM / NA) + (i % H) * 16, kk, lane);
+    };
+    auto products = [&](const i4v (&fa)[MI], const i4v (&fb)[NI]) {
+        #pragma unroll
+        for (int i = 0; i < MI; ++i)
             #pragma unroll
-            for (int kk = 0; kk < KBB / 64; ++kk) {
-                i4v fa[MI], fb[NI];
+            for (int j = 0; j < NI; ++j) {
+                // D's four registers run along the rows of the first operand: rows
+                // of C for f32 sums; for f64 they are 4 apart, and the columns take
+                // them so that lanes run along the rows
+                if constexpr (sizeof(R) == 4) acc[i][j] = TR::mma(fa[i], fb[j], acc[i][j]);
+                else acc[i][j] = TR::mma(fb[j], fa[i], acc[i][j]);
+            }
+    };
+    // (In both loops the slab read and the one filled are restrict parameters:
+    // different memory, or the compiler waits for the DMA before each transposed
+    // read.)
+    if constexpr (NW == 8) {
+        // Two waves share a SIMD: one reads its fragments while the other's
+        // products run, in turns of half a step between barriers.  The second
+        // half of the workgroup is one turn behind the first, which costs one
+        // barrier at either end.
+        const bool late = wid >= 4;
+        auto turn = [&]() {
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        turn();
+        if (late) turn();
+        for (int s = s0; s < s1; ++s) {
+            auto work = [&](const char* __restrict la, char* __restrict fill) __attribute__((always_inline)) {
                 #pragma unroll
-                for (int j = 0; j < NI; ++j) fb[j] = IB::frag(lb, wn * WN + j * 16, kk, lane);
-                #pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    constexpr int H = MI / NA;
-                    fa[i] = IA::frag(la + (i / H) * IA::BYTES, wm * (WM / NA) + (i % H) * 16, kk, lane);
+                for (int kk = 0; kk < KBB / 64; ++kk) {
+                    i4v fa[MI], fb[NI];
+                    // the slot behind was read to its end a turn ago by the later half
+                    if (kk == 0 && s + 1 < s1) issue(fill);
+                    reads(la, kk, fa, fb);
+                    // the next slab is there when the first half comes to read it:
+                    // one turn after this for the later half, two for the first
+                    if (kk == KBB / 64 - 1 && late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    turn();
+                    __builtin_amdgcn_s_setprio(1);
+                    products(fa, fb);
+                    __builtin_amdgcn_s_setprio(0);
+                    if (kk == KBB / 64 - 1 && !late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    turn();
+                }
+            };
+            work(smem + s % S * SLOT, smem + (s + S - 1) % S * SLOT);
+        }
+        if (!late) turn();
+    } else {
+        for (int s = s0; s < s1; ++s) {
+            // my part of step s has landed (of the steps behind it, LOADS each are in
+            // flight; a step that went through registers waited for all before it) ...
+            if (S > 2 && s + S - 2 < s1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * LOADS) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            // ... and everyone's, and everyone has read step s - 1's slot
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            auto work = [&](const char* __restrict la, char* __restrict fill) __attribute__((always_inline)) {
+                if constexpr (DMA) {
+                    if (s + S - 1 < s1) issue(fill);
+                } else if (s + 1 < s1) {
+                    fetch();
                 }
                 #pragma unroll
-                for (int i = 0; i < MI; ++i)
-                    #pragma unroll
-                    for (int j = 0; j < NI; ++j) {
-                        // D's four registers run along the rows of the first operand:
-                        // rows of C for f32 sums; for f64 they are 4 apart, and the
-                        // columns take them so that lanes run along the rows
-                        if constexpr (sizeof(R) == 4) acc[i][j] = TR::mma(fa[i], fb[j], acc[i][j]);
-                        else acc[i][j] = TR::mma(fb[j], fa[i], acc[i][j]);
-                    }
-            }
-        };
-        work(smem + s % S * SLOT, smem + (s + S - 1) % S * SLOT);
-        if constexpr (!DMA)
-            if (s + 1 < s1) write(s + 1);
+                for (int kk = 0; kk < KBB / 64; ++kk) {
+                    i4v fa[MI], fb[NI];
+                    reads(la, kk, fa, fb);
+                    products(fa, fb);
+                }
+            };
+            work(smem + s % S * SLOT, smem + (s + S - 1) % S * SLOT);
+            if constexpr (!DMA)
+                if (s + 1 < s1) write(s + 1);
+        }
     }
 
     constexpr int H = MI / NA, WH = WM / NA;
