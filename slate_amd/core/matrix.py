@@ -100,6 +100,7 @@ class BaseMatrix:
     # ---------------------------------------------------------------- copy
     def _clone(self, cls=None, **kw):
         new = _copy.copy(self)
+        new.__dict__.pop("_operand", None)      # what models/ffn.py remembers of a view
         if cls is not None:
             new.__class__ = cls
         for k, v in kw.items():

@@ -23,12 +23,18 @@ template <typename F> void real_dispatch(char dt, F&& f) {
     }
 }
 
-using Mats = std::vector<std::tuple<uintptr_t, i64, uintptr_t, i64, i64, i64>>;
-std::vector<ClipMat> mats(const Mats& v) {
+// six integers per matrix: A, lda, B, ldb, rows, columns
+std::vector<ClipMat> mats(const py::list& v) {
     std::vector<ClipMat> c;
-    c.reserve(v.size());
-    for (auto& [A, lda, B, ldb, m, n] : v)
-        if (m > 0 && n > 0) c.push_back({P(A), W(B), m, n, lda, ldb});
+    const Py_ssize_t n = PyList_GET_SIZE(v.ptr());
+    if (n % 6) throw std::invalid_argument("clip: six integers per matrix are wanted");
+    c.reserve(n / 6);
+    for (Py_ssize_t i = 0; i < n; i += 6) {
+        i64 x[6];
+        for (int j = 0; j < 6; ++j) x[j] = PyLong_AsLongLong(PyList_GET_ITEM(v.ptr(), i + j));
+        if (PyErr_Occurred()) throw py::error_already_set();
+        if (x[4] > 0 && x[5] > 0) c.push_back({P((uintptr_t)x[0]), W((uintptr_t)x[2]), x[4], x[5], x[1], x[3]});
+    }
     return c;
 }
 
@@ -79,15 +85,21 @@ void register_ffn(py::module& m) {
         if (bias_mode && !ws) throw std::invalid_argument("act_grad: workspace missing");
         real_dispatch(dt, [&](auto z) { act_grad<decltype(z)>(a, S(st)); });
     });
-    m.def("clip_ws", [](char ta, const Mats& v) { const auto c = mats(v); return clip_parts(ta, c.data(), (int)c.size()); });
-    m.def("clip_sum", [](char ta, const Mats& v, uintptr_t part, uintptr_t st) {
+    m.def("clip_parts", [](i64 count) { return clip_parts(count); });
+    m.def("clip_norm", [](char ta, char tb, const py::list& v, double limit, uintptr_t part, uintptr_t norm, bool scale,
+                          uintptr_t st) {
+        const auto c = mats(v);
+        const int n = clip_sum(ta, c.data(), (int)c.size(), (double*)W(part), S(st));
+        clip_scale(ta, tb, c.data(), (int)c.size(), limit, (const double*)P(part), n, (double*)W(norm), scale, S(st));
+    });
+    m.def("clip_sum", [](char ta, const py::list& v, uintptr_t part, uintptr_t st) {
         const auto c = mats(v);
         return (i64)clip_sum(ta, c.data(), (int)c.size(), (double*)W(part), S(st));
     });
     m.def("clip_join", [](uintptr_t part, i64 parts, uintptr_t out, uintptr_t st) {
         clip_join((const double*)P(part), (int)parts, (double*)W(out), S(st));
     });
-    m.def("clip_scale", [](char ta, char tb, const Mats& v, double limit, uintptr_t part, i64 parts, uintptr_t norm,
+    m.def("clip_scale", [](char ta, char tb, const py::list& v, double limit, uintptr_t part, i64 parts, uintptr_t norm,
                            bool scale, uintptr_t st) {
         const auto c = mats(v);
         clip_scale(ta, tb, c.data(), (int)c.size(), limit, (const double*)P(part), (int)parts, (double*)W(norm), scale,

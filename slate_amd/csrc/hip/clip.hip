@@ -193,9 +193,12 @@ __global__ void __launch_bounds__(256) clip_join_kernel(const double* part, int 
 int clip_fill(ClipArgs& a, const ClipMat* v, int count, int at, int unit) {
     a.count = std::max(0, std::min(CLIP_MATS, count - at));
     a.first[0] = 0;
+    i64 units = 0;
     for (int i = 0; i < a.count; ++i) {
         a.v[i] = v[at + i];
-        a.first[i + 1] = a.first[i] + (int)((a.v[i].m * a.v[i].n + unit - 1) / unit);
+        units += (a.v[i].m * a.v[i].n + unit - 1) / unit;
+        if (units > 0x7fffffff) throw std::invalid_argument("clip_norm: matrices too large for one call");
+        a.first[i + 1] = (int)units;
     }
     return a.first[a.count];
 }
@@ -218,20 +221,7 @@ void clip_scale_run(const ClipMat* v, int count, double limit, const double* par
 
 static int clip_unit_of(char t) { return t == 'd' ? clip_unit<double>() : t == 's' ? clip_unit<float>() : clip_unit<__bf16>(); }
 
-i64 clip_parts(char ta, const ClipMat* v, int count) {
-    const i64 unit = clip_unit_of(ta);
-    i64 parts = 0;
-    for (int at = 0; at < count; at += CLIP_MATS) {
-        i64 units = 0;
-        for (int i = at; i < std::min(count, at + CLIP_MATS); ++i) {
-            const i64 u = (v[i].m * v[i].n + unit - 1) / unit;
-            if (u + units > 0x7fffffff) throw std::invalid_argument("clip_norm: matrices too large for one call");
-            units += u;
-        }
-        parts += std::min<i64>(CLIP_BLOCKS, units);
-    }
-    return 3 * parts;
-}
+i64 clip_parts(i64 count) { return 3 * CLIP_BLOCKS * ((count + CLIP_MATS - 1) / CLIP_MATS); }
 
 int clip_sum(char ta, const ClipMat* v, int count, double* part, hipStream_t s) {
     int done = 0;

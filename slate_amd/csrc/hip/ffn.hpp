@@ -59,7 +59,7 @@ template <typename T> void act_grad(ActGradArgs a, hipStream_t s);
 // number of matrices.  part: clip_parts() doubles, three (sums of squares of
 // small, ordinary and large elements) per block of the first pass.
 struct ClipMat { const void* A; void* B; i64 m, n, lda, ldb; };
-i64 clip_parts(char ta, const ClipMat* v, int count);
+i64 clip_parts(i64 count);
 int clip_sum(char ta, const ClipMat* v, int count, double* part, hipStream_t s);          // -> partial sums written
 void clip_join(const double* part, int parts, double* out, hipStream_t s);                // all of them as one
 void clip_scale(char ta, char tb, const ClipMat* v, int count, double limit, const double* part, int parts,

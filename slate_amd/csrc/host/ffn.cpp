@@ -136,6 +136,44 @@ void multiply(i64 m, i64 n, i64 k, const std::vector<double>& A, const std::vect
         }
 }
 
+void clip_sum(char ta, const std::vector<i64>& v, double* s) {
+    s[0] = s[1] = s[2] = 0;
+    real_dispatch(ta, [&](auto z) {
+        using T = decltype(z);
+        for (size_t q = 0; q + 5 < v.size(); q += 6)
+            for (i64 j = 0; j < v[q + 5]; ++j)
+                for (i64 i = 0; i < v[q + 4]; ++i) {
+                    const double x = (double)ptr<const T>((uintptr_t)v[q])[i + j * v[q + 1]], a = std::fabs(x);
+                    if (a > 1e145) { const double w = x * 0x1p-600; s[2] += w * w; }
+                    else if (a < 1e-145) { const double w = x * 0x1p600; s[0] += w * w; }
+                    else s[1] += x * x;
+                }
+    });
+}
+
+void clip_scale(char ta, char tb, const std::vector<i64>& v, double limit, const double* s, double* norm_out, bool scale) {
+    double norm;
+    if (s[1] != s[1]) norm = s[1];
+    else if (s[2] > 0) norm = std::sqrt(s[2] + (s[1] * 0x1p-600) * 0x1p-600) * 0x1p600;
+    else if (s[1] > 0) norm = std::sqrt(s[1] + (s[0] * 0x1p-600) * 0x1p-600);
+    else norm = std::sqrt(s[0]) * 0x1p-600;
+    *norm_out = norm;
+    if (!scale) return;
+    const bool cut = norm > limit && norm < std::numeric_limits<double>::infinity();
+    const double f = cut ? limit / norm : 1.0;
+    real_dispatch(ta, [&](auto za) { real_dispatch(tb, [&](auto zb) {
+        using TA = decltype(za); using TB = decltype(zb);
+        for (size_t q = 0; q + 5 < v.size(); q += 6) {
+            if (!cut && v[q] == v[q + 2]) continue;
+            const TA* A = ptr<const TA>((uintptr_t)v[q]);
+            TB* B = ptr<TB>((uintptr_t)v[q + 2]);
+            for (i64 j = 0; j < v[q + 5]; ++j)
+                for (i64 i = 0; i < v[q + 4]; ++i)
+                    B[i + j * v[q + 3]] = put<TB>((double)A[i + j * v[q + 1]] * f);
+        }
+    }); });
+}
+
 }  // namespace
 
 void register_ffn(py::module& m) {
@@ -203,55 +241,24 @@ void register_ffn(py::module& m) {
             }
         });
     });
-    // matrices: (A, lda, B, ldb, m, n); triple: the sums of squares of small,
-    // ordinary and large elements (see csrc/hip/clip.hip)
-    using Mats = std::vector<std::tuple<uintptr_t, i64, uintptr_t, i64, i64, i64>>;
-    m.def("clip_ws", [](char, const Mats&) { return (i64)3; });
-    m.def("clip_sum", [](char ta, const Mats& v, uintptr_t part, uintptr_t) {
-        double s[3] = {0, 0, 0};
-        real_dispatch(ta, [&](auto z) {
-            using T = decltype(z);
-            for (auto& [A, lda, B, ldb, m, n] : v)
-                for (i64 j = 0; j < n; ++j)
-                    for (i64 i = 0; i < m; ++i) {
-                        const double x = (double)ptr<const T>(A)[i + j * lda], a = std::fabs(x);
-                        if (a > 1e145) { const double q = x * 0x1p-600; s[2] += q * q; }
-                        else if (a < 1e-145) { const double q = x * 0x1p600; s[0] += q * q; }
-                        else s[1] += x * x;
-                    }
-        });
-        for (int h = 0; h < 3; ++h) ptr<double>(part)[h] = s[h];
+    // matrices: A, lda, B, ldb, rows, columns one after the other; the sums of
+    // squares of small, ordinary and large elements (see csrc/hip/clip.hip)
+    m.def("clip_parts", [](i64) { return (i64)3; });
+    m.def("clip_sum", [](char ta, const std::vector<i64>& v, uintptr_t part, uintptr_t) {
+        clip_sum(ta, v, ptr<double>(part));
         return (i64)1;
     });
-    m.def("clip_join", [](uintptr_t part, i64 parts, uintptr_t out, uintptr_t) {
-        double s[3] = {0, 0, 0};
-        for (i64 i = 0; i < parts; ++i)
-            for (int h = 0; h < 3; ++h) s[h] += ptr<const double>(part)[3 * i + h];
-        for (int h = 0; h < 3; ++h) ptr<double>(out)[h] = s[h];
+    m.def("clip_join", [](uintptr_t part, i64, uintptr_t out, uintptr_t) {
+        std::memcpy(ptr<void>(out), ptr<const void>(part), 3 * sizeof(double));
     });
-    m.def("clip_scale", [](char ta, char tb, const Mats& v, double limit, uintptr_t part, i64 parts, uintptr_t norm_out,
-                           bool scale, uintptr_t) {
-        double s[3] = {0, 0, 0};
-        for (i64 i = 0; i < parts; ++i)
-            for (int h = 0; h < 3; ++h) s[h] += ptr<const double>(part)[3 * i + h];
-        double norm;
-        if (s[1] != s[1]) norm = s[1];
-        else if (s[2] > 0) norm = std::sqrt(s[2] + (s[1] * 0x1p-600) * 0x1p-600) * 0x1p600;
-        else if (s[1] > 0) norm = std::sqrt(s[1] + (s[0] * 0x1p-600) * 0x1p-600);
-        else norm = std::sqrt(s[0]) * 0x1p-600;
-        *ptr<double>(norm_out) = norm;
-        if (!scale) return;
-        const bool cut = norm > limit && norm < std::numeric_limits<double>::infinity();
-        const double f = cut ? limit / norm : 1.0;
-        real_dispatch(ta, [&](auto za) { real_dispatch(tb, [&](auto zb) {
-            using TA = decltype(za); using TB = decltype(zb);
-            for (auto& [A, lda, B, ldb, m, n] : v) {
-                if (!cut && A == B) continue;
-                for (i64 j = 0; j < n; ++j)
-                    for (i64 i = 0; i < m; ++i)
-                        ptr<TB>(B)[i + j * ldb] = put<TB>((double)ptr<const TA>(A)[i + j * lda] * f);
-            }
-        }); });
+    m.def("clip_scale", [](char ta, char tb, const std::vector<i64>& v, double limit, uintptr_t part, i64,
+                           uintptr_t norm, bool scale, uintptr_t) {
+        clip_scale(ta, tb, v, limit, ptr<const double>(part), ptr<double>(norm), scale);
+    });
+    m.def("clip_norm", [](char ta, char tb, const std::vector<i64>& v, double limit, uintptr_t part, uintptr_t norm,
+                          bool scale, uintptr_t) {
+        clip_sum(ta, v, ptr<double>(part));
+        clip_scale(ta, tb, v, limit, ptr<const double>(part), ptr<double>(norm), scale);
     });
     m.def("gecopy16", [](char ds, char dd, char uplo, char trans, i64 mm, i64 n, uintptr_t A, i64 lda, uintptr_t B,
                          i64 ldb, uintptr_t) {

@@ -51,9 +51,10 @@ class _Opd:
     address, leading dimension, stored and logical shape, whether it enters
     transposed, and the tensor that owns it."""
 
-    __slots__ = ("ptr", "end", "ld", "rows", "cols", "m", "n", "trans", "t")
+    __slots__ = ("ptr", "end", "ld", "rows", "cols", "m", "n", "trans", "t", "dt", "dev", "buf")
 
     def __init__(self, ptr, ld, rows, cols, trans, t):
+        self.dt, self.dev = (None, None) if t is None else (t.dtype, t.device)
         self.ptr, self.ld, self.rows, self.cols, self.trans, self.t = ptr, ld, rows, cols, trans, t
         self.m, self.n = (cols, rows) if trans else (rows, cols)
         self.end = ptr + ((cols - 1) * ld + rows) * _BYTES[t.dtype] if rows and cols else ptr
@@ -81,16 +82,24 @@ def _of_tensor(t, rows, cols, trans=False, name="matrix"):
 
 
 def _opd(M, name="matrix"):
-    """The (one) rank's operand of a view."""
+    """The (one) rank's operand of a view.  A view remembers it, and uses it again
+    while its storage has the same buffer at the same place, whole."""
     s = M.storage
     slot = s.origin_slot
+    x = M.__dict__.get("_operand")
+    if x is not None and s.local.get(slot) is x.buf and s._valid.get(slot) == s.table.version() \
+            and x.trans == (M._op is not Op.NoTrans) and x.t.data_ptr() == x.ptr:
+        return x
     if M._mt == s.mt and M._nt == s.nt and not (M.row0_offset or M.col0_offset) and M.last_mb is None \
             and M.last_nb is None and slot is not None:
-        t = s.local[slot] if s._valid.get(slot) == s.table.version() else s.prepare_local(slot)
-        bc = s.bc
-        return _of_tensor(t, bc.mloc, bc.nloc, M._op is not Op.NoTrans, name)
-    t = M.local_block().data
-    return _of_tensor(t, t.shape[0], t.shape[1], M._op is not Op.NoTrans, name)
+        t, rows, cols = s.prepare_local(slot), s.bc.mloc, s.bc.nloc
+    else:
+        t = M.local_block().data
+        rows, cols = t.shape
+    x = _of_tensor(t, rows, cols, M._op is not Op.NoTrans, name)
+    x.buf = s.local.get(slot)
+    M.__dict__["_operand"] = x
+    return x
 
 
 def _operands(what, names, mats):
@@ -108,14 +117,13 @@ def _operands(what, names, mats):
             raise SlateError(f"{what}: {name} has no tiles (insertLocalTiles)")
         x = _opd(M, name)
         if first is None:
-            first = x.t
-            dt, dev = first.dtype, first.device
+            first, dt, dev = x, x.dt, x.dev
             if dt not in REAL_CODE:
                 raise SlateError(f"{what}: element type {dt} (bfloat16, float16, float32 or float64 are wanted)")
-        elif x.t.dtype != dt:
-            raise SlateError(f"{what}: {name} has type {x.t.dtype}, the others {dt}")
-        elif x.t.device != dev:
-            raise SlateError(f"{what}: {name} is on {x.t.device}, the others on {dev}")
+        elif x.dt is not dt:
+            raise SlateError(f"{what}: {name} has type {x.dt}, the others {dt}")
+        elif x.dev != dev:
+            raise SlateError(f"{what}: {name} is on {x.dev}, the others on {dev}")
         out.append(x)
     return out
 
@@ -238,12 +246,15 @@ def _inc(b):
     return 1 if b.rows > 1 or b.cols <= 1 else b.ld
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 class _on:
     """The operands' device made current (launches and workspaces go there)."""
 
     def __init__(self, t):
         self.ctx = None
-        if t.is_cuda and t.device.index != torch.cuda.current_device():
+        if t.is_cuda and t.device.index != _current_device():
             self.ctx = torch.cuda.device(t.device)
 
     def __enter__(self):
@@ -664,9 +675,9 @@ def _clip_views(mats, what):
             raise SlateError(f"{what}: a matrix has no tiles (insertLocalTiles)")
         x = _opd(M)
         if dt is None:
-            dt, dev, comm = x.t.dtype, x.t.device, s.comm
-        elif x.t.dtype != dt or x.t.device != dev:
-            raise SlateError(f"{what}: the matrices differ in type or device ({x.t.dtype} on {x.t.device}, {dt} on {dev})")
+            dt, dev, comm = x.dt, x.dev, s.comm
+        elif x.dt is not dt or x.dev != dev:
+            raise SlateError(f"{what}: the matrices differ in type or device ({x.dt} on {x.dev}, {dt} on {dev})")
         elif s.comm is not comm and s.comm.ranks != comm.ranks:
             raise SlateError(f"{what}: the matrices differ in communicator")
         out.append(x)
@@ -706,9 +717,9 @@ def _clip(what, limit, A, B):
         return torch.zeros((), dtype=torch.float64)
     vb = va if B is A else _clip_views(B, what)
     t, comm = va[0].t, A[0].storage.comm
-    if len(vb) != len(va) or (vb is not va and vb[0].t.device != t.device):
+    if len(vb) != len(va) or (vb is not va and vb[0].dev != va[0].dev):
         raise SlateError(f"{what}: B has {len(vb)} matrices, A has {len(va)}, or they are on different devices")
-    ta, tb = t.dtype, vb[0].t.dtype
+    ta, tb = va[0].dt, vb[0].dt
     if _PARTS.get(ta, ta) not in REAL_CODE or not (ta == tb or (_BYTES[ta] == 2 and tb == torch.float32)):
         raise SlateError(f"{what}: no scaling from {ta} to {tb}")
     two = 2 if ta in _PARTS else 1
@@ -719,21 +730,28 @@ def _clip(what, limit, A, B):
                 if x.trans != y.trans or x.rows != y.rows or x.cols != y.cols or \
                         (comm.size > 1 and (X.m() != Y.m() or X.n() != Y.n() or not _same_place(X, Y))):
                     raise SlateError(f"{what}: B's matrices want the shapes, ops and distribution of A's")
-        if limit is not None and len({y.ptr for y in vb if y.end > y.ptr}) < sum([y.end > y.ptr for y in vb]):
-            raise SlateError(f"{what}: a matrix is in the list twice")
+        if limit is not None:
+            full = [y.ptr for y in vb if y.end > y.ptr]
+            if len(set(full)) < len(full):
+                raise SlateError(f"{what}: a matrix is in the list twice")
         mod, st = kmod(t), raw_stream(t)
-        mats = [(x.ptr, x.ld * two, y.ptr, y.ld * two, x.rows * two, x.cols) for x, y in zip(va, vb)]
+        # (A, lda, B, ldb, rows, columns) of every matrix; complex ones as pairs
+        mats = []
+        for x, y in zip(va, vb):
+            mats += (x.ptr, x.ld * two, y.ptr, y.ld * two, x.rows * two, x.cols)
+        top, scale = (0.0, False) if limit is None else (limit, True)
         with _on(t):
             # [norm, the ranks' common sums (3), partial sums]
-            ws = torch.empty(mod.clip_ws(ca, mats) + 4, dtype=torch.float64, device=t.device)
+            ws = torch.empty(4 + mod.clip_parts(len(va)), dtype=torch.float64, device=t.device)
             norm = ws.data_ptr()
             part = norm + 32
-            n = mod.clip_sum(ca, mats, part, st)
-            if comm.size > 1:
+            if comm.size == 1:
+                mod.clip_norm(ca, cb, mats, top, part, norm, scale, st)
+            else:
+                n = mod.clip_sum(ca, mats, part, st)
                 mod.clip_join(part, n, norm + 8, st)
                 comm.allreduce(ws[1:4], "sum")
-                part, n = norm + 8, 1
-            mod.clip_scale(ca, cb, mats, 0.0 if limit is None else limit, part, n, norm, limit is not None, st)
+                mod.clip_scale(ca, cb, mats, top, norm + 8, 1, norm, scale, st)
         if limit is not None:
             _modified(*B)
     return ws[0]

@@ -124,21 +124,36 @@ def _write_svg(path, allev, width=1600, row_h=20):
         f.write("\n".join(out))
 
 
+class trace_block:
+    """``with trace_block(name):`` -- one traced region.  Every region is also
+    a library region for the watchdog: it checks staleness only while some
+    driver is running, and every region entry / exit is a heartbeat."""
+
+    __slots__ = ("name", "span")
+
+    def __init__(self, name):
+        self.name = name
+        self.span = None
+
+    def __enter__(self):
+        _wd.enter(self.name)
+        if _rec.is_on():
+            try:
+                self.span = _traced(self.name)
+                self.span.__enter__()
+            except BaseException:
+                _wd.leave(self.name)
+                raise
+
+    def __exit__(self, *exc):
+        try:
+            if self.span is not None:
+                return self.span.__exit__(*exc)
+        finally:
+            _wd.leave(self.name)
+
+
 @contextlib.contextmanager
-def trace_block(name):
-    # every traced region is also a library region for the watchdog: it
-    # checks staleness only while some driver is running, and every region
-    # entry / exit is a heartbeat
-    _wd.enter(name)
-    try:
-        if not _rec.is_on():
-            yield
-            return
-        yield from _traced(name)
-    finally:
-        _wd.leave(name)
-
-
 def _traced(name):
     depth = getattr(_nest, "d", 0)
     _nest.d = depth + 1
