@@ -301,17 +301,19 @@ template <typename T, int R, bool KC, int KBB> struct GaImg {
             else return __builtin_bit_cast(i4v, d2{(double)v[0], (double)v[1]});
         }
     }
-    // bytes from the slab's first element that lane `lane` of chunk c stages;
-    // rows past the matrix read a row that exists and feed no stored output
-    __device__ static inline uint32_t offset(int c, int lane, i64 ld, i64 rows) {
+    // bytes from the slab's first element that lane `lane` of piece c (64 accesses
+    // of W bytes) stages; rows past the matrix read one that exists and feed no
+    // stored output
+    template <int W> __device__ static inline uint32_t offset(int c, int lane, i64 ld, i64 rows) {
+        const int at = (c * 64 + lane) * W, e = at % 16 / ES, half = W < ES ? at % ES : 0;
         int r, k;
-        src_of(c * 64 + lane, r, k);
+        src_of(at / 16, r, k);
         if constexpr (KC) {
             const i64 rr = r < rows ? r : rows - 1;
-            return (uint32_t)((rr * ld + k) * ES);
+            return (uint32_t)((rr * ld + k + e) * ES + half);
         } else {
-            const i64 rr = r < rows ? r : 0;
-            return (uint32_t)((k * ld + rr) * ES);
+            const i64 rr = W < 16 ? min((i64)(r + e), rows - 1) : r < rows ? r : 0;
+            return (uint32_t)((k * ld + rr) * ES + half);
         }
     }
     // 16-byte slot q of the slab at X, off elements from X, at any alignment; zeros
@@ -359,10 +361,13 @@ template <typename T, int BM, int BN, int WVM, int WVN, int KBB, int S> struct G
 };
 
 // ------------------------------------------------------------------ kernel
-// DMA: operands on 16 bytes, staged by LDS-DMA (the ragged end of K through
-// registers).  Otherwise every slab goes through registers, fetched before the
-// products of the slab ahead of it and written to LDS after them.
-template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int KBB, int S, bool GATED, bool DMA>
+// DMA: bytes of an LDS-DMA access (the ragged end of K goes through registers).
+// 16 where the operands' rows lie on 16 bytes, 4 for 32- and 64-bit elements
+// elsewhere: four times the instructions, still asynchronous (1503 x 777 x 1001
+// f32: 38 us against 53 us through registers).  0: every slab goes through
+// registers, fetched before the products of the slab ahead of it and written to
+// LDS after them.
+template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int KBB, int S, bool GATED, int DMA>
 __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a) {
     using TR = ga_traits<T>;
     using acc4 = typename TR::acc4;
@@ -372,9 +377,11 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
     using IA = GaImg<T, BMI, AKC, KBB>;
     using IB = GaImg<T, BN, BKC, KBB>;
     constexpr int SLOT = (BM + BN) * KBB;
-    constexpr int PA = (IA::CHUNKS + NW - 1) / NW, PB = (IB::CHUNKS + NW - 1) / NW;
+    constexpr int W = DMA ? DMA : 16, PCA = IA::BYTES / (64 * W), PCB = IB::BYTES / (64 * W);    // pieces of a slab
+    constexpr int PA = (PCA + NW - 1) / NW, PB = (PCB + NW - 1) / NW;
     static_assert(MI % NA == 0, "gated tiles pair their fragments");
     static_assert(S == 2 || DMA, "registers hold one slab");
+    static_assert(W == 16 || W <= (int)sizeof(T), "an access lies in one element");
     constexpr int LOADS = NA * PA + PB;              // DMA instructions of a wave's slab
     extern __shared__ __align__(16) char smem[];
 
@@ -411,13 +418,13 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             xa[h] = reinterpret_cast<const char*>(slabA(q, k0));
             da[h] = (AKC ? KB : KB * ld) * (i64)sizeof(T);
             #pragma unroll
-            for (int i = 0; i < PA; ++i) offA[h][i] = IA::offset(min(wid + i * NW, IA::CHUNKS - 1), lane, ld, rowsA);
+            for (int i = 0; i < PA; ++i) offA[h][i] = IA::template offset<W>(min(wid + i * NW, PCA - 1), lane, ld, rowsA);
         }
         const i64 ld = a.ldb[p];
         xb = reinterpret_cast<const char*>(slabB(p, k0));
         db = (BKC ? KB : KB * ld) * (i64)sizeof(T);
         #pragma unroll
-        for (int i = 0; i < PB; ++i) offB[i] = IB::offset(min(wid + i * NW, IB::CHUNKS - 1), lane, ld, rowsB);
+        for (int i = 0; i < PB; ++i) offB[i] = IB::template offset<W>(min(wid + i * NW, PCB - 1), lane, ld, rowsB);
     };
     int curp = sum ? (s0 >= nsteps ? 1 : 0) : pair;
     int kt = sum && s0 >= nsteps ? s0 - nsteps : s0;      // step of its product being staged
@@ -425,6 +432,10 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
 
     using gptr = const __attribute__((address_space(1))) void*;
     using lptr = __attribute__((address_space(3))) void*;
+    auto to_lds = [](const char* p, char* q) {
+        if constexpr (DMA == 4) __builtin_amdgcn_global_load_lds((gptr)p, (lptr)q, 4, 0, 0);
+        else __builtin_amdgcn_global_load_lds((gptr)p, (lptr)q, 16, 0, 0);
+    };
     // stages one step after the other
     auto issue = [&](char* slot) {
         if (sum && kt == nsteps) { kt = 0; curp = 1; aim(1, 0); }
@@ -434,15 +445,12 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             for (int h = 0; h < NA; ++h) {
                 #pragma unroll
                 for (int i = 0; i < PA; ++i)
-                    __builtin_amdgcn_global_load_lds(
-                        (gptr)(xa[h] + offA[h][i]),
-                        (lptr)(slot + h * IA::BYTES + min(wid + i * NW, IA::CHUNKS - 1) * 1024), 16, 0, 0);
+                    to_lds(xa[h] + offA[h][i], slot + h * IA::BYTES + min(wid + i * NW, PCA - 1) * (64 * W));
                 xa[h] += da[h];
             }
             #pragma unroll
             for (int i = 0; i < PB; ++i)
-                __builtin_amdgcn_global_load_lds((gptr)(xb + offB[i]),
-                                                 (lptr)(slot + BM * KBB + min(wid + i * NW, IB::CHUNKS - 1) * 1024), 16, 0, 0);
+                to_lds(xb + offB[i], slot + BM * KBB + min(wid + i * NW, PCB - 1) * (64 * W));
             xb += db;
         } else {
             #pragma unroll

@@ -6,7 +6,7 @@ namespace slate_hip {
 
 namespace {
 
-template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int KBB, int S, bool GATED, bool DMA>
+template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int KBB, int S, bool GATED, int DMA>
 void ga_launch(const GemmActArgs& a, hipStream_t s) {
     constexpr int BMI = GATED ? BM / 2 : BM, LDS = GaEpi<T, BM, BN, WVM, WVN, KBB, S>::LDS;
     auto kern = gemm_act_kernel<T, AKC, BKC, BM, BN, WVM, WVN, KBB, S, GATED, DMA>;
@@ -19,16 +19,17 @@ void ga_launch(const GemmActArgs& a, hipStream_t s) {
     HIP_LAUNCH_CHECK();
 }
 
-template <typename T, bool AKC, bool BKC, bool GATED, bool DMA>
+template <typename T, bool AKC, bool BKC, bool GATED, int DMA>
 void ga_tile(const GemmActArgs& a, int tile, hipStream_t s) {
-    if constexpr (sizeof(T) == 2 && DMA)
+    if constexpr (sizeof(T) == 2 && DMA == 16)
         if (tile == 0) return ga_launch<T, AKC, BKC, 256, 256, 2, 4, 128, 2, GATED, DMA>(a, s);
-    if (tile <= 1) return ga_launch<T, AKC, BKC, 128, 128, 2, 2, 128, 2, GATED, DMA>(a, s);
-    if (tile == 2) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 128, 2, GATED, DMA>(a, s);
+    if constexpr (sizeof(T) == 2)
+        if (tile == 1) return ga_launch<T, AKC, BKC, 128, 128, 2, 2, 128, 2, GATED, DMA>(a, s);
+    if (tile <= 2) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 128, 2, GATED, DMA>(a, s);
     return ga_launch<T, AKC, BKC, 128, 16, 4, 1, 128, 2, GATED, DMA>(a, s);
 }
 
-template <typename T, bool GATED, bool DMA>
+template <typename T, bool GATED, int DMA>
 void ga_layout(const GemmActArgs& a, bool akc, bool bkc, int tile, hipStream_t s) {
     if (akc) bkc ? ga_tile<T, true, true, GATED, DMA>(a, tile, s) : ga_tile<T, true, false, GATED, DMA>(a, tile, s);
     else bkc ? ga_tile<T, false, true, GATED, DMA>(a, tile, s) : ga_tile<T, false, false, GATED, DMA>(a, tile, s);
@@ -53,10 +54,11 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
     // LDS-DMA moves 16 bytes from 16-byte-aligned addresses at 32-bit offsets
     // inside a tile; a slab whose last vector would pass the end of the last
     // column goes through registers, as the ragged end of K does
-    bool dma = true;
+    bool dma = true, small = true;       // 32-bit offsets: `small`
     a.kfull = a.k / KB * KB;
     auto look = [&](const void* q, i64 ld, bool kc, i64 rows) {
-        dma = dma && (uintptr_t)q % 16 == 0 && (ld * ES) % 16 == 0 && (kc ? 256 : KB) * ld * ES < (i64)1 << 31;
+        small = small && (kc ? 256 : KB) * ld * ES < (i64)1 << 31;
+        dma = dma && small && (uintptr_t)q % 16 == 0 && (ld * ES) % 16 == 0;
         if (!kc && rows % E && a.k) a.kfull = std::min<i64>(a.kfull, (a.k - 1) / KB * KB);
     };
     for (int i = 0; i < na; ++i) look(a.A[i], a.lda[i], akc, a.m);
@@ -71,8 +73,15 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
     a.per_split = p.per_split;
     a.ldp = p.ldp;
     a.nsteps = (int)((a.k + KB - 1) / KB);
-    if (dma) gated ? ga_layout<T, true, true>(a, akc, bkc, p.tile, s) : ga_layout<T, false, true>(a, akc, bkc, p.tile, s);
-    else gated ? ga_layout<T, true, false>(a, akc, bkc, p.tile, s) : ga_layout<T, false, false>(a, akc, bkc, p.tile, s);
+    if (dma) {
+        gated ? ga_layout<T, true, 16>(a, akc, bkc, p.tile, s) : ga_layout<T, false, 16>(a, akc, bkc, p.tile, s);
+    } else if (ES >= 4 && small) {
+        a.kfull = a.k / KB * KB;           // no access passes an element
+        if constexpr (ES >= 4)
+            gated ? ga_layout<T, true, 4>(a, akc, bkc, p.tile, s) : ga_layout<T, false, 4>(a, akc, bkc, p.tile, s);
+    } else {
+        gated ? ga_layout<T, true, 0>(a, akc, bkc, p.tile, s) : ga_layout<T, false, 0>(a, akc, bkc, p.tile, s);
+    }
     if (p.splits > 1) {
         constexpr int V = 16 / (int)sizeof(typename ga_traits<T>::acc);
         const dim3 grid((unsigned)(((a.m + V - 1) / V * a.n + 63) / 64), 1, a.mode == GA_PAIR ? 2 : 1);

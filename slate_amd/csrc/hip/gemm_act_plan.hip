@@ -19,14 +19,14 @@ GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool 
     auto tiles = [&](i64 bm, i64 bn) { return ((rows + bm - 1) / bm) * ((n + bn - 1) / bn) * pairs; };
     // A larger tile reads less per flop, a smaller one fills the CUs with
     // several workgroups whose loads and epilogues overlap.  Measured at
-    // 2000^3 bf16: 41 us with 64 x 64, 49 us with 128 x 128; f32 138 and 162;
-    // at 4096^3 bf16: 245, 163 and 138 us with 256 x 256; f32 1013 and 971.
-    // f64 keeps 64 x 64 (its 128 x 128 tile runs one workgroup per CU:
-    // 4096^3 2722 and 2851 us).
+    // 2000^3 bf16: 41 us with 64 x 64, 49 us with 128 x 128; at 4096^3 245, 163
+    // and 138 us with 256 x 256.  32- and 64-bit products wait for the MFMAs,
+    // not for what a larger tile saves: f32 133 us at 2000^3 (128 x 128: 143 in
+    // two pieces), 992 at 4096^3 (967 to 1010), f64 290 (350) and 2220 (2720).
     i64 t;
     if (n <= 16) { p.tile = 3; t = tiles(128, 16); }
     else if (es == 2 && dma && k >= 192 && tiles(256, 256) >= 192) { p.tile = 0; t = tiles(256, 256); }
-    else if (es < 8 && tiles(128, 128) >= 768) { p.tile = 1; t = tiles(128, 128); }
+    else if (es == 2 && tiles(128, 128) >= 768) { p.tile = 1; t = tiles(128, 128); }
     else { p.tile = 2; t = tiles(64, 64); }
     // Few tiles: K in pieces of at least 4 steps, up to two workgroups per CU
     // (64 columns, 1024 x 4096 bf16: 13 us in 16 pieces, 20 us in 4).
