@@ -36,6 +36,7 @@ struct GemmActArgs {
 // tile -1: the kernel for few columns; bytes: workspace.
 struct GemmActPlan { int tile = 0, splits = 1, per_split = 0; i64 ldp = 0, bytes = 0; };
 GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool bkc, bool dma);
+bool gemm_act_pack(int mode, i64 m, i64 n, i64 k);    // lay operands whose rows lie across 16 bytes out anew?
 // Launches and returns 0, or returns the workspace wanted where part is null.
 template <typename T> i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s);
 

@@ -777,6 +777,33 @@ __global__ void __launch_bounds__(64 * NW) gemm_act_skinny_kernel(GemmActArgs a)
     }
 }
 
+// 16-bit columns laid out anew on 16 bytes, so that LDS-DMA takes them; a
+// thread moves four 16-byte vectors.
+template <typename T>
+__global__ void __launch_bounds__(256) ga_pack_kernel(const T* X, i64 ld, T* Y, i64 len, i64 cols) {
+    constexpr int E = 16 / (int)sizeof(T), U = 4;
+    using vE = ga_vec<T, E>;
+    const i64 nv = (len + E - 1) / E, first = (i64)blockIdx.x * (256 * U), c0 = first / nv;
+    const uint32_t r0 = (uint32_t)(first - c0 * nv) + threadIdx.x, nv32 = (uint32_t)nv;
+    vE v[U];
+    #pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t r = r0 + u * 256, q = r / nv32;
+        const i64 c = c0 + q, i = (i64)(r - q * nv32) * E;
+        if (c >= cols) continue;
+        const T* x = X + c * ld + i;
+        if (i + E <= len) v[u] = *reinterpret_cast<const vE*>(x);
+        else
+            #pragma unroll
+            for (int e = 0; e < E; ++e) v[u][e] = i + e < len ? x[e] : (T)0;
+    }
+    #pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t r = r0 + u * 256, q = r / nv32;
+        if (c0 + q < cols) *reinterpret_cast<vE*>(Y + (first + threadIdx.x + u * 256) * E) = v[u];
+    }
+}
+
 // Adds the partial sums and finishes them: 64 threads along the outputs, 4
 // along the pieces of K, so that small outputs (where K is split) keep enough
 // loads in flight; the order of the sums depends on the plan alone.

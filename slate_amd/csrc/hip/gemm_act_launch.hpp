@@ -25,7 +25,9 @@ void ga_tile(const GemmActArgs& a, int tile, hipStream_t s) {
         if (tile == 0) return ga_launch<T, AKC, BKC, 256, 256, 2, 4, 128, 2, GATED, DMA>(a, s);
     if constexpr (sizeof(T) == 2)
         if (tile == 1) return ga_launch<T, AKC, BKC, 128, 128, 2, 2, 128, 2, GATED, DMA>(a, s);
-    if (tile <= 2) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 128, 2, GATED, DMA>(a, s);
+    if constexpr (sizeof(T) == 2 && DMA == 16)
+        if (tile == 4) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 128, 3, GATED, DMA>(a, s);
+    if (tile == 2) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 128, 2, GATED, DMA>(a, s);
     return ga_launch<T, AKC, BKC, 128, 16, 4, 1, 128, 2, GATED, DMA>(a, s);
 }
 
@@ -33,6 +35,57 @@ template <typename T, bool GATED, int DMA>
 void ga_layout(const GemmActArgs& a, bool akc, bool bkc, int tile, hipStream_t s) {
     if (akc) bkc ? ga_tile<T, true, true, GATED, DMA>(a, tile, s) : ga_tile<T, true, false, GATED, DMA>(a, tile, s);
     else bkc ? ga_tile<T, false, true, GATED, DMA>(a, tile, s) : ga_tile<T, false, false, GATED, DMA>(a, tile, s);
+}
+
+// One operand as it is stored: columns of len elements
+struct GaOperand {
+    const void** ptr;
+    i64* ld;
+    i64 len, cols;
+    bool kc;                 // columns run along k
+    bool bad = false;        // rows not on 16 bytes, or 32-bit offsets too short
+    i64 at = -1;             // its place in the workspace
+    bool fits(i64 l, int es) const { return (kc ? 256 : 128 / es) * l * es < (i64)1 << 31; }
+    i64 whole() const { return (len + 7) / 8 * 8; }
+};
+
+// can all operands that need it be laid out anew?
+inline bool ga_packed(const GaOperand* op, int n, int es) {
+    for (int i = 0; i < n; ++i)
+        if (op[i].bad && !op[i].fits(op[i].whole(), es)) return false;
+    return true;
+}
+
+// their places behind the first `bytes` of the workspace; -> its size.  (Both
+// products of a pair often share an operand, which is laid out once.)
+inline i64 ga_place(GaOperand* op, int n, int es, i64 bytes) {
+    for (int i = 0; i < n; ++i) {
+        if (!op[i].bad) continue;
+        for (int j = 0; j < i && op[i].at < 0; ++j)
+            if (op[j].at >= 0 && *op[j].ptr == *op[i].ptr && *op[j].ld == *op[i].ld && op[j].len == op[i].len &&
+                op[j].cols == op[i].cols)
+                op[i].at = op[j].at;
+        if (op[i].at >= 0) continue;
+        op[i].at = bytes;
+        bytes += (op[i].whole() * op[i].cols * es + 255) / 256 * 256;
+    }
+    return bytes;
+}
+
+template <typename T> void ga_pack(GaOperand* op, int n, char* ws, hipStream_t s) {
+    for (int i = 0; i < n; ++i) {
+        if (op[i].at < 0) continue;
+        T* y = reinterpret_cast<T*>(ws + op[i].at);
+        bool done = false;
+        for (int j = 0; j < i; ++j) done = done || op[j].at == op[i].at;
+        const i64 nv = op[i].whole() / 8, ld = op[i].whole();
+        if (!done && nv * op[i].cols)
+            hipLaunchKernelGGL((ga_pack_kernel<T>), dim3((unsigned)((nv * op[i].cols + 1023) / 1024)), dim3(256), 0, s,
+                               static_cast<const T*>(*op[i].ptr), *op[i].ld, y, op[i].len, op[i].cols);
+        HIP_LAUNCH_CHECK();
+        *op[i].ptr = y;
+        *op[i].ld = ld;
+    }
 }
 
 template <typename T, int NF> void ga_skinny(const GemmActArgs& a, bool gated, hipStream_t s) {
@@ -55,20 +108,35 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
     // inside a tile; a slab whose last vector would pass the end of the last
     // column goes through registers, as the ragged end of K does
     bool dma = true, small = true;       // 32-bit offsets: `small`
-    a.kfull = a.k / KB * KB;
-    auto look = [&](const void* q, i64 ld, bool kc, i64 rows) {
-        small = small && (kc ? 256 : KB) * ld * ES < (i64)1 << 31;
-        dma = dma && small && (uintptr_t)q % 16 == 0 && (ld * ES) % 16 == 0;
-        if (!kc && rows % E && a.k) a.kfull = std::min<i64>(a.kfull, (a.k - 1) / KB * KB);
+    GaOperand op[4];
+    int nop = 0;
+    auto look = [&](const void*& q, i64& ld, bool kc, i64 rows) {
+        GaOperand x{&q, &ld, kc ? a.k : rows, kc ? rows : a.k, kc};
+        const bool fits = x.fits(ld, ES);
+        x.bad = !fits || (uintptr_t)q % 16 != 0 || (ld * ES) % 16 != 0;
+        small = small && fits;
+        dma = dma && !x.bad;
+        op[nop++] = x;
     };
     for (int i = 0; i < na; ++i) look(a.A[i], a.lda[i], akc, a.m);
     for (int i = 0; i < nb; ++i) look(a.B[i], a.ldb[i], bkc, a.n);
-    const GemmActPlan p = gemm_act_plan(ES, a.mode, a.m, a.n, a.k, akc, bkc, dma);
-    if (p.bytes && !a.part) return p.bytes;
+    const bool pack = ES == 2 && !dma && gemm_act_pack(a.mode, a.m, a.n, a.k) && ga_packed(op, nop, ES);
+    const GemmActPlan p = gemm_act_plan(ES, a.mode, a.m, a.n, a.k, akc, bkc, dma || pack);
     if (p.tile < 0) {
         ga_skinny<T, 1>(a, gated, s);
         return 0;
     }
+    i64 bytes = (p.bytes + 255) / 256 * 256;
+    if (pack) bytes = ga_place(op, nop, ES, bytes);
+    if (bytes && !a.part) return bytes;
+    if constexpr (ES == 2)
+        if (pack) {
+            dma = true;
+            ga_pack<T>(op, nop, static_cast<char*>(a.part), s);
+        }
+    a.kfull = a.k / KB * KB;
+    for (int i = 0; i < nop; ++i)
+        if (!op[i].kc && op[i].len % E && op[i].at < 0 && a.k) a.kfull = std::min<i64>(a.kfull, (a.k - 1) / KB * KB);
     a.splits = p.splits;
     a.per_split = p.per_split;
     a.ldp = p.ldp;

@@ -795,3 +795,31 @@ def test_no_host_sync():
         step()
     finally:
         torch.cuda.set_sync_debug_mode("default")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT", "TT"])
+@pytest.mark.parametrize("m,n,k", [(4090, 260, 4000), (1020, 2040, 1500), (1030, 250, 8200), (2000, 4100, 1000),
+                                   (1640, 4040, 5000), (8190, 510, 300), (200, 130, 5000), (70, 40, 65)])
+def test_half_tiles(dt, ta, tb, m, n, k):
+    """16-bit tiles of 64, 128 and 256 rows, two and three slots, with K in one piece and in several."""
+    Product(dt, "cuda", m, n, k, ta, tb, act="gelu", pad=-m % 8 if ta == "N" else -k % 8).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT", "TT"])
+@pytest.mark.parametrize("pad,off", [(0, 0), (3, 1)])
+def test_half_unaligned(dt, ta, tb, pad, off):
+    """Large operands whose columns lie across 16 bytes; what lies between the columns (NaN) is not used."""
+    Product(dt, "cuda", 2053, 2049, 2051, ta, tb, act="silu", pad=pad, off=off).check()
+    Gated(dt, "cuda", 1101, 2051, 2053, ta, tb, pad=pad, off=off).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN"])
+def test_half_unaligned_grad(dt, ta, tb):
+    grad_call(Product(dt, "cuda", 2051, 2049, 2053, ta, tb, pad=3), "gelu")
+    Gated(dt, "cuda", 1103, 2049, 2051, ta, tb, pad=1, off=3).check_grad()
