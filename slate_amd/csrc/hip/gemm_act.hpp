@@ -249,10 +249,18 @@ __device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, c
         if (a.Z[1]) put(static_cast<T*>(a.Z[1]) + m + n * a.ldz[1], s2, whole);
 }
 
+// W bytes per lane from p to q + W lane (q: of the wave), asynchronously
+template <int W> __device__ inline void ga_to_lds(const void* p, void* q) {
+    using gptr = const __attribute__((address_space(1))) void*;
+    using lptr = __attribute__((address_space(3))) void*;
+    if constexpr (W == 4) __builtin_amdgcn_global_load_lds((gptr)p, (lptr)q, 4, 0, 0);
+    else __builtin_amdgcn_global_load_lds((gptr)p, (lptr)q, 16, 0, 0);
+}
+
 // ------------------------------------------------------------- LDS images
-template <typename T, int R, bool KC, int KBB> struct GaImg {
-    static constexpr int ES = sizeof(T), E = 16 / ES, KB = KBB / ES, NC = KBB / 16;
-    static constexpr int BYTES = R * KBB, CHUNKS = BYTES / 1024;
+template <typename T, int R, bool KC> struct GaImg {
+    static constexpr int ES = sizeof(T), E = 16 / ES, KB = 128 / ES;
+    static constexpr int BYTES = R * 128;
     static constexpr int ROWB = R * ES;                       // MN: bytes per k
     static constexpr int SEGB = 16 * ES;                      // MN: bytes of a 16-row segment
     static constexpr int NSEG = R / 16;
@@ -263,12 +271,12 @@ template <typename T, int R, bool KC, int KBB> struct GaImg {
         else return (k >> 1) & 1 & (NSEG - 1);
     }
     // KC: 16 rows of one chunk column lie in 16 distinct 16-byte slots
-    __device__ static constexpr int turn(int r) { return NC == 8 ? (r >> 1) & 7 : (r >> 2) & 3; }
+    __device__ static constexpr int turn(int r) { return (r >> 1) & 7; }
     // row and k of the first element of 16-byte slot q
     __device__ static inline void src_of(int q, int& r, int& k) {
         if constexpr (KC) {
-            r = q / NC;
-            k = ((q % NC) ^ turn(r)) * E;
+            r = q / 8;
+            k = ((q % 8) ^ turn(r)) * E;
         } else {
             const int p = q * 16;
             k = p / ROWB;
@@ -280,7 +288,7 @@ template <typename T, int R, bool KC, int KBB> struct GaImg {
         const int l = lane & 15, g = lane >> 4;
         if constexpr (KC) {
             const int r = r0 + l;
-            return *reinterpret_cast<const i4v*>(img + r * KBB + (((kk * 4 + g) ^ turn(r)) << 4));
+            return *reinterpret_cast<const i4v*>(img + r * 128 + (((kk * 4 + g) ^ turn(r)) << 4));
         } else if constexpr (ES == 2) {
             typedef short s4 __attribute__((ext_vector_type(4)));
             typedef int i2 __attribute__((ext_vector_type(2)));
@@ -317,31 +325,62 @@ template <typename T, int R, bool KC, int KBB> struct GaImg {
         }
     }
     // 16-byte slot q of the slab at X, off elements from X, at any alignment; zeros
-    // past the matrix in k, anything in rows that do not exist
+    // past the matrix in k, anything in rows that do not exist.  A slot that
+    // passes the end of its column (of len elements) reads the column's last 16
+    // bytes and shifts them down.
     __device__ static inline i64 element(int q, i64 ld, i64 rows) {
         int r, k;
         src_of(q, r, k);
         if constexpr (KC) return (r < rows ? r : rows - 1) * ld + k;
         else return k * ld + r;
     }
-    __device__ static inline i4v fetch(const T* X, i64 off, int q, i64 rows, i64 kleft, bool inside) {
+    __device__ static inline i4v fetch(const T* X, i64 off, int q, i64 ld, i64 len, i64 rows, i64 kleft, bool inside) {
         using vE = ga_vec<T, E>;
+        if (inside) return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(X + off));
         int r, k;
         src_of(q, r, k);
-        if (inside || (KC ? kleft - k >= E : k < kleft && rows - r >= E))
-            return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(X + off));
-        vE w;
-        #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            w[e] = (T)0;
-            if (KC ? k + e < kleft : k < kleft && r + e < rows) w[e] = X[off + e];
+        const i64 over = max((i64)0, KC ? k + E - kleft : r + E - rows), below = KC ? 0 : max((i64)0, k + 1 - kleft);
+        const T* x = X + off - below * ld;
+        if (len < E) {                                   // (the whole matrix has shorter columns)
+            vE w;
+            #pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = !below && e + over < E ? x[e] : (T)0;
+            return __builtin_bit_cast(i4v, w);
         }
-        return __builtin_bit_cast(i4v, w);
+        typedef unsigned __int128 u128;
+        const u128 w = __builtin_bit_cast(u128, *reinterpret_cast<const vE*>(x - over));
+        return __builtin_bit_cast(i4v, over < E && !below ? w >> (int)(over * ES * 8) : (u128)0);
     }
-    template <int NT>
-    __device__ static inline void stage(const T* X, i64 ld, i64 rows, i64 kleft, char* img, int tid) {
-        for (int q = tid; q < BYTES / 16; q += NT)
-            *reinterpret_cast<i4v*>(img + q * 16) = fetch(X, element(q, ld, rows), q, rows, kleft, false);
+    // A slab with an end of the matrix in it, wave wid of NW.  DMA of 16 bytes:
+    // accesses that lie inside go to LDS directly, the others from registers.
+    // DMA of 4: all from registers in 16-byte accesses (four times fewer; 452 x 17
+    // x 7897 f32, two products: 21 us against 24).
+    template <int W, int NW>
+    __device__ static inline void stage(const T* X, i64 ld, i64 len, i64 rows, i64 kleft, char* img, int wid, int lane) {
+        constexpr int N = BYTES / 1024;
+        if constexpr (W == 16) {
+            #pragma unroll 1
+            for (int c = wid; c < N; c += NW) {
+                const int q = c * 64 + lane;
+                const i64 off = element(q, ld, rows);
+                int r, k;
+                src_of(q, r, k);
+                if (KC ? k + E <= kleft : k < kleft && r + E <= rows) ga_to_lds<16>(X + off, img + c * 1024);
+                else if (k < kleft && (KC || r < rows))
+                    *reinterpret_cast<i4v*>(img + q * 16) = fetch(X, off, q, ld, len, rows, kleft, false);
+                else *reinterpret_cast<i4v*>(img + q * 16) = i4v{0, 0, 0, 0};
+            }
+        } else {
+            constexpr int C = (N + NW - 1) / NW;
+            i4v w[C];
+            #pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const int q = min(wid + i * NW, N - 1) * 64 + lane;
+                w[i] = fetch(X, element(q, ld, rows), q, ld, len, rows, kleft, false);
+            }
+            #pragma unroll
+            for (int i = 0; i < C; ++i) *reinterpret_cast<i4v*>(img + (min(wid + i * NW, N - 1) * 64 + lane) * 16) = w[i];
+        }
     }
 };
 
@@ -349,10 +388,10 @@ template <typename T, int R, bool KC, int KBB> struct GaImg {
 // fragments at a time, so that stores (and the loads of bias and residual) run
 // along the rows in 16-byte accesses and the activation appears in the code
 // once: unrolled over the 32 fragments of a wave it is 16 000 instructions.
-template <typename T, int BM, int BN, int WVM, int WVN, int KBB, int S> struct GaEpi {
+template <typename T, int BM, int BN, int WVM, int WVN, int S> struct GaEpi {
     static constexpr int AS = sizeof(typename ga_traits<T>::acc), NW = WVM * WVN, NI = BN / WVN / 16;
     static constexpr int LDR = BM / WVM + 16 / AS;                    // rows of a column, and 16 bytes against conflicts
-    static constexpr int RING = S * (BM + BN) * KBB, MOST = RING > 131071 ? 163840 : (RING > 65535 ? 81920 : RING);
+    static constexpr int RING = S * (BM + BN) * 128, MOST = RING > 131071 ? 163840 : (RING > 65535 ? 81920 : RING);
     static constexpr int bytes(int nj) { return NW * LDR * 16 * nj * AS; }
     static constexpr int pick() { int nj = NI; while (nj > 1 && bytes(nj) > MOST) nj /= 2; return nj; }
     static constexpr int NJ = pick();
@@ -367,16 +406,16 @@ template <typename T, int BM, int BN, int WVM, int WVN, int KBB, int S> struct G
 // f32: 38 us against 53 us through registers).  0: every slab goes through
 // registers, fetched before the products of the slab ahead of it and written to
 // LDS after them.
-template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int KBB, int S, bool GATED, int DMA>
+template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int S, bool GATED, int DMA>
 __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a) {
     using TR = ga_traits<T>;
     using acc4 = typename TR::acc4;
     using R = typename TR::acc;
     constexpr int NW = WVM * WVN, NT = 64 * NW, NA = GATED ? 2 : 1, BMI = BM / NA;
-    constexpr int WM = BM / WVM, WN = BN / WVN, MI = WM / 16, NI = WN / 16, KB = KBB / (int)sizeof(T);
-    using IA = GaImg<T, BMI, AKC, KBB>;
-    using IB = GaImg<T, BN, BKC, KBB>;
-    constexpr int SLOT = (BM + BN) * KBB;
+    constexpr int WM = BM / WVM, WN = BN / WVN, MI = WM / 16, NI = WN / 16, KB = 128 / (int)sizeof(T);
+    using IA = GaImg<T, BMI, AKC>;
+    using IB = GaImg<T, BN, BKC>;
+    constexpr int SLOT = (BM + BN) * 128;
     constexpr int W = DMA ? DMA : 16, PCA = IA::BYTES / (64 * W), PCB = IB::BYTES / (64 * W);    // pieces of a slab
     constexpr int PA = (PCA + NW - 1) / NW, PB = (PCB + NW - 1) / NW;
     static_assert(MI % NA == 0, "gated tiles pair their fragments");
@@ -430,12 +469,6 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
     int kt = sum && s0 >= nsteps ? s0 - nsteps : s0;      // step of its product being staged
     if constexpr (DMA) aim(curp, (i64)kt * KB);
 
-    using gptr = const __attribute__((address_space(1))) void*;
-    using lptr = __attribute__((address_space(3))) void*;
-    auto to_lds = [](const char* p, char* q) {
-        if constexpr (DMA == 4) __builtin_amdgcn_global_load_lds((gptr)p, (lptr)q, 4, 0, 0);
-        else __builtin_amdgcn_global_load_lds((gptr)p, (lptr)q, 16, 0, 0);
-    };
     // stages one step after the other
     auto issue = [&](char* slot) {
         if (sum && kt == nsteps) { kt = 0; curp = 1; aim(1, 0); }
@@ -445,19 +478,20 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             for (int h = 0; h < NA; ++h) {
                 #pragma unroll
                 for (int i = 0; i < PA; ++i)
-                    to_lds(xa[h] + offA[h][i], slot + h * IA::BYTES + min(wid + i * NW, PCA - 1) * (64 * W));
+                    ga_to_lds<W>(xa[h] + offA[h][i], slot + h * IA::BYTES + min(wid + i * NW, PCA - 1) * (64 * W));
                 xa[h] += da[h];
             }
             #pragma unroll
             for (int i = 0; i < PB; ++i)
-                to_lds(xb + offB[i], slot + BM * KBB + min(wid + i * NW, PCB - 1) * (64 * W));
+                ga_to_lds<W>(xb + offB[i], slot + BM * 128 + min(wid + i * NW, PCB - 1) * (64 * W));
             xb += db;
         } else {
             #pragma unroll
             for (int h = 0; h < NA; ++h)
-                IA::template stage<NT>(slabA(GATED ? h : curp, k0), a.lda[GATED ? h : curp], rowsA, a.k - k0,
-                                       slot + h * IA::BYTES, tid);
-            IB::template stage<NT>(slabB(curp, k0), a.ldb[curp], rowsB, a.k - k0, slot + BM * KBB, tid);
+                IA::template stage<W, NW>(slabA(GATED ? h : curp, k0), a.lda[GATED ? h : curp], AKC ? a.k : a.m, rowsA,
+                                          a.k - k0, slot + h * IA::BYTES, wid, lane);
+            IB::template stage<W, NW>(slabB(curp, k0), a.ldb[curp], BKC ? a.k : a.n, rowsB, a.k - k0, slot + BM * 128,
+                                      wid, lane);
         }
     };
 
@@ -474,19 +508,21 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
         for (int i = 0; i < CB; ++i) elB[i] = IB::element(min(tid + i * NT, QB - 1), a.ldb[p], rowsB);
     };
     const T *ya[NA], *yb;
-    i64 ea[NA], eb;
+    i64 ea[NA], eb, lea[NA], leb;
     auto point = [&](int p, i64 k0) {
         elements(p);
         #pragma unroll
         for (int h = 0; h < NA; ++h) {
             ya[h] = slabA(GATED ? h : p, k0);
-            ea[h] = AKC ? KB : KB * a.lda[GATED ? h : p];
+            lea[h] = a.lda[GATED ? h : p];
+            ea[h] = AKC ? KB : KB * lea[h];
         }
         yb = slabB(p, k0);
-        eb = BKC ? KB : KB * a.ldb[p];
+        leb = a.ldb[p];
+        eb = BKC ? KB : KB * leb;
     };
     if constexpr (!DMA) point(curp, (i64)kt * KB);
-    const i64 kall = a.k;
+    const i64 kall = a.k, am = a.m, an = a.n;
     auto fetch = [&]() {
         if (sum && kt == nsteps) { kt = 0; curp = 1; point(1, 0); }
         const i64 left = kall - (i64)kt++ * KB;
@@ -495,9 +531,9 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
         for (int h = 0; h < NA; ++h)
             #pragma unroll
             for (int i = 0; i < CA; ++i)
-                ra[h][i] = IA::fetch(ya[h], elA[h][i], min(tid + i * NT, QA - 1), rowsA, left, inA);
+                ra[h][i] = IA::fetch(ya[h], elA[h][i], min(tid + i * NT, QA - 1), lea[h], AKC ? kall : am, rowsA, left, inA);
         #pragma unroll
-        for (int i = 0; i < CB; ++i) rb[i] = IB::fetch(yb, elB[i], min(tid + i * NT, QB - 1), rowsB, left, inB);
+        for (int i = 0; i < CB; ++i) rb[i] = IB::fetch(yb, elB[i], min(tid + i * NT, QB - 1), leb, BKC ? kall : an, rowsB, left, inB);
         #pragma unroll
         for (int h = 0; h < NA; ++h) ya[h] += ea[h];
         yb += eb;
@@ -510,7 +546,7 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             for (int i = 0; i < CA; ++i)
                 *reinterpret_cast<i4v*>(slot + h * IA::BYTES + min(tid + i * NT, QA - 1) * 16) = ra[h][i];
         #pragma unroll
-        for (int i = 0; i < CB; ++i) *reinterpret_cast<i4v*>(slot + BM * KBB + min(tid + i * NT, QB - 1) * 16) = rb[i];
+        for (int i = 0; i < CB; ++i) *reinterpret_cast<i4v*>(slot + BM * 128 + min(tid + i * NT, QB - 1) * 16) = rb[i];
     };
 
     const int wm = wid / WVN, wn = wid % WVN;
@@ -532,7 +568,7 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
     auto reads = [&](const char* la, int kk, i4v (&fa)[MI], i4v (&fb)[NI]) {
         constexpr int H = MI / NA;
         #pragma unroll
-        for (int j = 0; j < NI; ++j) fb[j] = IB::frag(la + BM * KBB, wn * WN + j * 16, kk, lane);
+        for (int j = 0; j < NI; ++j) fb[j] = IB::frag(la + BM * 128, wn * WN + j * 16, kk, lane);
         #pragma unroll
         for (int i = 0; i < MI; ++i)
             fa[i] = IA::frag(la + (i / H) * IA::BYTES, wm * (WM / NA) + (i % H) * 16, kk, lane);
@@ -570,20 +606,20 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
         for (int s = s0; s < s1; ++s) {
             auto work = [&](const char* __restrict la, char* __restrict fill) __attribute__((always_inline)) {
                 #pragma unroll
-                for (int kk = 0; kk < KBB / 64; ++kk) {
+                for (int kk = 0; kk < 2; ++kk) {
                     i4v fa[MI], fb[NI];
                     // the slot behind was read to its end a turn ago by the later half
                     if (kk == 0 && s + 1 < s1) issue(fill);
                     reads(la, kk, fa, fb);
                     // the next slab is there when the first half comes to read it:
                     // one turn after this for the later half, two for the first
-                    if (kk == KBB / 64 - 1 && late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    if (kk == 1 && late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     turn();
                     __builtin_amdgcn_s_setprio(1);
                     products(fa, fb);
                     __builtin_amdgcn_s_setprio(0);
-                    if (kk == KBB / 64 - 1 && !late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    if (kk == 1 && !late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                     turn();
                 }
             };
@@ -606,7 +642,7 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
                     fetch();
                 }
                 #pragma unroll
-                for (int kk = 0; kk < KBB / 64; ++kk) {
+                for (int kk = 0; kk < 2; ++kk) {
                     i4v fa[MI], fb[NI];
                     reads(la, kk, fa, fb);
                     products(fa, fb);
@@ -644,7 +680,7 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             }
         return;
     }
-    using EP = GaEpi<T, BM, BN, WVM, WVN, KBB, S>;
+    using EP = GaEpi<T, BM, BN, WVM, WVN, S>;
     constexpr int NJ = EP::NJ, LDR = EP::LDR, V = 16 / (int)sizeof(T);
     R* img = reinterpret_cast<R*>(smem) + wid * (LDR * 16 * NJ);
     __syncthreads();                                 // every wave has read its last slab
@@ -679,55 +715,48 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
 }
 
 // ------------------------------------------------------------ few columns
-// C of up to 16 NF columns (tokens), both operands contiguous along k: bound by
+// C of up to 16 columns (tokens), both operands contiguous along k: bound by
 // reading op(A) once.  A workgroup takes 16 rows and all of K, its NW waves
 // interleaved slabs of 128 bytes per row, fragments straight from memory to
 // registers with 2 U of them in flight per wave and operand (no LDS, no
 // barrier in the loop); the waves' sums are added in LDS in their order.
-template <typename T, int NF, bool GATED, int NW>
+template <typename T, bool GATED, int NW>
 __global__ void __launch_bounds__(64 * NW) gemm_act_skinny_kernel(GemmActArgs a) {
     using TR = ga_traits<T>;
     using acc4 = typename TR::acc4;
     using R = typename TR::acc;
-    constexpr int NA = GATED ? 2 : 1, E = 16 / (int)sizeof(T), KB = 8 * E, U = NF * NA <= 1 ? 4 : 2, LD = 16 + 16 / (int)sizeof(R);
-    __shared__ __align__(16) R red[NW][NA][NF][16 * LD];
+    constexpr int NA = GATED ? 2 : 1, E = 16 / (int)sizeof(T), KB = 8 * E, U = GATED ? 2 : 4, LD = 16 + 16 / (int)sizeof(R);
+    __shared__ __align__(16) R red[NW][NA][16 * LD];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
     const i64 m0 = (i64)xcd_remap(blockIdx.x, gridDim.x) * 16;
     // rows and columns past the matrix read one that exists and are not stored
     const T* pa[NA];
-    const T* pb[NF];
     #pragma unroll
     for (int h = 0; h < NA; ++h) pa[h] = static_cast<const T*>(a.A[h]) + min(m0 + l, a.m - 1) * a.lda[h] + g * E;
-    #pragma unroll
-    for (int j = 0; j < NF; ++j) pb[j] = static_cast<const T*>(a.B[0]) + min((i64)(j * 16 + l), a.n - 1) * a.ldb[0] + g * E;
-    acc4 acc[NA][NF];
+    const T* pb = static_cast<const T*>(a.B[0]) + min((i64)l, a.n - 1) * a.ldb[0] + g * E;
+    acc4 acc[NA];
     #pragma unroll
     for (int h = 0; h < NA; ++h)
         #pragma unroll
-        for (int j = 0; j < NF; ++j)
-            #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[h][j][r] = R(0);
-    auto mul = [&](const i4v (&fa)[NA], const i4v (&fb)[NF]) {
+        for (int r = 0; r < 4; ++r) acc[h][r] = R(0);
+    auto mul = [&](const i4v (&fa)[NA], i4v fb) {
         #pragma unroll
-        for (int h = 0; h < NA; ++h)
-            #pragma unroll
-            for (int j = 0; j < NF; ++j) {
-                if constexpr (sizeof(R) == 4) acc[h][j] = TR::mma(fa[h], fb[j], acc[h][j]);
-                else acc[h][j] = TR::mma(fb[j], fa[h], acc[h][j]);
-            }
+        for (int h = 0; h < NA; ++h) {
+            if constexpr (sizeof(R) == 4) acc[h] = TR::mma(fa[h], fb, acc[h]);
+            else acc[h] = TR::mma(fb, fa[h], acc[h]);
+        }
     };
     const int slabs = (int)(a.k / KB);
     int s = w;
     for (; s + (U - 1) * NW < slabs; s += U * NW) {
-        i4v fa[2 * U][NA], fb[2 * U][NF];
+        i4v fa[2 * U][NA], fb[2 * U];
         #pragma unroll
         for (int u = 0; u < 2 * U; ++u) {
             const i64 k = (i64)(s + (u >> 1) * NW) * KB + (u & 1) * (4 * E);
             #pragma unroll
             for (int h = 0; h < NA; ++h)
                 fa[u][h] = __builtin_bit_cast(i4v, __builtin_nontemporal_load(reinterpret_cast<const ga_vec<T, E>*>(pa[h] + k)));
-            #pragma unroll
-            for (int j = 0; j < NF; ++j) fb[u][j] = __builtin_bit_cast(i4v, *reinterpret_cast<const ga_vec<T, E>*>(pb[j] + k));
+            fb[u] = __builtin_bit_cast(i4v, *reinterpret_cast<const ga_vec<T, E>*>(pb + k));
         }
         #pragma unroll
         for (int u = 0; u < 2 * U; ++u) mul(fa[u], fb[u]);
@@ -737,7 +766,7 @@ __global__ void __launch_bounds__(64 * NW) gemm_act_skinny_kernel(GemmActArgs a)
         for (int kk = 0; kk < 2; ++kk) {
             const i64 k = (i64)s * KB + kk * (4 * E);
             const int left = (int)min((i64)E, a.k - k - g * E);
-            i4v fa[NA], fb[NF];
+            i4v fa[NA];
             auto get = [&](const T* p) {
                 using vE = ga_vec<T, E>;
                 vE x;
@@ -748,32 +777,28 @@ __global__ void __launch_bounds__(64 * NW) gemm_act_skinny_kernel(GemmActArgs a)
             };
             #pragma unroll
             for (int h = 0; h < NA; ++h) fa[h] = get(pa[h]);
-            #pragma unroll
-            for (int j = 0; j < NF; ++j) fb[j] = get(pb[j]);
-            mul(fa, fb);
+            mul(fa, get(pb));
         }
     }
     #pragma unroll
     for (int h = 0; h < NA; ++h)
         #pragma unroll
-        for (int j = 0; j < NF; ++j)
-            #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = sizeof(R) == 4 ? g * 4 + r : l, col = sizeof(R) == 4 ? l : g + 4 * r;
-                red[w][h][j][col * LD + row] = acc[h][j][r];
-            }
+        for (int r = 0; r < 4; ++r) {
+            const int row = sizeof(R) == 4 ? g * 4 + r : l, col = sizeof(R) == 4 ? l : g + 4 * r;
+            red[w][h][col * LD + row] = acc[h][r];
+        }
     __syncthreads();
-    for (int t = threadIdx.x; t < NF * 256; t += 64 * NW) {
-        const int j = t >> 8, col = (t >> 4) & 15, row = t & 15;
-        if (j * 16 + col >= a.n) break;
+    for (int t = threadIdx.x; t < 256; t += 64 * NW) {
+        const int col = t >> 4, row = t & 15;
+        if (col >= a.n) break;
         R x[NA];
         #pragma unroll
         for (int h = 0; h < NA; ++h) {
-            x[h] = red[0][h][j][col * LD + row];
+            x[h] = red[0][h][col * LD + row];
             #pragma unroll
-            for (int q = 1; q < NW; ++q) x[h] += red[q][h][j][col * LD + row];
+            for (int q = 1; q < NW; ++q) x[h] += red[q][h][col * LD + row];
         }
-        ga_finish<T, 1, GATED>(a, 0, m0 + row, j * 16 + col, &x[0], &x[NA - 1]);
+        ga_finish<T, 1, GATED>(a, 0, m0 + row, col, &x[0], &x[NA - 1]);
     }
 }
 

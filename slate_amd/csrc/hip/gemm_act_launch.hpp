@@ -6,10 +6,10 @@ namespace slate_hip {
 
 namespace {
 
-template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int KBB, int S, bool GATED, int DMA>
+template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int S, bool GATED, int DMA>
 void ga_launch(const GemmActArgs& a, hipStream_t s) {
-    constexpr int BMI = GATED ? BM / 2 : BM, LDS = GaEpi<T, BM, BN, WVM, WVN, KBB, S>::LDS;
-    auto kern = gemm_act_kernel<T, AKC, BKC, BM, BN, WVM, WVN, KBB, S, GATED, DMA>;
+    constexpr int BMI = GATED ? BM / 2 : BM, LDS = GaEpi<T, BM, BN, WVM, WVN, S>::LDS;
+    auto kern = gemm_act_kernel<T, AKC, BKC, BM, BN, WVM, WVN, S, GATED, DMA>;
     if constexpr (LDS > 65536)
         HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                       LDS));
@@ -22,13 +22,13 @@ void ga_launch(const GemmActArgs& a, hipStream_t s) {
 template <typename T, bool AKC, bool BKC, bool GATED, int DMA>
 void ga_tile(const GemmActArgs& a, int tile, hipStream_t s) {
     if constexpr (sizeof(T) == 2 && DMA == 16)
-        if (tile == 0) return ga_launch<T, AKC, BKC, 256, 256, 2, 4, 128, 2, GATED, DMA>(a, s);
-    if constexpr (sizeof(T) == 2)
-        if (tile == 1) return ga_launch<T, AKC, BKC, 128, 128, 2, 2, 128, 2, GATED, DMA>(a, s);
+        if (tile == 0) return ga_launch<T, AKC, BKC, 256, 256, 2, 4, 2, GATED, DMA>(a, s);
     if constexpr (sizeof(T) == 2 && DMA == 16)
-        if (tile == 4) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 128, 3, GATED, DMA>(a, s);
-    if (tile == 2) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 128, 2, GATED, DMA>(a, s);
-    return ga_launch<T, AKC, BKC, 128, 16, 4, 1, 128, 2, GATED, DMA>(a, s);
+        if (tile == 1) return ga_launch<T, AKC, BKC, 128, 128, 2, 2, 2, GATED, DMA>(a, s);
+    if constexpr (sizeof(T) == 2 && DMA == 16)
+        if (tile == 4) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 3, GATED, DMA>(a, s);
+    if (tile == 2) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 2, GATED, DMA>(a, s);
+    return ga_launch<T, AKC, BKC, 128, 16, 4, 1, 2, GATED, DMA>(a, s);
 }
 
 template <typename T, bool GATED, int DMA>
@@ -88,11 +88,11 @@ template <typename T> void ga_pack(GaOperand* op, int n, char* ws, hipStream_t s
     }
 }
 
-template <typename T, int NF> void ga_skinny(const GemmActArgs& a, bool gated, hipStream_t s) {
+template <typename T> void ga_skinny(const GemmActArgs& a, bool gated, hipStream_t s) {
     constexpr int NW = 8;
     const dim3 grid((unsigned)((a.m + 15) / 16));
-    if (gated) hipLaunchKernelGGL((gemm_act_skinny_kernel<T, NF, true, NW>), grid, dim3(64 * NW), 0, s, a);
-    else hipLaunchKernelGGL((gemm_act_skinny_kernel<T, NF, false, NW>), grid, dim3(64 * NW), 0, s, a);
+    if (gated) hipLaunchKernelGGL((gemm_act_skinny_kernel<T, true, NW>), grid, dim3(64 * NW), 0, s, a);
+    else hipLaunchKernelGGL((gemm_act_skinny_kernel<T, false, NW>), grid, dim3(64 * NW), 0, s, a);
     HIP_LAUNCH_CHECK();
 }
 
@@ -123,7 +123,7 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
     const bool pack = ES == 2 && !dma && gemm_act_pack(a.mode, a.m, a.n, a.k) && ga_packed(op, nop, ES);
     const GemmActPlan p = gemm_act_plan(ES, a.mode, a.m, a.n, a.k, akc, bkc, dma || pack);
     if (p.tile < 0) {
-        ga_skinny<T, 1>(a, gated, s);
+        ga_skinny<T>(a, gated, s);
         return 0;
     }
     i64 bytes = (p.bytes + 255) / 256 * 256;

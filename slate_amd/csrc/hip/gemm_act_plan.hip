@@ -15,21 +15,29 @@ bool gemm_act_pack(int mode, i64 m, i64 n, i64 k) {
 
 namespace {
 
-// Microseconds that a square tile of 16-bit operands takes, by how many of its
-// workgroups a CU holds at once (256 CUs): per step of K, and for its start and
+// Microseconds that a square tile takes, by how many of its workgroups a CU
+// holds at once (256 CUs): per step of K (128 bytes), and for its start and
 // epilogue; measured on outputs of 256 to 8192 rows and columns, K of 256 to
 // 11456.  A larger tile reads less per flop, a smaller one fills the CUs and
-// overlaps one workgroup's epilogue with another's products: 4096^3 127 us with
-// 256 x 256 (128: 149, 64: 218), 4096 x 2048 x 4096 71 with 128 x 128 (101, 97),
-// 4096 x 512 x 4096 31 with 64 x 64 and three slots (256: 95, 128: 52, two slots
-// 39), 2048 x 2048 x 4096 51 with two slots (99, 53, three slots 60: a CU holds
-// four workgroups of the one, three of the other).
-struct GaCost { int tile, size, per_cu; double step[4], ends[4]; };
+// overlaps one workgroup's epilogue with another's products.  bf16: 4096^3 127
+// us with 256 x 256 (128: 149, 64: 218), 4096 x 2048 x 4096 71 with 128 x 128
+// (101, 97), 4096 x 512 x 4096 31 with 64 x 64 and three slots (256: 95, 128: 52,
+// two slots 39), 2048 x 2048 x 4096 51 with two slots (99, 53, three slots 60: a
+// CU holds four workgroups of the one, three of the other).  32- and 64-bit
+// products wait for the MFMAs, not for what a larger tile would save: 64 x 64
+// f32 133 us at 2000^3 (128 x 128: 143), 992 at 4096^3 (967 to 1010), f64 290
+// (350) and 2220 (2720).  (1024 x 4096 x 1024 of 16-bit operands that go through
+// registers: 30 us, 2048 x 4096 x 512 31; with 128 x 128 tiles 39.)
+enum { HALF_DMA, HALF_REGS, SINGLE, DOUBLE };
+struct GaCost { int kind, tile, size, per_cu; double step[4], ends[4]; };
 const GaCost ga_costs[] = {
-    {0, 256, 1, {1.72}, {11}},
-    {1, 128, 2, {0.70, 0.95}, {4, 7}},
-    {2, 64, 4, {0.515, 0.54, 0.60, 0.68}, {1, 2, 3, 3}},
-    {4, 64, 3, {0.36, 0.45, 0.60}, {1, 2, 3}},
+    {HALF_DMA, 0, 256, 1, {1.72}, {11}},
+    {HALF_DMA, 1, 128, 2, {0.70, 0.95}, {4, 7}},
+    {HALF_DMA, 2, 64, 4, {0.515, 0.54, 0.60, 0.68}, {1, 2, 3, 3}},
+    {HALF_DMA, 4, 64, 3, {0.36, 0.45, 0.60}, {1, 2, 3}},
+    {HALF_REGS, 2, 64, 4, {0.80, 0.82, 0.95, 1.40}, {1, 2, 3, 3}},
+    {SINGLE, 2, 64, 4, {0.72, 1.10, 1.65, 2.15}, {1, 2, 3, 3}},
+    {DOUBLE, 2, 64, 4, {0.80, 1.25, 1.85, 2.40}, {1, 2, 3, 3}},
 };
 double ga_time(const GaCost& c, i64 wgs, int steps) {
     const i64 full = wgs / (256 * c.per_cu), rest = wgs - full * 256 * c.per_cu;
@@ -58,15 +66,18 @@ GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool 
     const i64 rows = mode == GA_GATED ? 2 * m : m, pairs = mode == GA_PAIR ? 2 : 1;
     const int steps = std::max<int>(1, (int)((k * es + 127) / 128) * (mode == GA_SUM ? 2 : 1));
     auto tiles = [&](i64 bm, i64 bn) { return ((rows + bm - 1) / bm) * ((n + bn - 1) / bn) * pairs; };
-    if (n > 16 && es == 2 && dma) {
-        // 16-bit products: the tile and the pieces of K with the least time by
-        // the costs below.  What the operands take from memory bounds them all.
-        const double outs = 4e-6 * (mode == GA_GATED || mode == GA_PAIR ? 2 : 1) * m * n;       // MB of a partial sum
-        const double mem = 2.0 * k * ((double)rows * pairs + (double)n * pairs) / 4.4e6;
+    if (n > 16) {
+        // The tile and the pieces of K (4 steps or more) with the least time by
+        // the costs above.  What the operands take from memory bounds them all;
+        // partial sums go there and back.
+        const int kind = es == 2 ? (dma ? HALF_DMA : HALF_REGS) : es == 4 ? SINGLE : DOUBLE;
+        const double outs = 1e-6 * std::max(es, 4) * (mode == GA_GATED || mode == GA_PAIR ? 2 : 1) * m * n;     // MB
+        const double mem = es * (double)k * pairs * (rows + n) / 4.4e6;
         double best = 0;
         for (const GaCost& c : ga_costs) {
+            if (c.kind != kind) continue;
             const i64 t = tiles(c.size, c.size);
-            for (int want = 1; want <= 32 && (want == 1 || (want <= steps / 4 && t * want <= 1024)); ++want) {
+            for (int want = 1; want == 1 || (want <= steps / 4 && t * want <= 1024); ++want) {
                 const int per = (steps + want - 1) / want, sp = (steps + per - 1) / per;
                 if (sp != want) continue;
                 const double x = std::max(ga_time(c, t * sp, per), mem) + (sp > 1 ? 2 + 0.45 * outs * sp : 0);
@@ -74,18 +85,11 @@ GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool 
             }
         }
     } else {
-        // 32- and 64-bit products wait for the MFMAs, not for what a larger tile
-        // would save: f32 133 us at 2000^3 (128 x 128: 143 in two pieces), 992 at
-        // 4096^3 (967 to 1010), f64 290 (350) and 2220 (2720).  16-bit operands
-        // that go through registers: 4096^3 383 us with 128 x 128, 516 with 64 x 64.
-        i64 t;
-        if (n <= 16) { p.tile = 3; t = tiles(128, 16); }
-        else if (es == 2 && tiles(128, 128) >= 768) { p.tile = 1; t = tiles(128, 128); }
-        else { p.tile = 2; t = tiles(64, 64); }
-        // Few tiles: K in pieces of at least 4 steps, up to two workgroups per CU
-        // (64 columns, 1024 x 4096 bf16: 13 us in 16 pieces, 20 us in 4).
-        const i64 want = p.tile == 3 ? 1024 : 512;
-        if (t < want / 2 && steps >= 8) p.splits = (int)std::min<i64>(steps / 4, want / t);
+        // K in pieces of at least 4 steps, up to four workgroups per CU (16
+        // columns, 4096 x 4096 bf16: 15 us in 16 pieces, 21 us in 4)
+        p.tile = 3;
+        const i64 t = tiles(128, 16);
+        if (t < 512 && steps >= 8) p.splits = (int)std::min<i64>(steps / 4, 1024 / t);
     }
     if (p.splits > 1) {
         p.per_split = (steps + p.splits - 1) / p.splits;
