@@ -12,17 +12,18 @@ namespace slate_hip {
 
 namespace {
 
-constexpr int AG_WAVES = 4;
-
-// grid.x: blocks of 64 E rows (bias_mode 0, 1); grid.y: chunks of columns
+// grid.x: blocks of E 2^tx rows (bias_mode 0, 1), grid.y: chunks of columns; the
+// 256 threads lie 2^tx along the rows and 256 / 2^tx along the columns, so that
+// short columns keep every lane busy (16 x 393 bf16, gelu: 17 us with the lanes
+// of a wave along the rows alone).
 template <typename T, bool GATED>
-__global__ void __launch_bounds__(64 * AG_WAVES) act_grad_rows_kernel(ActGradArgs a, i64 cols) {
+__global__ void __launch_bounds__(256) act_grad_rows_kernel(ActGradArgs a, i64 cols, int tx) {
     using R = typename ga_traits<T>::acc;
     constexpr int E = 16 / sizeof(T);
     constexpr bool FAST = sizeof(T) == 2;
     using vE = ga_vec<T, E>;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const i64 m = ((i64)blockIdx.x * 64 + lane) * E;
+    const int lane = threadIdx.x & ((1 << tx) - 1), w = threadIdx.x >> tx, ny = 256 >> tx;
+    const i64 m = (((i64)blockIdx.x << tx) + lane) * E;
     const int left = (int)max((i64)0, min((i64)E, a.m - m));
     const i64 n0 = (i64)blockIdx.y * cols, n1 = min(a.n, n0 + cols);
     const bool wide = left == E;
@@ -31,8 +32,10 @@ __global__ void __launch_bounds__(64 * AG_WAVES) act_grad_rows_kernel(ActGradArg
     for (int e = 0; e < E; ++e) sum[e] = R(0);
     auto get = [&](const void* p, i64 ld, i64 n, T* v) {
         const T* x = static_cast<const T*>(p) + m + n * ld;
-        if (wide) {
-            const vE y = *reinterpret_cast<const vE*>(x);
+        if (a.m >= E) {          // a column's end: its last 16 bytes, shifted down
+            typedef unsigned __int128 u128;
+            const u128 w = __builtin_bit_cast(u128, *reinterpret_cast<const vE*>(x - (E - left)));
+            const vE y = __builtin_bit_cast(vE, w >> ((E - left) * (int)sizeof(T) * 8));
             #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = y[e];
         } else {
@@ -52,7 +55,7 @@ __global__ void __launch_bounds__(64 * AG_WAVES) act_grad_rows_kernel(ActGradArg
             for (int e = 0; e < E; ++e) if (e < left) x[e] = (T)v[e];
         }
     };
-    // UN columns' loads are in flight per wave
+    // UN columns' loads are in flight per thread
     constexpr int UN = GATED ? 2 : 4;
     auto column = [&](i64 n, const T* c, const T* z1, const T* z2) {
         R d1[E], d2[E], z[E], v[E], d[E];
@@ -70,11 +73,11 @@ __global__ void __launch_bounds__(64 * AG_WAVES) act_grad_rows_kernel(ActGradArg
         if constexpr (GATED) put(a.dZ2, n, d2);
     };
     if (left > 0)
-        for (i64 n = n0 + w; n < n1; n += AG_WAVES * UN) {
+        for (i64 n = n0 + w; n < n1; n += ny * UN) {
             T c[UN][E], z1[UN][E], z2[UN][E];
             #pragma unroll
             for (int u = 0; u < UN; ++u) {
-                const i64 nu = min(n + u * AG_WAVES, n1 - 1);
+                const i64 nu = min(n + u * ny, n1 - 1);
                 get(a.dC, a.lddc, nu, c[u]);
                 if (a.Z1) get(a.Z1, a.ldz1, nu, z1[u]);
                 if constexpr (GATED) get(a.Z2, a.ldz2, nu, z2[u]);
@@ -88,19 +91,18 @@ __global__ void __launch_bounds__(64 * AG_WAVES) act_grad_rows_kernel(ActGradArg
                     if (q == u)
                         #pragma unroll
                         for (int e = 0; e < E; ++e) { cu[e] = c[q][e]; zu[e] = z1[q][e]; wu[e] = z2[q][e]; }
-                if (n + u * AG_WAVES < n1) column(n + u * AG_WAVES, cu, zu, wu);
+                if (n + u * ny < n1) column(n + u * ny, cu, zu, wu);
             }
         }
     if (a.bias_mode == 1) {
-        __shared__ R red[AG_WAVES][64 * E];
+        __shared__ R red[256 * E];
         #pragma unroll
-        for (int e = 0; e < E; ++e) red[w][lane * E + e] = sum[e];
+        for (int e = 0; e < E; ++e) red[threadIdx.x * E + e] = sum[e];
         __syncthreads();
-        for (int i = threadIdx.x; i < 64 * E; i += 64 * AG_WAVES) {
-            R s = red[0][i];
-            #pragma unroll
-            for (int q = 1; q < AG_WAVES; ++q) s += red[q][i];
-            const i64 mm = (i64)blockIdx.x * 64 * E + i;
+        for (int i = threadIdx.x; i < E << tx; i += 256) {
+            R s = red[i];
+            for (int q = 1; q < ny; ++q) s += red[(q * E << tx) + i];
+            const i64 mm = ((i64)blockIdx.x * E << tx) + i;
             if (mm < a.m) static_cast<R*>(a.part)[blockIdx.y * a.m + mm] = s;
         }
     }
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(256) act_grad_join_kernel(const typename ga_tr
     const i64 i = (i64)blockIdx.x * 32 + x;
     R s = R(0);
     if (i < len) {
-        #pragma unroll 4
+        #pragma unroll 8
         for (int c = y; c < chunks; c += 8) s += part[c * len + i];
     }
     red[y][x] = s;
@@ -154,11 +156,20 @@ __global__ void __launch_bounds__(256) act_grad_join_kernel(const typename ga_tr
 
 }  // namespace
 
-// Enough blocks for the 256 CUs several times over, none with less than 16
-// columns (or 512 rows) of its own.
+// log2 of the threads along the rows
+int act_grad_tx(int es, i64 m) {
+    int tx = 0;
+    while (tx < 6 && (16 / es << tx) < m) ++tx;
+    return tx;
+}
+
+// Enough blocks for the 256 CUs several times over; none with less than a column
+// for each of its threads, or 512 rows of its own.
 int act_grad_chunks(int bias_mode, int es, i64 m, i64 n) {
-    const i64 other = bias_mode == 2 ? (n + 3) / 4 : (m + 64 * (16 / es) - 1) / (64 * (16 / es));
-    const i64 most = bias_mode == 2 ? (m + 511) / 512 : (n + 15) / 16;
+    const int tx = act_grad_tx(es, m);
+    const i64 rb = 16 / es << tx, cb = 256 >> tx;
+    const i64 other = bias_mode == 2 ? (n + 3) / 4 : (m + rb - 1) / rb;
+    const i64 most = bias_mode == 2 ? (m + 511) / 512 : (n + cb - 1) / cb;
     return (int)std::max<i64>(1, std::min<i64>(most, (1024 + other - 1) / std::max<i64>(1, other)));
 }
 
@@ -169,10 +180,11 @@ template <typename T> void act_grad(ActGradArgs a, hipStream_t s) {
         const i64 rows = (a.m + chunks - 1) / chunks;
         hipLaunchKernelGGL((act_grad_cols_kernel<T>), dim3((unsigned)((a.n + 3) / 4), chunks), dim3(256), 0, s, a, rows);
     } else {
-        const i64 cols = (a.n + chunks - 1) / chunks, rb = 64 * (16 / ES);
+        const int tx = act_grad_tx(ES, a.m);
+        const i64 cols = (a.n + chunks - 1) / chunks, rb = 16 / ES << tx;
         const dim3 grid((unsigned)((a.m + rb - 1) / rb), chunks);
-        if (a.Z2) hipLaunchKernelGGL((act_grad_rows_kernel<T, true>), grid, dim3(64 * AG_WAVES), 0, s, a, cols);
-        else hipLaunchKernelGGL((act_grad_rows_kernel<T, false>), grid, dim3(64 * AG_WAVES), 0, s, a, cols);
+        if (a.Z2) hipLaunchKernelGGL((act_grad_rows_kernel<T, true>), grid, dim3(256), 0, s, a, cols, tx);
+        else hipLaunchKernelGGL((act_grad_rows_kernel<T, false>), grid, dim3(256), 0, s, a, cols, tx);
     }
     HIP_LAUNCH_CHECK();
     if (a.bias_mode) {
