@@ -334,8 +334,11 @@ template <typename T, int R, bool KC> struct GaImg {
         if constexpr (KC) return (r < rows ? r : rows - 1) * ld + k;
         else return k * ld + r;
     }
-    __device__ static inline i4v fetch(const T* X, i64 off, int q, i64 ld, i64 len, i64 rows, i64 kleft, bool inside) {
+    // (the shift, by `down` bits, is left to the caller: it waits for the load)
+    __device__ static inline i4v fetch(const T* X, i64 off, int q, i64 ld, i64 len, i64 rows, i64 kleft, bool inside,
+                                       int& down) {
         using vE = ga_vec<T, E>;
+        down = 0;
         if (inside) return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(X + off));
         int r, k;
         src_of(q, r, k);
@@ -347,9 +350,13 @@ template <typename T, int R, bool KC> struct GaImg {
             for (int e = 0; e < E; ++e) w[e] = !below && e + over < E ? x[e] : (T)0;
             return __builtin_bit_cast(i4v, w);
         }
+        down = over < E && !below ? (int)over * ES * 8 : 128;
+        return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(x - over));
+    }
+    __device__ static inline i4v shift(i4v w, int down) {
         typedef unsigned __int128 u128;
-        const u128 w = __builtin_bit_cast(u128, *reinterpret_cast<const vE*>(x - over));
-        return __builtin_bit_cast(i4v, over < E && !below ? w >> (int)(over * ES * 8) : (u128)0);
+        const u128 x = __builtin_bit_cast(u128, w) >> (down & 127);
+        return __builtin_bit_cast(i4v, down < 128 ? x : (u128)0);
     }
     // A slab with an end of the matrix in it, wave wid of NW.  DMA of 16 bytes:
     // accesses that lie inside go to LDS directly, the others from registers.
@@ -366,20 +373,24 @@ template <typename T, int R, bool KC> struct GaImg {
                 int r, k;
                 src_of(q, r, k);
                 if (KC ? k + E <= kleft : k < kleft && r + E <= rows) ga_to_lds<16>(X + off, img + c * 1024);
-                else if (k < kleft && (KC || r < rows))
-                    *reinterpret_cast<i4v*>(img + q * 16) = fetch(X, off, q, ld, len, rows, kleft, false);
-                else *reinterpret_cast<i4v*>(img + q * 16) = i4v{0, 0, 0, 0};
+                else if (k < kleft && (KC || r < rows)) {
+                    int down;
+                    const i4v w = fetch(X, off, q, ld, len, rows, kleft, false, down);
+                    *reinterpret_cast<i4v*>(img + q * 16) = shift(w, down);
+                } else *reinterpret_cast<i4v*>(img + q * 16) = i4v{0, 0, 0, 0};
             }
         } else {
             constexpr int C = (N + NW - 1) / NW;
             i4v w[C];
+            int down[C];
             #pragma unroll
             for (int i = 0; i < C; ++i) {
                 const int q = min(wid + i * NW, N - 1) * 64 + lane;
-                w[i] = fetch(X, element(q, ld, rows), q, ld, len, rows, kleft, false);
+                w[i] = fetch(X, element(q, ld, rows), q, ld, len, rows, kleft, false, down[i]);
             }
             #pragma unroll
-            for (int i = 0; i < C; ++i) *reinterpret_cast<i4v*>(img + (min(wid + i * NW, N - 1) * 64 + lane) * 16) = w[i];
+            for (int i = 0; i < C; ++i)
+                *reinterpret_cast<i4v*>(img + (min(wid + i * NW, N - 1) * 64 + lane) * 16) = shift(w[i], down[i]);
         }
     }
 };
@@ -498,6 +509,8 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
     // through registers
     constexpr int QA = IA::BYTES / 16, QB = IB::BYTES / 16, CA = DMA ? 1 : (QA + NT - 1) / NT, CB = DMA ? 1 : (QB + NT - 1) / NT;
     i4v ra[NA][CA], rb[CB];
+    int sa[NA][CA], sb[CB];
+    bool inside = true;
     i64 elA[NA][CA], elB[CB];
     auto elements = [&](int p) {
         #pragma unroll
@@ -526,27 +539,37 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
     auto fetch = [&]() {
         if (sum && kt == nsteps) { kt = 0; curp = 1; point(1, 0); }
         const i64 left = kall - (i64)kt++ * KB;
-        const bool inA = left >= KB && (AKC || rowsA >= BMI), inB = left >= KB && (BKC || rowsB >= BN);
+        inside = left >= KB && (AKC || rowsA >= BMI) && (BKC || rowsB >= BN);
         #pragma unroll
         for (int h = 0; h < NA; ++h)
             #pragma unroll
             for (int i = 0; i < CA; ++i)
-                ra[h][i] = IA::fetch(ya[h], elA[h][i], min(tid + i * NT, QA - 1), lea[h], AKC ? kall : am, rowsA, left, inA);
+                ra[h][i] = IA::fetch(ya[h], elA[h][i], min(tid + i * NT, QA - 1), lea[h], AKC ? kall : am, rowsA, left, inside,
+                                     sa[h][i]);
         #pragma unroll
-        for (int i = 0; i < CB; ++i) rb[i] = IB::fetch(yb, elB[i], min(tid + i * NT, QB - 1), leb, BKC ? kall : an, rowsB, left, inB);
+        for (int i = 0; i < CB; ++i) rb[i] = IB::fetch(yb, elB[i], min(tid + i * NT, QB - 1), leb, BKC ? kall : an, rowsB, left, inside, sb[i]);
         #pragma unroll
         for (int h = 0; h < NA; ++h) ya[h] += ea[h];
         yb += eb;
     };
     auto write = [&](int s) {
         char* slot = smem + (s % S) * SLOT;
-        #pragma unroll
-        for (int h = 0; h < NA; ++h)
+        auto put = [&](auto whole) {
             #pragma unroll
-            for (int i = 0; i < CA; ++i)
-                *reinterpret_cast<i4v*>(slot + h * IA::BYTES + min(tid + i * NT, QA - 1) * 16) = ra[h][i];
-        #pragma unroll
-        for (int i = 0; i < CB; ++i) *reinterpret_cast<i4v*>(slot + BM * 128 + min(tid + i * NT, QB - 1) * 16) = rb[i];
+            for (int h = 0; h < NA; ++h)
+                #pragma unroll
+                for (int i = 0; i < CA; ++i) {
+                    if constexpr (!whole) ra[h][i] = IA::shift(ra[h][i], sa[h][i]);
+                    *reinterpret_cast<i4v*>(slot + h * IA::BYTES + min(tid + i * NT, QA - 1) * 16) = ra[h][i];
+                }
+            #pragma unroll
+            for (int i = 0; i < CB; ++i) {
+                if constexpr (!whole) rb[i] = IB::shift(rb[i], sb[i]);
+                *reinterpret_cast<i4v*>(slot + BM * 128 + min(tid + i * NT, QB - 1) * 16) = rb[i];
+            }
+        };
+        if (inside) put(std::true_type());
+        else put(std::false_type());
     };
 
     const int wm = wid / WVN, wn = wid % WVN;
