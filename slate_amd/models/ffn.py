@@ -401,8 +401,9 @@ def _run_dist(mode, alpha, A, B, C, bias=None, bias_mode=0, act=0, beta=0.0, R=N
     b = _NONE if bias is None else _vector(bias, bias_mode, W[0])
     if grid_rank:
         As, Bs, Ws = ((x + [_NONE])[:2] for x in (As, Bs, [_opd(w) for w in W]))
-        _launch(mode, alpha, *As, *Bs, *Ws, b, bias_mode, act, beta, _NONE if Rw is None else _opd(Rw),
-                *[_NONE if z is None else _opd(z) for z in Zw])
+        with _on(Ws[0].t):
+            _launch(mode, alpha, *As, *Bs, *Ws, b, bias_mode, act, beta, _NONE if Rw is None else _opd(Rw),
+                    *[_NONE if z is None else _opd(z) for z in Zw])
     _modified(*W, *Zw)
     for w, c in zip(list(W) + Zw, list(C) + list(Z)):
         if w is not None and w is not c:
@@ -644,7 +645,8 @@ def _dz_dist(act, dC, Z, dbias, bmode):
     if s.bc.pr >= 0 and (act or two or dbias is not None):
         oz = [_NONE if z is None else _opd(z) for z in Zw]
         od = [_opd(d) for d in dZ] if act or two else [_NONE]
-        _act_grad(lb.mloc, lb.nloc, act, _opd(W), oz[0], oz[1], od[0], od[1] if two else _NONE, db, bmode, True)
+        with _on(lb.data):
+            _act_grad(lb.mloc, lb.nloc, act, _opd(W), oz[0], oz[1], od[0], od[1] if two else _NONE, db, bmode, True)
     if act or two:
         _modified(*dZ)
     if dbias is not None:
@@ -682,6 +684,32 @@ def _clip_views(mats, what):
             raise SlateError(f"{what}: the matrices differ in communicator")
         out.append(x)
     return out
+
+
+def _clip_apart(what, va, vb):
+    """What is written shares no element with another matrix of the call."""
+    todo = [(y.ptr, y.end, i) for i, y in enumerate(vb)]
+    if vb is not va:
+        todo += [(x.ptr, x.end, ~i) for i, x in enumerate(va)]
+    todo.sort()
+    last = 0
+    for lo, hi, _ in todo:
+        if lo < last and hi > lo:
+            break
+        last = max(last, hi)
+    else:
+        return
+    # address ranges overlap: element by element, each against those that begin inside it
+    for i, (_, hi, p) in enumerate(todo):
+        x = vb[p] if p >= 0 else va[~p]
+        for lo, _, q in todo[i + 1:]:
+            if lo >= hi:
+                break
+            y = vb[q] if q >= 0 else va[~q]
+            if y.end == y.ptr or p < 0 and q < 0 or p == ~q and (x.ptr, x.ld, x.dt) == (y.ptr, y.ld, y.dt):
+                continue
+            if _overlap(x, y):
+                raise SlateError(f"{what}: matrices {p if p >= 0 else ~p} and {q if q >= 0 else ~q} of the call overlap")
 
 
 def clip_norm(max_norm, A, B=None, opts=None):
@@ -731,9 +759,7 @@ def _clip(what, limit, A, B):
                         (comm.size > 1 and (X.m() != Y.m() or X.n() != Y.n() or not _same_place(X, Y))):
                     raise SlateError(f"{what}: B's matrices want the shapes, ops and distribution of A's")
         if limit is not None:
-            full = [y.ptr for y in vb if y.end > y.ptr]
-            if len(set(full)) < len(full):
-                raise SlateError(f"{what}: a matrix is in the list twice")
+            _clip_apart(what, va, vb)
         mod, st = kmod(t), raw_stream(t)
         # (A, lda, B, ldb, rows, columns) of every matrix; complex ones as pairs
         mats = []

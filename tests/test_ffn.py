@@ -823,3 +823,57 @@ def test_half_unaligned(dt, ta, tb, pad, off):
 def test_half_unaligned_grad(dt, ta, tb):
     grad_call(Product(dt, "cuda", 2051, 2049, 2053, ta, tb, pad=3), "gelu")
     Gated(dt, "cuda", 1103, 2049, 2051, ta, tb, pad=1, off=3).check_grad()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_clip_overlaps(dev):
+    """Matrices that are written share no element with others; blocks of one buffer may lie in each other's range."""
+    x = cm(40, 30, torch.float32, 1, dev)
+    y = cm(40, 30, torch.float32, 2, dev)
+    norm, f = clip_want([x[:20], x[20:]], 1.0)
+    was = x.double()
+    halves = [mat(x[:20]), mat(x[20:])]
+    for A, B in (([mat(x), mat(x)], None), ([mat(x), mat(x[5:9])], None), ([mat(x[:21]), mat(x[20:])], None),
+                 (halves, [mat(y[:20]), mat(x[:20])]), ([mat(x[:20])], [mat(x[1:21])]), (halves[:1] * 2, [mat(y[:20])] * 2)):
+        with pytest.raises(SlateError, match="overlap"):
+            sl.clip_norm(1.0, A, B)
+    # read twice, written once each
+    s = sl.clip_norm(1e9, halves[:1] * 2, [mat(y[:20]), mat(y[20:])])
+    assert torch.equal(y[:20], x[:20]) and torch.equal(y[20:], x[:20])
+    assert abs(float(s) - math.sqrt(2) * float(x[:20].double().norm())) < 1e-6
+    s = sl.clip_norm(1.0, halves)
+    assert abs(float(s) - norm) <= 1e-12 * norm
+    within(x, f * was, 4 * 2.0 ** -24 * f * was.abs())
+
+
+@pytest.mark.gpu
+def test_far_offsets():
+    """Elements more than 2^31 beyond the first: many columns, and long sums in both layouts."""
+    n = 2 ** 25 + 3
+    A = cm(72, 40, torch.bfloat16, 1, "cuda", 0.1)
+    B = torch.zeros(n, 72, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, n // 2, n - 65, n - 1], device="cuda")
+    B[at] = torch.randn(4, 72, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    C = torch.full((n, 40), 7.0, dtype=torch.bfloat16, device="cuda")
+    sl.gemm_bias_act(1.0, mat(A, True, 2 ** 20), mat(B.t(), nb=2 ** 20), None, "silu", 0.0, None, mat(C.t(), nb=2 ** 20))
+    a, b = A.double(), B[at].double()
+    z, S = b @ a, b.abs() @ a.abs()
+    y = act64("silu", z)[0]
+    e = 1.13 * 76 * 2.0 ** -24 * S + act_bound(z, 2.0 ** -24)
+    within(C[at], y, e + 2.0 ** -8 * (y.abs() + e))
+    C[at] = 0
+    assert int(torch.count_nonzero(C)) == 0
+    del B, C
+    # sums of few terms, exact in 16 bits: 8 rows of 2^28 + 64 elements, and 2^25 + 5 columns of 72
+    for rows, k, trans in ((8, 2 ** 28 + 64, True), (72, 2 ** 25 + 5, False)):
+        X = torch.zeros((rows, k) if trans else (k, rows), dtype=torch.bfloat16, device="cuda")
+        Y = torch.zeros(2, k, dtype=torch.bfloat16, device="cuda")
+        for i, p in enumerate((0, k // 2, k - 1)):
+            (X[:, p] if trans else X[p]).copy_(torch.arange(1, rows + 1, device="cuda") * 2.0 ** i / 8)
+            Y[:, p] = torch.tensor([1.0, 2.0], device="cuda")
+        C = torch.empty(2, rows, dtype=torch.float32, device="cuda").to(torch.bfloat16)
+        sl.gemm_bias_act(1.0, mat(X.t(), trans, 2 ** 28), mat(Y.t(), nb=2 ** 28), None, "identity", 0.0, None, mat(C.t()))
+        want = torch.arange(1, rows + 1).double() * 7 / 8
+        want = torch.stack([want, 2 * want])
+        within(C.cpu(), want, 2.0 ** -8 * want.abs())
+        del X, Y
