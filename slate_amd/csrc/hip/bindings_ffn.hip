@@ -3,6 +3,7 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include "ffn.hpp"
+#include "clip_apart.hpp"
 
 namespace py = pybind11;
 using namespace slate_hip;
@@ -24,19 +25,24 @@ template <typename F> void real_dispatch(char dt, F&& f) {
 }
 
 // six integers per matrix: A, lda, B, ldb, rows, columns
-std::vector<ClipMat> mats(const py::list& v) {
-    std::vector<ClipMat> c;
+std::vector<i64> ints(const py::list& v) {
     const Py_ssize_t n = PyList_GET_SIZE(v.ptr());
     if (n % 6) throw std::invalid_argument("clip: six integers per matrix are wanted");
-    c.reserve(n / 6);
-    for (Py_ssize_t i = 0; i < n; i += 6) {
-        i64 x[6];
-        for (int j = 0; j < 6; ++j) x[j] = PyLong_AsLongLong(PyList_GET_ITEM(v.ptr(), i + j));
-        if (PyErr_Occurred()) throw py::error_already_set();
+    std::vector<i64> x(n);
+    for (Py_ssize_t i = 0; i < n; ++i) x[i] = PyLong_AsLongLong(PyList_GET_ITEM(v.ptr(), i));
+    if (PyErr_Occurred()) throw py::error_already_set();
+    return x;
+}
+std::vector<ClipMat> mats(const std::vector<i64>& v) {
+    std::vector<ClipMat> c;
+    c.reserve(v.size() / 6);
+    for (size_t i = 0; i < v.size(); i += 6) {
+        const i64* x = &v[i];
         if (x[4] > 0 && x[5] > 0) c.push_back({P((uintptr_t)x[0]), W((uintptr_t)x[2]), x[4], x[5], x[1], x[3]});
     }
     return c;
 }
+int bytes_of(char t) { return t == 'd' ? 8 : t == 's' ? 4 : 2; }
 
 }  // namespace
 
@@ -86,14 +92,18 @@ void register_ffn(py::module& m) {
         real_dispatch(dt, [&](auto z) { act_grad<decltype(z)>(a, S(st)); });
     });
     m.def("clip_parts", [](i64 count) { return clip_parts(count); });
+    // false, and nothing launched, where `look` is set and address ranges of the call overlap
     m.def("clip_norm", [](char ta, char tb, const py::list& v, double limit, uintptr_t part, uintptr_t norm, bool scale,
-                          uintptr_t st) {
-        const auto c = mats(v);
+                          bool look, uintptr_t st) {
+        const auto x = ints(v);
+        if (scale && look && !clip_apart(x.data(), x.size() / 6, bytes_of(ta), bytes_of(tb))) return false;
+        const auto c = mats(x);
         const int n = clip_sum(ta, c.data(), (int)c.size(), (double*)W(part), S(st));
         clip_scale(ta, tb, c.data(), (int)c.size(), limit, (const double*)P(part), n, (double*)W(norm), scale, S(st));
+        return true;
     });
     m.def("clip_sum", [](char ta, const py::list& v, uintptr_t part, uintptr_t st) {
-        const auto c = mats(v);
+        const auto c = mats(ints(v));
         return (i64)clip_sum(ta, c.data(), (int)c.size(), (double*)W(part), S(st));
     });
     m.def("clip_join", [](uintptr_t part, i64 parts, uintptr_t out, uintptr_t st) {
@@ -101,7 +111,7 @@ void register_ffn(py::module& m) {
     });
     m.def("clip_scale", [](char ta, char tb, const py::list& v, double limit, uintptr_t part, i64 parts, uintptr_t norm,
                            bool scale, uintptr_t st) {
-        const auto c = mats(v);
+        const auto c = mats(ints(v));
         clip_scale(ta, tb, c.data(), (int)c.size(), limit, (const double*)P(part), (int)parts, (double*)W(norm), scale,
                    S(st));
     });

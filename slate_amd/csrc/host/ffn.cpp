@@ -12,6 +12,8 @@
 #include <stdexcept>
 #include <vector>
 
+#include "clip_apart.hpp"
+
 namespace py = pybind11;
 
 namespace slate_host {
@@ -256,9 +258,13 @@ void register_ffn(py::module& m) {
         clip_scale(ta, tb, v, limit, ptr<const double>(part), ptr<double>(norm), scale);
     });
     m.def("clip_norm", [](char ta, char tb, const std::vector<i64>& v, double limit, uintptr_t part, uintptr_t norm,
-                          bool scale, uintptr_t) {
+                          bool scale, bool look, uintptr_t) {
+        auto es = [](char t) { return t == 'd' ? 8 : t == 's' ? 4 : 2; };
+        if (v.size() % 6) throw std::invalid_argument("clip: six integers per matrix are wanted");
+        if (scale && look && !clip_apart(v.data(), v.size() / 6, es(ta), es(tb))) return false;
         clip_sum(ta, v, ptr<double>(part));
         clip_scale(ta, tb, v, limit, ptr<const double>(part), ptr<double>(norm), scale);
+        return true;
     });
     m.def("gecopy16", [](char ds, char dd, char uplo, char trans, i64 mm, i64 n, uintptr_t A, i64 lda, uintptr_t B,
                          i64 ldb, uintptr_t) {

@@ -45,6 +45,9 @@ _ACT.update({a.name.lower(): i for a, i in list(_ACT.items())})
 _BYTES = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4, torch.float64: 8, torch.complex64: 8, torch.complex128: 16}
 
 
+_DEVICES = {}          # one object per device, so that operands compare them by identity
+
+
 # ------------------------------------------------------------------ operands
 class _Opd:
     """One rank's strided column-major operand: first and one past the last
@@ -54,7 +57,7 @@ class _Opd:
     __slots__ = ("ptr", "end", "ld", "rows", "cols", "m", "n", "trans", "t", "dt", "dev", "buf")
 
     def __init__(self, ptr, ld, rows, cols, trans, t):
-        self.dt, self.dev = (None, None) if t is None else (t.dtype, t.device)
+        self.dt, self.dev = (None, None) if t is None else (t.dtype, _DEVICES.setdefault(t.device, t.device))
         self.ptr, self.ld, self.rows, self.cols, self.trans, self.t = ptr, ld, rows, cols, trans, t
         self.m, self.n = (cols, rows) if trans else (rows, cols)
         self.end = ptr + ((cols - 1) * ld + rows) * _BYTES[t.dtype] if rows and cols else ptr
@@ -122,7 +125,7 @@ def _operands(what, names, mats):
                 raise SlateError(f"{what}: element type {dt} (bfloat16, float16, float32 or float64 are wanted)")
         elif x.dt is not dt:
             raise SlateError(f"{what}: {name} has type {x.dt}, the others {dt}")
-        elif x.dev != dev:
+        elif x.dev is not dev:
             raise SlateError(f"{what}: {name} is on {x.dev}, the others on {dev}")
         out.append(x)
     return out
@@ -665,25 +668,36 @@ def _dz_dist(act, dC, Z, dbias, bmode):
 
 # ------------------------------------------------------------------ clipping
 def _clip_views(mats, what):
-    """Operands of a list of matrices of one type, device and communicator."""
+    """Operands of a list of matrices of one type, device and communicator, and
+    the storages among theirs whose state a write changes."""
     if not isinstance(mats, (list, tuple)):
         raise SlateError(f"{what}: a list of matrices is wanted")
-    out, dt, dev, comm = [], None, None, None
+    out, todo, dt, dev, comm = [], [], None, None, None
+    add = out.append
     for M in mats:
         s = M.storage
-        if M._kind != "general" or s.bc is None:
-            raise SlateError(f"{what}: general block-cyclic matrices are wanted")
-        if s.origin_slot is None:
-            raise SlateError(f"{what}: a matrix has no tiles (insertLocalTiles)")
-        x = _opd(M)
+        slot = s.origin_slot
+        x = M.__dict__.get("_operand")
+        # (a remembered operand was looked at before; its use, as in _opd, without the call)
+        now = s.table.version()
+        if x is None or s.local.get(slot) is not x.buf or s._valid.get(slot) != now \
+                or x.trans != (M._op is not Op.NoTrans) or x.t.data_ptr() != x.ptr:
+            if M._kind != "general" or s.bc is None:
+                raise SlateError(f"{what}: general block-cyclic matrices are wanted")
+            if slot is None:
+                raise SlateError(f"{what}: a matrix has no tiles (insertLocalTiles)")
+            x = _opd(M)
+            now = s.table.version()
         if dt is None:
             dt, dev, comm = x.dt, x.dev, s.comm
-        elif x.dt is not dt or x.dev != dev:
+        elif x.dt is not dt or x.dev is not dev:
             raise SlateError(f"{what}: the matrices differ in type or device ({x.dt} on {x.dev}, {dt} on {dev})")
         elif s.comm is not comm and s.comm.ranks != comm.ranks:
             raise SlateError(f"{what}: the matrices differ in communicator")
-        out.append(x)
-    return out
+        if s._marked != (slot, now):
+            todo.append(s)
+        add(x)
+    return out, todo
 
 
 def _clip_apart(what, va, vb):
@@ -740,12 +754,14 @@ _PARTS = {torch.complex64: torch.float32, torch.complex128: torch.float64}
 
 
 def _clip(what, limit, A, B):
-    va = _clip_views(A, what)
+    va, todo = _clip_views(A, what)
     if not va:
         return torch.zeros((), dtype=torch.float64)
-    vb = va if B is A else _clip_views(B, what)
+    vb = va
+    if B is not A:
+        vb, todo = _clip_views(B, what)
     t, comm = va[0].t, A[0].storage.comm
-    if len(vb) != len(va) or (vb is not va and vb[0].dev != va[0].dev):
+    if len(vb) != len(va) or (vb is not va and vb[0].dev is not va[0].dev):
         raise SlateError(f"{what}: B has {len(vb)} matrices, A has {len(va)}, or they are on different devices")
     ta, tb = va[0].dt, vb[0].dt
     if _PARTS.get(ta, ta) not in REAL_CODE or not (ta == tb or (_BYTES[ta] == 2 and tb == torch.float32)):
@@ -753,18 +769,18 @@ def _clip(what, limit, A, B):
     two = 2 if ta in _PARTS else 1
     ca, cb = REAL_CODE[_PARTS.get(ta, ta)], REAL_CODE[_PARTS.get(tb, tb)]
     with trace_block(what):
-        if vb is not va:
-            for X, Y, x, y in zip(A, B, va, vb):
-                if x.trans != y.trans or x.rows != y.rows or x.cols != y.cols or \
-                        (comm.size > 1 and (X.m() != Y.m() or X.n() != Y.n() or not _same_place(X, Y))):
-                    raise SlateError(f"{what}: B's matrices want the shapes, ops and distribution of A's")
-        if limit is not None:
-            _clip_apart(what, va, vb)
-        mod, st = kmod(t), raw_stream(t)
         # (A, lda, B, ldb, rows, columns) of every matrix; complex ones as pairs
         mats = []
         for x, y in zip(va, vb):
-            mats += (x.ptr, x.ld * two, y.ptr, y.ld * two, x.rows * two, x.cols)
+            rows, cols = x.rows, x.cols
+            if rows != y.rows or cols != y.cols or x.trans is not y.trans:
+                raise SlateError(f"{what}: B's matrices want the shapes and ops of A's")
+            mats += (x.ptr, x.ld * two, y.ptr, y.ld * two, rows * two, cols)
+        if vb is not va and comm.size > 1:
+            for X, Y in zip(A, B):
+                if X.m() != Y.m() or X.n() != Y.n() or not _same_place(X, Y):
+                    raise SlateError(f"{what}: B's matrices want the shapes and distribution of A's")
+        mod, st = kmod(t), raw_stream(t)
         top, scale = (0.0, False) if limit is None else (limit, True)
         with _on(t):
             # [norm, the ranks' common sums (3), partial sums]
@@ -772,14 +788,19 @@ def _clip(what, limit, A, B):
             norm = ws.data_ptr()
             part = norm + 32
             if comm.size == 1:
-                mod.clip_norm(ca, cb, mats, top, part, norm, scale, st)
+                if not mod.clip_norm(ca, cb, mats, top, part, norm, scale, True, st):
+                    _clip_apart(what, va, vb)
+                    mod.clip_norm(ca, cb, mats, top, part, norm, scale, False, st)
             else:
+                if scale:
+                    _clip_apart(what, va, vb)
                 n = mod.clip_sum(ca, mats, part, st)
                 mod.clip_join(part, n, norm + 8, st)
                 comm.allreduce(ws[1:4], "sum")
                 mod.clip_scale(ca, cb, mats, top, norm + 8, 1, norm, scale, st)
-        if limit is not None:
-            _modified(*B)
+        if scale:
+            for s in todo:
+                s.mark_local_modified(s.origin_slot)
     return ws[0]
 
 
