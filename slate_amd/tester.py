@@ -15,7 +15,8 @@ Cholesky potrf potrs posv potri trtri posv_mixed; LU getrf getrs gesv
 getri gesv_nopiv gesv_tntpiv/calu gesv_rbt gesv_mixed gesv_mixed_gmres;
 band gbsv pbsv gbmm hbmm tbsm; QR/LQ geqrf unmqr gelqf cholqr gels;
 eigen/SVD heev/syev heev_vals hegv/sygv svd svd_vals; indefinite
-hesv/sysv; aux norm colnorms add redistribute gecondest pocondest
+hesv/sysv; feed-forward (types s, d) gemm_bias_act gemm_gated, their
+_grad, clip_norm; aux norm colnorms add redistribute gecondest pocondest
 trcondest matgen.
 """
 from __future__ import annotations
@@ -104,6 +105,71 @@ def t_gemm(c, m, n, k, **p):
     _, t = c.timed(lambda: sl.gemm(1.0, A, B, 1.0, C, c.opts))
     err = _rel(D(C) - (Ad @ Bd + Cd), Ad.abs().max() * Bd.abs().max() * k) if c.a.check == 'y' else None
     return err, t, 2.0 * m * n * k
+
+
+def _real_types(f):
+    """A routine of real matrices: types c and z run as s and d."""
+    return lambda c, m, n, k, **p: f(Ctx(c.a, {'c': 's', 'z': 'd'}.get(c.t, c.t)), m, n, k, **p)
+
+
+def _silu(z):
+    s = torch.sigmoid(z)
+    return z * s, s * (1 + z * (1 - s))
+
+
+@_real_types
+def t_gemm_bias_act(c, m, n, k, **p):
+    A, B, b, R, C, Z = (c.mat(*d, seed=i) for i, d in enumerate(((m, k), (k, n), (m, 1), (m, n), (m, n), (m, n)), 1))
+    _, t = c.timed(lambda: sl.gemm_bias_act(1.0, A, B, b, "silu", 1.0, R, C, Z, c.opts))
+    z = D(A) @ D(B) + D(b)
+    scale = D(A).abs().max() * D(B).abs().max() * k + 1
+    err = max(_rel(D(Z) - z, scale), _rel(D(C) - (_silu(z)[0] + D(R)), scale)) if c.a.check == 'y' else None
+    return err, t, 2.0 * m * n * k
+
+
+@_real_types
+def t_gemm_bias_act_grad(c, m, n, k, **p):
+    A, B, Z, G = c.mat(m, k, seed=1), c.mat(k, n, seed=2), c.mat(m, n, seed=3), c.mat(m, n, seed=4)
+    dA, dB, db = c.mat(m, k, seed=5), c.mat(k, n, seed=6), c.mat(m, 1, seed=7)
+    _, t = c.timed(lambda: sl.gemm_bias_act_grad(1.0, A, B, "silu", Z, G, dA, dB, db, c.opts))
+    dz = D(G) * _silu(D(Z))[1]
+    err = max(_rel(D(dA) - dz @ D(B).mT, dz.abs().max() * n), _rel(D(dB) - D(A).mT @ dz, dz.abs().max() * m),
+              _rel(D(db) - dz.sum(1, keepdim=True), dz.abs().max() * n)) if c.a.check == 'y' else None
+    return err, t, 4.0 * m * n * k
+
+
+@_real_types
+def t_gemm_gated(c, m, n, k, **p):
+    A1, A2, B, C = c.mat(m, k, seed=1), c.mat(m, k, seed=2), c.mat(k, n, seed=3), c.mat(m, n, seed=4)
+    _, t = c.timed(lambda: sl.gemm_gated(A1, A2, B, "silu", C, opts=c.opts))
+    z1, z2 = D(A1) @ D(B), D(A2) @ D(B)
+    err = _rel(D(C) - _silu(z1)[0] * z2, (1 + z1.abs().max()) * (1 + z2.abs().max()) * k) if c.a.check == 'y' else None
+    return err, t, 4.0 * m * n * k
+
+
+@_real_types
+def t_gemm_gated_grad(c, m, n, k, **p):
+    A1, A2, B = c.mat(m, k, seed=1), c.mat(m, k, seed=2), c.mat(k, n, seed=3)
+    Z1, Z2, G = c.mat(m, n, seed=4), c.mat(m, n, seed=5), c.mat(m, n, seed=6)
+    g1, g2, gb = c.mat(m, k, seed=7), c.mat(m, k, seed=8), c.mat(k, n, seed=9)
+    _, t = c.timed(lambda: sl.gemm_gated_grad(A1, A2, B, "silu", Z1, Z2, G, g1, g2, gb, c.opts))
+    v, s = _silu(D(Z1))
+    d1, d2 = D(G) * D(Z2) * s, D(G) * v
+    big = max(d1.abs().max(), d2.abs().max())
+    err = max(_rel(D(g1) - d1 @ D(B).mT, big * n), _rel(D(g2) - d2 @ D(B).mT, big * n),
+              _rel(D(gb) - (D(A1).mT @ d1 + D(A2).mT @ d2), 2 * big * m)) if c.a.check == 'y' else None
+    return err, t, 8.0 * m * n * k
+
+
+def t_clip_norm(c, m, n, k, **p):
+    A = [c.mat(m, n, seed=1), c.mat(n, k, seed=2), c.mat(k, 1, seed=3)]
+    was = [D(X) for X in A]
+    s, t = c.timed(lambda: sl.clip_norm(0.5, A))
+    want = sum(float((x.abs().double() ** 2).sum()) for x in was) ** 0.5
+    f = min(1.0, 0.5 / want)
+    err = max([abs(float(s) - want) / want] + [_rel(D(X) - f * x, f * x.abs().max()) for X, x in zip(A, was)]) \
+        if c.a.check == 'y' else None
+    return err, t, 3.0 * (m * n + n * k + k)
 
 
 def t_herk(c, m, n, k, uplo=Uplo.Lower, **p):
@@ -1020,7 +1086,8 @@ def t_bdsqr(c, m, n, k, **p):
     return err, t, 12.0 * n ** 3
 
 
-ROUTINES = {"gemm": t_gemm, "herk": t_herk, "syrk": t_herk, "trsm": t_trsm, "potrf": t_potrf,
+ROUTINES = {"gemm": t_gemm, "gemm_bias_act": t_gemm_bias_act, "gemm_bias_act_grad": t_gemm_bias_act_grad,
+            "gemm_gated": t_gemm_gated, "gemm_gated_grad": t_gemm_gated_grad, "clip_norm": t_clip_norm, "herk": t_herk, "syrk": t_herk, "trsm": t_trsm, "potrf": t_potrf,
             "posv": t_posv, "getrf": t_getrf, "gesv": t_gesv, "geqrf": t_geqrf, "gels": t_gels,
             "heev": t_heev, "syev": t_heev, "svd": t_svd, "norm": t_norm, "genorm": t_norm,
             "gesv_mixed": t_gesv_mixed, "hesv": t_hesv, "sysv": t_hesv,
