@@ -25,6 +25,7 @@ struct GemmActArgs {
     int act = ACT_IDENTITY;
     // filled by the launcher
     i64 kfull = 0;          // first k that LDS-DMA does not stage
+    i64 lenA = 0, lenB = 0; // length of the operands' columns, 16 bytes or more where they go through registers
     int nsteps = 0;         // K steps per product
     int group_m = 8;
     int splits = 1, per_split = 0;

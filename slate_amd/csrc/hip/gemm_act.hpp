@@ -367,6 +367,31 @@ template <typename T, int R, bool KC> struct GaImg {
         const u128 x = __builtin_bit_cast(u128, w) >> (down & 127);
         return __builtin_bit_cast(i4v, down < 128 ? x : (u128)0);
     }
+    // The same for slabs that all go through registers: what a slot's addresses
+    // need, made once, and a load without a branch (the loads of two slabs are in
+    // flight, and a load behind a branch would be waited for at once).  avail: the
+    // columns' length (MN: from the tile's first row), 16 bytes or more.
+    struct Slot { i64 el, el0; int k, cut; };
+    __device__ static inline Slot slot(int q, i64 ld, i64 rows, i64 avail) {
+        int r, k;
+        src_of(q, r, k);
+        if constexpr (KC) return {min((i64)r, rows - 1) * ld + k, 0, k, 0};
+        else {
+            const i64 over = max((i64)0, r + E - avail);
+            return {k * ld + r - over, r - over, k, over < E ? (int)over * ES * 8 : 128};
+        }
+    }
+    __device__ static inline i4v load(const T* X, const Slot& t, int kl, int& down) {
+        using vE = ga_vec<T, E>;
+        if constexpr (KC) {
+            const int over = max(0, t.k + E - kl);
+            down = over < E ? over * ES * 8 : 128;
+            return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(X + (t.el - over)));
+        } else {
+            down = t.k < kl ? t.cut : 128;
+            return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(X + (t.k < kl ? t.el : t.el0)));
+        }
+    }
     // A slab with an end of the matrix in it, wave wid of NW.  DMA of 16 bytes:
     // accesses that lie inside go to LDS directly, the others from registers.
     // DMA of 4: all from registers in 16-byte accesses (four times fewer; 452 x 17
@@ -424,8 +449,7 @@ template <typename T, int BM, int BN, int WVM, int WVN, int S> struct GaEpi {
 // 16 where the operands' rows lie on 16 bytes, 4 for 32- and 64-bit elements
 // elsewhere: four times the instructions, still asynchronous (1503 x 777 x 1001
 // f32: 38 us against 53 us through registers).  0: every slab goes through
-// registers, fetched before the products of the slab ahead of it and written to
-// LDS after them.
+// registers, two slabs ahead of its products.
 template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int S, bool GATED, int DMA>
 __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a) {
     using TR = ga_traits<T>;
@@ -515,71 +539,72 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
         }
     };
 
-    // through registers
+    // through registers: slab s + 1 is in one of two sets while slab s is
+    // multiplied and slab s + 2 is fetched into the other
     constexpr int QA = IA::BYTES / 16, QB = IB::BYTES / 16, CA = DMA ? 1 : (QA + NT - 1) / NT, CB = DMA ? 1 : (QB + NT - 1) / NT;
-    i4v ra[NA][CA], rb[CB];
-    int sa[NA][CA], sb[CB];
-    bool inside = true;
-    i64 elA[NA][CA], elB[CB];
-    auto elements = [&](int p) {
-        #pragma unroll
-        for (int h = 0; h < NA; ++h)
-            #pragma unroll
-            for (int i = 0; i < CA; ++i) elA[h][i] = IA::element(min(tid + i * NT, QA - 1), a.lda[GATED ? h : p], rowsA);
-        #pragma unroll
-        for (int i = 0; i < CB; ++i) elB[i] = IB::element(min(tid + i * NT, QB - 1), a.ldb[p], rowsB);
+    struct Held {
+        i4v a[NA][CA], b[CB];
+        int sa[NA][CA], sb[CB];
+        bool whole;
     };
+    typename IA::Slot slotA[NA][CA];
+    typename IB::Slot slotB[CB];
     const T *ya[NA], *yb;
-    i64 ea[NA], eb, lea[NA], leb;
+    i64 ea[NA], eb;
+    const i64 kA = AKC ? a.lenA : a.k, kB = BKC ? a.lenB : a.k, availA = a.lenA - m0, availB = a.lenB - n0;
+    int fetched = s0;
     auto point = [&](int p, i64 k0) {
-        elements(p);
         #pragma unroll
         for (int h = 0; h < NA; ++h) {
+            const i64 ld = a.lda[GATED ? h : p];
             ya[h] = slabA(GATED ? h : p, k0);
-            lea[h] = a.lda[GATED ? h : p];
-            ea[h] = AKC ? KB : KB * lea[h];
+            ea[h] = AKC ? KB : KB * ld;
+            #pragma unroll
+            for (int i = 0; i < CA; ++i) slotA[h][i] = IA::slot(min(tid + i * NT, QA - 1), ld, rowsA, availA);
         }
+        const i64 ld = a.ldb[p];
         yb = slabB(p, k0);
-        leb = a.ldb[p];
-        eb = BKC ? KB : KB * leb;
+        eb = BKC ? KB : KB * ld;
+        #pragma unroll
+        for (int i = 0; i < CB; ++i) slotB[i] = IB::slot(min(tid + i * NT, QB - 1), ld, rowsB, availB);
     };
     if constexpr (!DMA) point(curp, (i64)kt * KB);
-    const i64 kall = a.k, am = a.m, an = a.n;
-    auto fetch = [&]() {
+    // (after the last slab it reads that one again)
+    auto fetch = [&](Held& x) {
         if (sum && kt == nsteps) { kt = 0; curp = 1; point(1, 0); }
-        const i64 left = kall - (i64)kt++ * KB;
-        inside = left >= KB && (AKC || rowsA >= BMI) && (BKC || rowsB >= BN);
+        const int lA = (int)min(kA - (i64)kt * KB, (i64)KB), lB = (int)min(kB - (i64)kt * KB, (i64)KB);
+        x.whole = lA == KB && lB == KB && (AKC || availA >= BMI) && (BKC || availB >= BN);
         #pragma unroll
         for (int h = 0; h < NA; ++h)
             #pragma unroll
-            for (int i = 0; i < CA; ++i)
-                ra[h][i] = IA::fetch(ya[h], elA[h][i], min(tid + i * NT, QA - 1), lea[h], AKC ? kall : am, rowsA, left, inside,
-                                     sa[h][i]);
+            for (int i = 0; i < CA; ++i) x.a[h][i] = IA::load(ya[h], slotA[h][i], lA, x.sa[h][i]);
         #pragma unroll
-        for (int i = 0; i < CB; ++i) rb[i] = IB::fetch(yb, elB[i], min(tid + i * NT, QB - 1), leb, BKC ? kall : an, rowsB, left, inside, sb[i]);
-        #pragma unroll
-        for (int h = 0; h < NA; ++h) ya[h] += ea[h];
-        yb += eb;
+        for (int i = 0; i < CB; ++i) x.b[i] = IB::load(yb, slotB[i], lB, x.sb[i]);
+        if (++fetched < s1) {
+            ++kt;
+            #pragma unroll
+            for (int h = 0; h < NA; ++h) ya[h] += ea[h];
+            yb += eb;
+        }
     };
-    auto write = [&](int s) {
+    auto write = [&](int s, const Held& x) {
         char* slot = smem + (s % S) * SLOT;
         auto put = [&](auto whole) {
             #pragma unroll
             for (int h = 0; h < NA; ++h)
                 #pragma unroll
-                for (int i = 0; i < CA; ++i) {
-                    if constexpr (!whole) ra[h][i] = IA::shift(ra[h][i], sa[h][i]);
-                    *reinterpret_cast<i4v*>(slot + h * IA::BYTES + min(tid + i * NT, QA - 1) * 16) = ra[h][i];
-                }
+                for (int i = 0; i < CA; ++i)
+                    *reinterpret_cast<i4v*>(slot + h * IA::BYTES + min(tid + i * NT, QA - 1) * 16) =
+                        whole ? x.a[h][i] : IA::shift(x.a[h][i], x.sa[h][i]);
             #pragma unroll
-            for (int i = 0; i < CB; ++i) {
-                if constexpr (!whole) rb[i] = IB::shift(rb[i], sb[i]);
-                *reinterpret_cast<i4v*>(slot + BM * 128 + min(tid + i * NT, QB - 1) * 16) = rb[i];
-            }
+            for (int i = 0; i < CB; ++i)
+                *reinterpret_cast<i4v*>(slot + BM * 128 + min(tid + i * NT, QB - 1) * 16) =
+                    whole ? x.b[i] : IB::shift(x.b[i], x.sb[i]);
         };
-        if (inside) put(std::true_type());
+        if (x.whole) put(std::true_type());
         else put(std::false_type());
     };
+    Held held0, held1;
 
     const int wm = wid / WVN, wn = wid % WVN;
     acc4 acc[MI][NI];
@@ -595,7 +620,11 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             #pragma unroll
             for (int i = 0; i < S - 1; ++i)
                 if (s0 + i < s1) issue(smem + (s0 + i) % S * SLOT);
-        } else { fetch(); write(s0); }
+        } else {
+            fetch(held0);
+            write(s0, held0);
+            fetch(held1);
+        }
     }
     auto reads = [&](const char* la, int kk, i4v (&fa)[MI], i4v (&fb)[NI]) {
         constexpr int H = MI / NA;
@@ -659,20 +688,18 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
         }
         if (!late) turn();
     } else {
-        for (int s = s0; s < s1; ++s) {
+        auto step = [&](int s, Held& next, Held& spare) __attribute__((always_inline)) {
             // my part of step s has landed (of the steps behind it, LOADS each are in
             // flight; a step that went through registers waited for all before it) ...
-            if (S > 2 && s + S - 2 < s1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * LOADS) : "memory");
+            if constexpr (!DMA) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            else if (S > 2 && s + S - 2 < s1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * LOADS) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             // ... and everyone's, and everyone has read step s - 1's slot
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             auto work = [&](const char* __restrict la, char* __restrict fill) __attribute__((always_inline)) {
-                if constexpr (DMA) {
-                    if (s + S - 1 < s1) issue(fill);
-                } else if (s + 1 < s1) {
-                    fetch();
-                }
+                if constexpr (!DMA) fetch(spare);
+                else if (s + S - 1 < s1) issue(fill);
                 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
                     i4v fa[MI], fb[NI];
@@ -682,7 +709,15 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             };
             work(smem + s % S * SLOT, smem + (s + S - 1) % S * SLOT);
             if constexpr (!DMA)
-                if (s + 1 < s1) write(s + 1);
+                if (s + 1 < s1) write(s + 1, next);
+        };
+        if constexpr (DMA) {
+            for (int s = s0; s < s1; ++s) step(s, held0, held1);
+        } else {
+            for (int s = s0; s < s1; s += 2) {
+                step(s, held1, held0);
+                if (s + 1 < s1) step(s + 1, held0, held1);
+            }
         }
     }
 
@@ -834,8 +869,8 @@ __global__ void __launch_bounds__(64 * NW) gemm_act_skinny_kernel(GemmActArgs a)
     }
 }
 
-// 16-bit columns laid out anew on 16 bytes, so that LDS-DMA takes them; a
-// thread moves four 16-byte vectors.
+// Columns laid out anew on 16 bytes, with zeros behind their ends, so that
+// LDS-DMA takes them; a thread moves four 16-byte vectors.
 template <typename T>
 __global__ void __launch_bounds__(256) ga_pack_kernel(const T* X, i64 ld, T* Y, i64 len, i64 cols) {
     constexpr int E = 16 / (int)sizeof(T), U = 4;

@@ -46,13 +46,13 @@ struct GaOperand {
     bool bad = false;        // rows not on 16 bytes, or 32-bit offsets too short
     i64 at = -1;             // its place in the workspace
     bool fits(i64 l, int es) const { return (kc ? 256 : 128 / es) * l * es < (i64)1 << 31; }
-    i64 whole() const { return (len + 7) / 8 * 8; }
+    i64 whole(int es) const { return (len * es + 15) / 16 * (16 / es); }
 };
 
 // can all operands that need it be laid out anew?
 inline bool ga_packed(const GaOperand* op, int n, int es) {
     for (int i = 0; i < n; ++i)
-        if (op[i].bad && !op[i].fits(op[i].whole(), es)) return false;
+        if (op[i].bad && !op[i].fits(op[i].whole(es), es)) return false;
     return true;
 }
 
@@ -67,7 +67,7 @@ inline i64 ga_place(GaOperand* op, int n, int es, i64 bytes) {
                 op[i].at = op[j].at;
         if (op[i].at >= 0) continue;
         op[i].at = bytes;
-        bytes += (op[i].whole() * op[i].cols * es + 255) / 256 * 256;
+        bytes += (op[i].whole(es) * op[i].cols * es + 255) / 256 * 256;
     }
     return bytes;
 }
@@ -78,7 +78,7 @@ template <typename T> void ga_pack(GaOperand* op, int n, char* ws, hipStream_t s
         T* y = reinterpret_cast<T*>(ws + op[i].at);
         bool done = false;
         for (int j = 0; j < i; ++j) done = done || op[j].at == op[i].at;
-        const i64 nv = op[i].whole() / 8, ld = op[i].whole();
+        const i64 ld = op[i].whole(sizeof(T)), nv = ld * (i64)sizeof(T) / 16;
         if (!done && nv * op[i].cols)
             hipLaunchKernelGGL((ga_pack_kernel<T>), dim3((unsigned)((nv * op[i].cols + 1023) / 1024)), dim3(256), 0, s,
                                static_cast<const T*>(*op[i].ptr), *op[i].ld, y, op[i].len, op[i].cols);
@@ -126,14 +126,16 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
         ga_skinny<T>(a, gated, s);
         return 0;
     }
+    const bool regs = !dma && !pack && !(ES >= 4 && small);
+    if (regs)            // through registers: columns of 16 bytes or more
+        for (int i = 0; i < nop; ++i) op[i].bad = op[i].len < E;
     i64 bytes = (p.bytes + 255) / 256 * 256;
-    if (pack) bytes = ga_place(op, nop, ES, bytes);
+    if (pack || regs) bytes = ga_place(op, nop, ES, bytes);
     if (bytes && !a.part) return bytes;
-    if constexpr (ES == 2)
-        if (pack) {
-            dma = true;
-            ga_pack<T>(op, nop, static_cast<char*>(a.part), s);
-        }
+    if (pack || regs) ga_pack<T>(op, nop, static_cast<char*>(a.part), s);
+    dma = dma || pack;
+    a.lenA = op[0].at < 0 ? op[0].len : op[0].whole(ES);
+    a.lenB = op[na].at < 0 ? op[na].len : op[na].whole(ES);
     a.kfull = a.k / KB * KB;
     for (int i = 0; i < nop; ++i)
         if (!op[i].kc && op[i].len % E && op[i].at < 0 && a.k) a.kfull = std::min<i64>(a.kfull, (a.k - 1) / KB * KB);

@@ -877,3 +877,33 @@ def test_far_offsets():
         want = torch.stack([want, 2 * want])
         within(C.cpu(), want, 2.0 ** -8 * want.abs())
         del X, Y
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT", "TT"])
+@pytest.mark.parametrize("pad,off", [(0, 0), (1, 1)])
+def test_short_columns(dev, dt, ta, tb, pad, off):
+    """Columns of fewer than 16 bytes, aligned and not."""
+    for m, n, k in ((5, 40, 3), (3, 70, 6), (90, 5, 7), (7, 33, 70), (70, 1, 1), (1, 20, 9)):
+        Product(dt, dev, m, n, k, ta, tb, pad=pad, off=off).check()
+    Gated(dt, dev, 6, 35, 5, ta, tb, pad=pad, off=off).check()
+    Gated(dt, dev, 6, 35, 5, ta, tb, pad=pad, off=off).check_grad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("m,n,k", [(70, 40, 130), (40, 20, 3), (3, 90, 70)])
+def test_wide_leading_dimension(dt, m, n, k):
+    """Columns so far apart that 32 bits do not reach over a tile."""
+    es = torch.finfo(dt).bits // 8
+    far = 2 ** 31 // 256 // es + 5                        # along k; columns across it in the second call
+    for ta, far in (("T", far), ("N", min(2 ** 24, 2 ** 32 // (k * es)) + 3)):
+        p = Product(dt, "cuda", m, n, k, ta, "N")
+        rows, cols = p.A.shape
+        buf = torch.full((cols * far,), float("nan"), dtype=dt, device="cuda")
+        A = buf.as_strided((rows, cols), (1, far))
+        A.copy_(p.A)
+        p.A = A
+        p.check()
+        del buf, A
