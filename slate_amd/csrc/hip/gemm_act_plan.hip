@@ -5,12 +5,12 @@
 namespace slate_hip {
 
 // Laying misaligned 16-bit operands out anew costs a pass over them and two
-// launches; the products gain LDS-DMA and with it the larger tiles: 4096^3 146
-// against 426 us, 512 x 4096 x 4096 56 against 72, 2000^3 53 against 54; where
-// the operands are long for what is computed it loses: 4096 x 128 x 4096 35
-// against 28 us, 1000^3 24 against 19.
+// launches; the products gain LDS-DMA and with it the larger tiles: 4096^3 144
+// against 362 us, 512 x 4096 x 4096 47 against 61, 2000^3 51 against 52; where
+// the operands are long for what is computed, or small, it loses: 4096 x 128 x
+// 4096 35 against 28 us, 1000^3 20 against 15.
 bool gemm_act_pack(int mode, i64 m, i64 n, i64 k) {
-    return (mode == GA_PLAIN ? 1 : 2) * m * n * k >= (i64)1 << 33 && m * n >= 256 * (m + n);
+    return (mode == GA_PLAIN ? 1 : 2) * m * n * k >= 8000000000 && m * n >= 256 * (m + n);
 }
 
 namespace {
@@ -27,7 +27,7 @@ namespace {
 // products wait for the MFMAs, not for what a larger tile would save: 64 x 64
 // f32 133 us at 2000^3 (128 x 128: 143), 992 at 4096^3 (967 to 1010), f64 290
 // (350) and 2220 (2720).  (1024 x 4096 x 1024 of 16-bit operands that go through
-// registers: 30 us, 2048 x 4096 x 512 31; with 128 x 128 tiles 39.)
+// registers: 31 us, 2048 x 4096 x 512 33; with 128 x 128 tiles 39.)
 enum { HALF_DMA, HALF_REGS, SINGLE, DOUBLE };
 struct GaCost { int kind, tile, size, per_cu; double step[4], ends[4]; };
 const GaCost ga_costs[] = {
@@ -35,7 +35,7 @@ const GaCost ga_costs[] = {
     {HALF_DMA, 1, 128, 2, {0.70, 0.95}, {4, 7}},
     {HALF_DMA, 2, 64, 4, {0.515, 0.54, 0.60, 0.68}, {1, 2, 3, 3}},
     {HALF_DMA, 4, 64, 3, {0.36, 0.45, 0.60}, {1, 2, 3}},
-    {HALF_REGS, 2, 64, 4, {0.80, 0.82, 0.95, 1.40}, {1, 2, 3, 3}},
+    {HALF_REGS, 2, 64, 4, {0.55, 0.78, 1.10, 1.50}, {1, 2, 3, 3}},
     {SINGLE, 2, 64, 4, {0.72, 1.10, 1.65, 2.15}, {1, 2, 3, 3}},
     {DOUBLE, 2, 64, 4, {0.80, 1.25, 1.85, 2.40}, {1, 2, 3, 3}},
 };
