@@ -37,37 +37,36 @@ typedef _Float16 hf8v __attribute__((ext_vector_type(8)));
 template <typename T, int V> struct ga_vec_of { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
 template <typename T, int V> using ga_vec = typename ga_vec_of<T, V>::type;
 
+// mma: the u-th of the N MFMAs that multiply two fragments
 template <typename T> struct ga_traits;
 template <> struct ga_traits<__bf16> {
     using acc = float; using acc4 = f4;
-    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c) {
+    static constexpr int N = 1;
+    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c, int) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c,
                                                        0, 0, 0);
     }
 };
 template <> struct ga_traits<_Float16> {
     using acc = float; using acc4 = f4;
-    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c) {
+    static constexpr int N = 1;
+    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c, int) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8v, a), __builtin_bit_cast(hf8v, b), c,
                                                       0, 0, 0);
     }
 };
 template <> struct ga_traits<float> {
     using acc = float; using acc4 = f4;
-    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c) {
-        const f4 x = __builtin_bit_cast(f4, a), y = __builtin_bit_cast(f4, b);
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-        return c;
+    static constexpr int N = 4;
+    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c, int u) {
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, a)[u], __builtin_bit_cast(f4, b)[u], c, 0, 0, 0);
     }
 };
 template <> struct ga_traits<double> {
     using acc = double; using acc4 = d4;
-    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c) {
-        const d2 x = __builtin_bit_cast(d2, a), y = __builtin_bit_cast(d2, b);
-        #pragma unroll
-        for (int j = 0; j < 2; ++j) c = __builtin_amdgcn_mfma_f64_16x16x4f64(x[j], y[j], c, 0, 0, 0);
-        return c;
+    static constexpr int N = 2;
+    __device__ static inline acc4 mma(i4v a, i4v b, acc4 c, int u) {
+        return __builtin_amdgcn_mfma_f64_16x16x4f64(__builtin_bit_cast(d2, a)[u], __builtin_bit_cast(d2, b)[u], c, 0, 0, 0);
     }
 };
 
@@ -450,8 +449,11 @@ template <typename T, int BM, int BN, int WVM, int WVN, int S> struct GaEpi {
 // elsewhere: four times the instructions, still asynchronous (1503 x 777 x 1001
 // f32: 38 us against 53 us through registers).  0: every slab goes through
 // registers, two slabs ahead of its products.
+// Two workgroups a CU at least: with one, the compiler keeps the sums in vector
+// registers between steps and copies them to accumulation registers and back in
+// each (f64 4096^3 2230 us against 2010).
 template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int S, bool GATED, int DMA>
-__global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a) {
+__global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs a) {
     using TR = ga_traits<T>;
     using acc4 = typename TR::acc4;
     using R = typename TR::acc;
@@ -635,16 +637,19 @@ __global__ void __launch_bounds__(64 * WVM * WVN) gemm_act_kernel(GemmActArgs a)
             fa[i] = IA::frag(la + (i / H) * IA::BYTES, wm * (WM / NA) + (i % H) * 16, kk, lane);
     };
     auto products = [&](const i4v (&fa)[MI], const i4v (&fb)[NI]) {
+        // (an accumulator's next MFMA comes after all the others')
         #pragma unroll
-        for (int i = 0; i < MI; ++i)
+        for (int u = 0; u < TR::N; ++u)
             #pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                // D's four registers run along the rows of the first operand: rows
-                // of C for f32 sums; for f64 they are 4 apart, and the columns take
-                // them so that lanes run along the rows
-                if constexpr (sizeof(R) == 4) acc[i][j] = TR::mma(fa[i], fb[j], acc[i][j]);
-                else acc[i][j] = TR::mma(fb[j], fa[i], acc[i][j]);
-            }
+            for (int i = 0; i < MI; ++i)
+                #pragma unroll
+                for (int j = 0; j < NI; ++j) {
+                    // D's four registers run along the rows of the first operand: rows
+                    // of C for f32 sums; for f64 they are 4 apart, and the columns take
+                    // them so that lanes run along the rows
+                    if constexpr (sizeof(R) == 4) acc[i][j] = TR::mma(fa[i], fb[j], acc[i][j], u);
+                    else acc[i][j] = TR::mma(fb[j], fa[i], acc[i][j], u);
+                }
     };
     // (In both loops the slab read and the one filled are restrict parameters:
     // different memory, or the compiler waits for the DMA before each transposed
@@ -808,10 +813,12 @@ __global__ void __launch_bounds__(64 * NW) gemm_act_skinny_kernel(GemmActArgs a)
         for (int r = 0; r < 4; ++r) acc[h][r] = R(0);
     auto mul = [&](const i4v (&fa)[NA], i4v fb) {
         #pragma unroll
-        for (int h = 0; h < NA; ++h) {
-            if constexpr (sizeof(R) == 4) acc[h] = TR::mma(fa[h], fb, acc[h]);
-            else acc[h] = TR::mma(fb, fa[h], acc[h]);
-        }
+        for (int u = 0; u < TR::N; ++u)
+            #pragma unroll
+            for (int h = 0; h < NA; ++h) {
+                if constexpr (sizeof(R) == 4) acc[h] = TR::mma(fa[h], fb, acc[h], u);
+                else acc[h] = TR::mma(fb, fa[h], acc[h], u);
+            }
     };
     const int slabs = (int)(a.k / KB);
     int s = w;

@@ -25,9 +25,9 @@ namespace {
 // two slots 39), 2048 x 2048 x 4096 51 with two slots (99, 53, three slots 60: a
 // CU holds four workgroups of the one, three of the other).  32- and 64-bit
 // products wait for the MFMAs, not for what a larger tile would save: 64 x 64
-// f32 133 us at 2000^3 (128 x 128: 143), 992 at 4096^3 (967 to 1010), f64 290
-// (350) and 2220 (2720).  (1024 x 4096 x 1024 of 16-bit operands that go through
-// registers: 31 us, 2048 x 4096 x 512 33; with 128 x 128 tiles 39.)
+// f32 134 us at 2000^3 (128 x 128: 142 in two pieces), 989 at 4096^3 (966), f64
+// 256 (275) and 2020 (1943).  (1024 x 4096 x 1024 of 16-bit operands that go
+// through registers: 31 us, 2048 x 4096 x 512 33; with 128 x 128 tiles 39.)
 enum { HALF_DMA, HALF_REGS, SINGLE, DOUBLE };
 struct GaCost { int kind, tile, size, per_cu; double step[4], ends[4]; };
 const GaCost ga_costs[] = {
@@ -36,8 +36,8 @@ const GaCost ga_costs[] = {
     {HALF_DMA, 2, 64, 4, {0.515, 0.54, 0.60, 0.68}, {1, 2, 3, 3}},
     {HALF_DMA, 4, 64, 3, {0.36, 0.45, 0.60}, {1, 2, 3}},
     {HALF_REGS, 2, 64, 4, {0.55, 0.78, 1.10, 1.50}, {1, 2, 3, 3}},
-    {SINGLE, 2, 64, 4, {0.72, 1.10, 1.65, 2.15}, {1, 2, 3, 3}},
-    {DOUBLE, 2, 64, 4, {0.80, 1.25, 1.85, 2.40}, {1, 2, 3, 3}},
+    {SINGLE, 2, 64, 4, {0.72, 1.10, 1.60, 2.10}, {1, 2, 3, 3}},
+    {DOUBLE, 2, 64, 4, {0.72, 1.15, 1.55, 2.05}, {1, 2, 3, 3}},
 };
 double ga_time(const GaCost& c, i64 wgs, int steps) {
     const i64 full = wgs / (256 * c.per_cu), rest = wgs - full * 256 * c.per_cu;
