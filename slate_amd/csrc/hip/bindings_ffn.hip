@@ -24,16 +24,16 @@ template <typename F> void real_dispatch(char dt, F&& f) {
     }
 }
 
-// six integers per matrix: A, lda, B, ldb, rows, columns
 std::vector<i64> ints(const py::list& v) {
     const Py_ssize_t n = PyList_GET_SIZE(v.ptr());
-    if (n % 6) throw std::invalid_argument("clip: six integers per matrix are wanted");
     std::vector<i64> x(n);
     for (Py_ssize_t i = 0; i < n; ++i) x[i] = PyLong_AsLongLong(PyList_GET_ITEM(v.ptr(), i));
     if (PyErr_Occurred()) throw py::error_already_set();
     return x;
 }
+// six integers per matrix: A, lda, B, ldb, rows, columns
 std::vector<ClipMat> mats(const std::vector<i64>& v) {
+    if (v.size() % 6) throw std::invalid_argument("clip: six integers per matrix are wanted");
     std::vector<ClipMat> c;
     c.reserve(v.size() / 6);
     for (size_t i = 0; i < v.size(); i += 6) {
@@ -43,6 +43,63 @@ std::vector<ClipMat> mats(const std::vector<i64>& v) {
     return c;
 }
 int bytes_of(char t) { return t == 'd' ? 8 : t == 's' ? 4 : 2; }
+
+// A backward pass: dZ (and the bias gradient), then the products that read it.
+// v: rows, columns, act, dC, ldc, Z1, ldz1, Z2, ldz2, db, incb, bias_mode, how many
+// dZ are made; then 18 integers for each product: mode, op(A) and op(B) transposed,
+// m, n, k and address and leading dimension of A, A2, B, B2, C, C2, where the
+// addresses -1 and -2 are the dZ made here.  The workspace holds them, the bias
+// gradient's partial sums, and behind them what one product after the other wants.
+// -> its size; without one nothing is launched.
+template <typename T> i64 ffn_grad(double alpha, const std::vector<i64>& v, char* ws, hipStream_t s) {
+    constexpr size_t HEAD = 13, PER = 18;
+    if (v.size() < HEAD || (v.size() - HEAD) % PER) throw std::invalid_argument("ffn_grad: 13 + 18 n integers are wanted");
+    auto round = [](i64 x, i64 to) { return (x + to - 1) / to * to; };
+    ActGradArgs g;
+    g.m = v[0]; g.n = v[1]; g.act = (int)v[2];
+    g.dC = P((uintptr_t)v[3]); g.lddc = v[4];
+    g.Z1 = P((uintptr_t)v[5]); g.ldz1 = v[6];
+    g.Z2 = P((uintptr_t)v[7]); g.ldz2 = v[8];
+    g.db = W((uintptr_t)v[9]); g.incb = v[10]; g.bias_mode = (int)v[11];
+    const int ndz = (int)v[12];
+    g.lddz = round(std::max<i64>(g.m, 1), g.m >= 64 ? 64 : 8);
+    const i64 dz = round(g.lddz * g.n * (i64)sizeof(T), 256);
+    const i64 sums = g.bias_mode ? (i64)act_grad_chunks(g.bias_mode, sizeof(T), g.m, g.n) * (g.bias_mode == 1 ? g.m : g.n) *
+                                       (sizeof(T) == 8 ? 8 : 4) : 0;
+    const i64 rest = round(ndz * dz + sums, 256);
+    // (an address to plan with: as aligned as the workspace's)
+    char* base = ws ? ws : reinterpret_cast<char*>(4096);
+    if (ws && (ndz || g.bias_mode)) {
+        if (ndz > 0) g.dZ1 = base;
+        if (ndz > 1) g.dZ2 = base + dz;
+        g.part = base + ndz * dz;
+        act_grad<T>(g, s);
+    }
+    i64 most = 0;
+    for (size_t i = HEAD; i < v.size(); i += PER) {
+        const i64* x = &v[i];
+        GemmActArgs a;
+        a.alpha = alpha;
+        a.mode = (int)x[0];
+        a.m = x[3]; a.n = x[4]; a.k = x[5];
+        auto at = [&](int j, i64& ld) -> void* {
+            ld = x[j + 1];
+            if (x[j] >= 0 || x[j] < -2) return W((uintptr_t)x[j]);
+            ld = g.lddz;
+            return base + (x[j] == -2 ? dz : 0);
+        };
+        for (int j = 0; j < 2; ++j) {
+            a.A[j] = at(6 + 2 * j, a.lda[j]);
+            a.B[j] = at(10 + 2 * j, a.ldb[j]);
+            a.C[j] = W((uintptr_t)x[14 + 2 * j]);
+            a.ldc[j] = x[15 + 2 * j];
+        }
+        a.part = base + rest;
+        a.plan = !ws;
+        most = std::max(most, gemm_act<T>(a, x[1] ? 'T' : 'N', x[2] ? 'T' : 'N', s));
+    }
+    return rest + most;
+}
 
 }  // namespace
 
@@ -91,13 +148,19 @@ void register_ffn(py::module& m) {
         if (bias_mode && !ws) throw std::invalid_argument("act_grad: workspace missing");
         real_dispatch(dt, [&](auto z) { act_grad<decltype(z)>(a, S(st)); });
     });
+    m.def("ffn_grad", [](char dt, double alpha, const py::list& v, uintptr_t ws, uintptr_t st) {
+        const auto x = ints(v);
+        i64 bytes = 0;
+        real_dispatch(dt, [&](auto z) { bytes = ffn_grad<decltype(z)>(alpha, x, (char*)W(ws), S(st)); });
+        return bytes;
+    });
     m.def("clip_parts", [](i64 count) { return clip_parts(count); });
     // false, and nothing launched, where `look` is set and address ranges of the call overlap
     m.def("clip_norm", [](char ta, char tb, const py::list& v, double limit, uintptr_t part, uintptr_t norm, bool scale,
                           bool look, uintptr_t st) {
         const auto x = ints(v);
-        if (scale && look && !clip_apart(x.data(), x.size() / 6, bytes_of(ta), bytes_of(tb))) return false;
         const auto c = mats(x);
+        if (scale && look && !clip_apart(x.data(), x.size() / 6, bytes_of(ta), bytes_of(tb))) return false;
         const int n = clip_sum(ta, c.data(), (int)c.size(), (double*)W(part), S(st));
         clip_scale(ta, tb, c.data(), (int)c.size(), limit, (const double*)P(part), n, (double*)W(norm), scale, S(st));
         return true;

@@ -31,6 +31,7 @@ struct GemmActArgs {
     int splits = 1, per_split = 0;
     void* part = nullptr;   // splits > 1: partial sums, plane (split, i) of n columns of ldp
     i64 ldp = 0;
+    bool plan = false;      // only the workspace wanted is returned, nothing launched
 };
 
 // Which kernel, and in how many pieces K: from sizes, types and alignment alone.

@@ -123,7 +123,7 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
     const bool pack = ES == 2 && !dma && gemm_act_pack(a.mode, a.m, a.n, a.k) && ga_packed(op, nop, ES);
     const GemmActPlan p = gemm_act_plan(ES, a.mode, a.m, a.n, a.k, akc, bkc, dma || pack);
     if (p.tile < 0) {
-        ga_skinny<T>(a, gated, s);
+        if (!a.plan) ga_skinny<T>(a, gated, s);
         return 0;
     }
     const bool regs = !dma && !pack && !(ES >= 4 && small);
@@ -131,7 +131,7 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
         for (int i = 0; i < nop; ++i) op[i].bad = op[i].len < E;
     i64 bytes = (p.bytes + 255) / 256 * 256;
     if (pack || regs) bytes = ga_place(op, nop, ES, bytes);
-    if (bytes && !a.part) return bytes;
+    if (a.plan || (bytes && !a.part)) return bytes;
     if (pack || regs) ga_pack<T>(op, nop, static_cast<char*>(a.part), s);
     dma = dma || pack;
     a.lenA = op[0].at < 0 ? op[0].len : op[0].whole(ES);

@@ -513,6 +513,39 @@ def _act_grad(m, n, act, dC, Z1, Z2, dZ1, dZ2, db=_NONE, bias_mode=0, wide=False
                  db.ptr, _inc(db), bias_mode, wide, 0 if ws is None else ws.data_ptr(), raw_stream(t))
 
 
+class _Made:
+    """Stands for a dZ in the workspace of :func:`_grad_run`."""
+    __slots__ = ("ptr", "ld")
+
+    def __init__(self, ptr):
+        self.ptr, self.ld = ptr, 0
+
+
+_DZ1, _DZ2 = _Made(-1), _Made(-2)
+
+
+def _step(steps, mode, k, a, at, b, bt, c, a2=_NONE, b2=_NONE, c2=_NONE):
+    """Adds a product op(a) op(b) into c, of either orientation, to steps; at and
+    bt: does the operand enter transposed?"""
+    if c.t is None:
+        return
+    if ops._FLOPS is not None:
+        ops._FLOPS[0] += 2 * c.rows * c.cols * k * (1 if mode == PLAIN else 2)
+    if c.trans:
+        a, at, a2, b, bt, b2 = b, not bt, b2, a, not at, a2
+    steps += (mode, at, bt, c.rows, c.cols, k, a.ptr, a.ld, a2.ptr, a2.ld, b.ptr, b.ld, b2.ptr, b2.ld,
+              c.ptr, c.ld, c2.ptr, c2.ld)
+
+
+def _grad_run(alpha, oc, steps):
+    """One rank's backward pass on the device as two calls: its workspace, itself."""
+    t = oc.t
+    code, st, call = REAL_CODE[t.dtype], raw_stream(t), kmod(t).ffn_grad
+    nbytes = call(code, alpha, steps, 0, st)
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=t.device)
+    call(code, alpha, steps, ws.data_ptr(), st)
+
+
 def gemm_bias_act_grad(alpha, A, B, act, Z, dC, dA, dB, dbias, opts=None):
     """Gradients of :func:`gemm_bias_act` with respect to A, B and bias:
 
@@ -551,9 +584,23 @@ def gemm_bias_act_grad(alpha, A, B, act, Z, dC, dA, dB, dbias, opts=None):
             if a or mode:
                 oz = _NONE if not a else oz if oz.trans == oc.trans else _turn(oz, oc.trans)
                 if a and (dA is not None or dB is not None):
-                    dZ = _like(oc, oc.rows, oc.cols, oc.trans)
+                    dZ = None
                 if mode and oc.trans:
                     mode = 3 - mode
+            if oc.t.is_cuda and m and n:
+                made = dZ is None
+                if made:
+                    dZ = _DZ1
+                steps = [oc.rows, oc.cols, a, oc.ptr, oc.ld, oz.ptr, oz.ld, 0, 0, gv.ptr, _inc(gv), mode, made]
+                tr = oc.trans
+                _step(steps, PLAIN, n if alpha else 0, dZ, tr, ob, not ob.trans, ga)
+                _step(steps, PLAIN, m if alpha else 0, oa, not oa.trans, dZ, tr, gb)
+                _grad_run(alpha, oc, steps)
+                _modified(dA, dB, dbias)
+                return
+            if dZ is None:
+                dZ = _like(oc, oc.rows, oc.cols, oc.trans)
+            if a or mode:
                 _act_grad(oc.rows, oc.cols, a, oc, oz, _NONE, _NONE if dZ is oc else dZ, _NONE, gv, mode)
             if dA is not None:
                 _product(PLAIN, alpha, dZ, _NONE, ob.T, _NONE, ga, _NONE)
@@ -604,9 +651,25 @@ def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
         _outputs(what, pairs[6:], pairs[:6])
         with _on(oc.t):
             tr = oc.trans
+            if z1.trans != tr:
+                z1 = _turn(z1, tr)
+            if z2.trans != tr:
+                z2 = _turn(z2, tr)
+            if dB is not None and o2.trans != o1.trans:
+                o2 = _turn(o2, o1.trans)
+            if oc.t.is_cuda and m and n:
+                steps = [oc.rows, oc.cols, a, oc.ptr, oc.ld, z1.ptr, z1.ld, z2.ptr, z2.ld, 0, 1, 0, 2]
+                if dA1 is not None and dA2 is not None and g1.trans == g2.trans:
+                    _step(steps, PAIR, n, _DZ1, tr, ob, not ob.trans, g1, _DZ2, ob, g2)
+                else:
+                    _step(steps, PLAIN, n, _DZ1, tr, ob, not ob.trans, g1)
+                    _step(steps, PLAIN, n, _DZ2, tr, ob, not ob.trans, g2)
+                _step(steps, SUM, m, o1, not o1.trans, _DZ1, tr, gb, o2, _DZ2)
+                _grad_run(1.0, oc, steps)
+                _modified(dA1, dA2, dB)
+                return
             d1, d2 = _like(oc, oc.rows, oc.cols, tr), _like(oc, oc.rows, oc.cols, tr)
-            _act_grad(oc.rows, oc.cols, a, oc, z1 if z1.trans == tr else _turn(z1, tr),
-                      z2 if z2.trans == tr else _turn(z2, tr), d1, d2)
+            _act_grad(oc.rows, oc.cols, a, oc, z1, z2, d1, d2)
             if dA1 is not None and dA2 is not None and g1.trans == g2.trans:
                 _product(PAIR, 1.0, d1, d2, ob.T, ob.T, g1, g2)
             else:
@@ -614,8 +677,6 @@ def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
                     if g.t is not None:
                         _product(PLAIN, 1.0, d, _NONE, ob.T, _NONE, g, _NONE)
             if dB is not None:
-                if o2.trans != o1.trans:
-                    o2 = _turn(o2, o1.trans)
                 _product(SUM, 1.0, o1.T, o2.T, d1, d2, gb, _NONE)
         _modified(dA1, dA2, dB)
 
