@@ -532,6 +532,9 @@ __global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs
                 ga_to_lds<W>(xb + offB[i], slot + BM * 128 + min(wid + i * NW, PCB - 1) * (64 * W));
             xb += db;
         } else {
+            // it may take fewer DMA instructions than the counted wait allows for: the
+            // slabs before it have landed first
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             #pragma unroll
             for (int h = 0; h < NA; ++h)
                 IA::template stage<W, NW>(slabA(GATED ? h : curp, k0), a.lda[GATED ? h : curp], AKC ? a.k : a.m, rowsA,
@@ -695,7 +698,7 @@ __global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs
     } else {
         auto step = [&](int s, Held& next, Held& spare) __attribute__((always_inline)) {
             // my part of step s has landed (of the steps behind it, LOADS each are in
-            // flight; a step that went through registers waited for all before it) ...
+            // flight, or less where all before that one had landed) ...
             if constexpr (!DMA) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             else if (S > 2 && s + S - 2 < s1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * LOADS) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");

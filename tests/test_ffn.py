@@ -907,3 +907,18 @@ def test_wide_leading_dimension(dt, m, n, k):
         p.A = A
         p.check()
         del buf, A
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT", "TT"])
+def test_short_last_step(dt, ta, tb):
+    """K that ends early in its last step, of one product and of a sum of two; the same bits every time."""
+    for k in (72, 136, 200, 328, 520):
+        p = Product(dt, "cuda", 328, 264, k, ta, tb)
+        p.check()
+        first = p.C.clone()
+        for _ in range(8):
+            sl.gemm_bias_act(p.alpha, *p.handles()[:3], p.act, p.beta, *p.handles()[3:])
+            assert torch.equal(p.C, first)
+        Gated(dt, "cuda", k, 264, 328, ta, tb).check_grad(("B",))
