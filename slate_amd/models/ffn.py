@@ -54,7 +54,7 @@ class _Opd:
     address, leading dimension, stored and logical shape, whether it enters
     transposed, and the tensor that owns it."""
 
-    __slots__ = ("ptr", "end", "ld", "rows", "cols", "m", "n", "trans", "t", "dt", "dev", "buf")
+    __slots__ = ("ptr", "end", "ld", "rows", "cols", "m", "n", "trans", "t", "dt", "dev", "version")
 
     def __init__(self, ptr, ld, rows, cols, trans, t):
         self.dt, self.dev = (None, None) if t is None else (t.dtype, _DEVICES.setdefault(t.device, t.device))
@@ -86,13 +86,13 @@ def _of_tensor(t, rows, cols, trans=False, name="matrix"):
 
 def _opd(M, name="matrix"):
     """The (one) rank's operand of a view.  A view remembers it, and uses it again
-    while its storage has the same buffer at the same place, whole."""
+    while no state of its storage's tiles has changed (new buffers and writes on
+    the other side do) and its buffer is at the same place."""
     s = M.storage
-    slot = s.origin_slot
     x = M.__dict__.get("_operand")
-    if x is not None and s.local.get(slot) is x.buf and s._valid.get(slot) == s.table.version() \
-            and x.trans == (M._op is not Op.NoTrans) and x.t.data_ptr() == x.ptr:
+    if x is not None and x.version == s.table.version() and x.t.data_ptr() == x.ptr:
         return x
+    slot = s.origin_slot
     if M._mt == s.mt and M._nt == s.nt and not (M.row0_offset or M.col0_offset) and M.last_mb is None \
             and M.last_nb is None and slot is not None:
         t, rows, cols = s.prepare_local(slot), s.bc.mloc, s.bc.nloc
@@ -100,7 +100,7 @@ def _opd(M, name="matrix"):
         t = M.local_block().data
         rows, cols = t.shape
     x = _of_tensor(t, rows, cols, M._op is not Op.NoTrans, name)
-    x.buf = s.local.get(slot)
+    x.version = s.table.version() if s._valid.get(slot) == s.table.version() else -1
     M.__dict__["_operand"] = x
     return x
 
@@ -741,8 +741,7 @@ def _clip_views(mats, what):
         x = M.__dict__.get("_operand")
         # (a remembered operand was looked at before; its use, as in _opd, without the call)
         now = s.table.version()
-        if x is None or s.local.get(slot) is not x.buf or s._valid.get(slot) != now \
-                or x.trans != (M._op is not Op.NoTrans) or x.t.data_ptr() != x.ptr:
+        if x is None or x.version != now or x.t.data_ptr() != x.ptr:
             if M._kind != "general" or s.bc is None:
                 raise SlateError(f"{what}: general block-cyclic matrices are wanted")
             if slot is None:
