@@ -24,7 +24,7 @@
 // k order, so one, four or two MFMAs multiply it.
 //
 // Large products are bound by the MFMAs: bf16 8192 columns, 4096 -> 16384,
-// gelu_tanh with Z stored 935 us (1176 TFLOP/s), gated 4096 -> 8192 893 us (1231),
+// gelu_tanh with Z stored 920 us (1195 TFLOP/s), gated 4096 -> 8192 877 us (1254),
 // f32 4096^3 990 us (139), f64 2010 us (68).  Few columns are bound by reading
 // op(A): f16 33 columns, 8192 -> 2048 9.5 us and 3.5 us to join 16 pieces of K.
 #pragma once
@@ -185,8 +185,10 @@ template <bool FAST, int V, typename R> __device__ inline void ga_act_grad(int a
     }
 }
 
-// V rows of column n: the epilogue on finished sums
-template <typename T, int V, bool GATED>
+// V rows of column n: the epilogue on finished sums.  PAST: outputs past the
+// caches, which keep the operands instead (256 x 256 tiles: 916 us against 938 for
+// 8192 columns, 4096 -> 16384 with Z; smaller outputs are often read next).
+template <typename T, int V, bool GATED, bool PAST = false>
 __device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, const typename ga_traits<T>::acc* s1,
                                  const typename ga_traits<T>::acc* s2) {
     using R = typename ga_traits<T>::acc;
@@ -241,7 +243,8 @@ __device__ inline void ga_finish(const GemmActArgs& a, int pair, i64 m, i64 n, c
             vT x;
             #pragma unroll
             for (int r = 0; r < V; ++r) x[r] = (T)v[r];
-            *reinterpret_cast<vT*>(p) = x;
+            if constexpr (PAST) __builtin_nontemporal_store(x, reinterpret_cast<vT*>(p));
+            else *reinterpret_cast<vT*>(p) = x;
         } else {
             #pragma unroll
             for (int r = 0; r < V; ++r) if (r < left) p[r] = (T)v[r];
@@ -788,7 +791,7 @@ __global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs
                 x[r] = img[cc * LDR + rr + r];
                 if constexpr (GATED) y[r] = img[cc * LDR + WH + rr + r];
             }
-            ga_finish<T, V, GATED>(a, pair, mw + rr, nw + pass * (16 * NJ) + cc, x, y);
+            ga_finish<T, V, GATED, BM == 256>(a, pair, mw + rr, nw + pass * (16 * NJ) + cc, x, y);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
