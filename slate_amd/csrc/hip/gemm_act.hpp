@@ -265,6 +265,13 @@ template <int W> __device__ inline void ga_to_lds(const void* p, void* q) {
 }
 
 // ------------------------------------------------------------- LDS images
+// 16 bytes moved down by `down` bits, zeros behind them
+__device__ inline i4v ga_shift(i4v w, int down) {
+    typedef unsigned __int128 u128;
+    const u128 x = __builtin_bit_cast(u128, w) >> (down & 127);
+    return __builtin_bit_cast(i4v, down < 128 ? x : (u128)0);
+}
+
 template <typename T, int R, bool KC> struct GaImg {
     static constexpr int ES = sizeof(T), E = 16 / ES, KB = 128 / ES;
     static constexpr int BYTES = R * 128;
@@ -369,11 +376,6 @@ template <typename T, int R, bool KC> struct GaImg {
         down = over < E && !below ? (int)over * ES * 8 : 128;
         return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(x - over));
     }
-    __device__ static inline i4v shift(i4v w, int down) {
-        typedef unsigned __int128 u128;
-        const u128 x = __builtin_bit_cast(u128, w) >> (down & 127);
-        return __builtin_bit_cast(i4v, down < 128 ? x : (u128)0);
-    }
     // The same for slabs that all go through registers: what a slot's addresses
     // need, made once, and a load without a branch (the loads of two slabs are in
     // flight, and a load behind a branch would be waited for at once).  avail: the
@@ -417,7 +419,7 @@ template <typename T, int R, bool KC> struct GaImg {
                 else if (k < kleft && (KC || r < rows)) {
                     int down;
                     const i4v w = fetch(X, off, q, ld, len, rows, kleft, false, down);
-                    *reinterpret_cast<i4v*>(img + q * 16) = shift(w, down);
+                    *reinterpret_cast<i4v*>(img + q * 16) = ga_shift(w, down);
                 } else *reinterpret_cast<i4v*>(img + q * 16) = i4v{0, 0, 0, 0};
             }
         } else {
@@ -431,7 +433,7 @@ template <typename T, int R, bool KC> struct GaImg {
             }
             #pragma unroll
             for (int i = 0; i < C; ++i)
-                *reinterpret_cast<i4v*>(img + (min(wid + i * NW, N - 1) * 64 + lane) * 16) = shift(w[i], down[i]);
+                *reinterpret_cast<i4v*>(img + (min(wid + i * NW, N - 1) * 64 + lane) * 16) = ga_shift(w[i], down[i]);
         }
     }
 };
@@ -608,11 +610,11 @@ __global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs
                 #pragma unroll
                 for (int i = 0; i < CA; ++i)
                     *reinterpret_cast<i4v*>(slot + h * IA::BYTES + min(tid + i * NT, QA - 1) * 16) =
-                        whole ? x.a[h][i] : IA::shift(x.a[h][i], x.sa[h][i]);
+                        whole ? x.a[h][i] : ga_shift(x.a[h][i], x.sa[h][i]);
             #pragma unroll
             for (int i = 0; i < CB; ++i)
                 *reinterpret_cast<i4v*>(slot + BM * 128 + min(tid + i * NT, QB - 1) * 16) =
-                    whole ? x.b[i] : IB::shift(x.b[i], x.sb[i]);
+                    whole ? x.b[i] : ga_shift(x.b[i], x.sb[i]);
         };
         if (x.whole) put(std::true_type());
         else put(std::false_type());
@@ -803,14 +805,15 @@ __global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs
 // interleaved slabs of 128 bytes per row, fragments straight from memory to
 // registers with 2 U of them in flight per wave and operand (no LDS, no
 // barrier in the loop); the waves' sums are added in LDS in their order.
-// One column: 4096 x 4096 bf16 9.3 us (3.6 TB/s), two f16 matrices of 8192 x
-// 4096 30 us (4.4 TB/s).
+// One column: 4096 x 4096 bf16 8.6 us (3.9 TB/s), two f16 matrices of 8192 x
+// 4096 29 us (4.6 TB/s).  Columns that lie across 16 bytes cost 2.5 times as
+// much (bf16 5120 x 11772: 138 us, 44 aligned).
 template <typename T, bool GATED, int NW>
 __global__ void __launch_bounds__(64 * NW) gemm_act_skinny_kernel(GemmActArgs a) {
     using TR = ga_traits<T>;
     using acc4 = typename TR::acc4;
     using R = typename TR::acc;
-    constexpr int NA = GATED ? 2 : 1, E = 16 / (int)sizeof(T), KB = 8 * E, U = GATED ? 2 : 4, LD = 16 + 16 / (int)sizeof(R);
+    constexpr int NA = GATED ? 2 : 1, E = 16 / (int)sizeof(T), KB = 8 * E, U = 4, LD = 16 + 16 / (int)sizeof(R);
     __shared__ __align__(16) R red[NW][NA][16 * LD];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
     const i64 m0 = (i64)xcd_remap(blockIdx.x, gridDim.x) * 16;
@@ -834,39 +837,56 @@ __global__ void __launch_bounds__(64 * NW) gemm_act_skinny_kernel(GemmActArgs a)
             }
     };
     const int slabs = (int)(a.k / KB);
-    int s = w;
-    for (; s + (U - 1) * NW < slabs; s += U * NW) {
-        i4v fa[2 * U][NA], fb[2 * U];
-        #pragma unroll
-        for (int u = 0; u < 2 * U; ++u) {
-            const i64 k = (i64)(s + (u >> 1) * NW) * KB + (u & 1) * (4 * E);
-            #pragma unroll
-            for (int h = 0; h < NA; ++h)
-                fa[u][h] = __builtin_bit_cast(i4v, __builtin_nontemporal_load(reinterpret_cast<const ga_vec<T, E>*>(pa[h] + k)));
-            fb[u] = __builtin_bit_cast(i4v, *reinterpret_cast<const ga_vec<T, E>*>(pb + k));
-        }
-        #pragma unroll
-        for (int u = 0; u < 2 * U; ++u) mul(fa[u], fb[u]);
-    }
-    for (; s * KB < a.k; s += NW) {
+    using vE = ga_vec<T, E>;
+    auto get = [](const T* p) { return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(p)); };
+    // the ragged end of K: its loads come first, its products last
+    const bool rag = a.k % KB != 0 && slabs % NW == w;
+    i4v ra[2][NA], rb[2];
+    int down[2] = {0, 0};
+    if (rag)
         #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            const i64 k = (i64)s * KB + kk * (4 * E);
-            const int left = (int)min((i64)E, a.k - k - g * E);
-            i4v fa[NA];
-            auto get = [&](const T* p) {
-                using vE = ga_vec<T, E>;
+            const i64 k = (i64)slabs * KB + kk * (4 * E), end = a.k - E - g * E;
+            const int left = (int)max((i64)0, min((i64)E, a.k - k - g * E));
+            auto last = [&](const T* p) {
+                if (a.k >= E) return get(p + min(k, end));       // a column's last 16 bytes, to be shifted down
                 vE x;
-                if (left == E) return __builtin_bit_cast(i4v, *reinterpret_cast<const vE*>(p + k));
                 #pragma unroll
                 for (int e = 0; e < E; ++e) x[e] = e < left ? p[k + e] : (T)0;
                 return __builtin_bit_cast(i4v, x);
             };
+            if (a.k >= E) down[kk] = left ? (E - left) * (int)sizeof(T) * 8 : 128;
             #pragma unroll
-            for (int h = 0; h < NA; ++h) fa[h] = get(pa[h]);
-            mul(fa, get(pb));
+            for (int h = 0; h < NA; ++h) ra[kk][h] = last(pa[h]);
+            rb[kk] = last(pb);
         }
-    }
+    // (slabs that do not exist end the loads: guarded one by one, each guard waits
+    // for the loads before it, 5120 x 5888 f32 times one column 55 us against 33)
+    auto batch = [&](int s, auto whole) __attribute__((always_inline)) {
+        i4v fa[2 * U][NA], fb[2 * U];
+        #pragma unroll
+        for (int u = 0; u < 2 * U; ++u) {
+            if (!whole && s + (u >> 1) * NW >= slabs) break;
+            const i64 k = (i64)(s + (u >> 1) * NW) * KB + (u & 1) * (4 * E);
+            #pragma unroll
+            for (int h = 0; h < NA; ++h) fa[u][h] = get(pa[h] + k);
+            fb[u] = get(pb + k);
+        }
+        __builtin_amdgcn_sched_barrier(0);                       // all of them in flight
+        #pragma unroll
+        for (int u = 0; u < 2 * U; ++u)
+            if (whole || s + (u >> 1) * NW < slabs) mul(fa[u], fb[u]);
+    };
+    int s = w;
+    for (; s + (U - 1) * NW < slabs; s += U * NW) batch(s, std::true_type());
+    for (; s < slabs; s += U * NW) batch(s, std::false_type());
+    if (rag)
+        #pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            #pragma unroll
+            for (int h = 0; h < NA; ++h) ra[kk][h] = ga_shift(ra[kk][h], down[kk]);
+            mul(ra[kk], ga_shift(rb[kk], down[kk]));
+        }
     #pragma unroll
     for (int h = 0; h < NA; ++h)
         #pragma unroll

@@ -27,6 +27,8 @@ void ga_tile(const GemmActArgs& a, int tile, hipStream_t s) {
         if (tile == 1) return ga_launch<T, AKC, BKC, 128, 128, 2, 2, 2, GATED, DMA>(a, s);
     if constexpr (sizeof(T) == 2 && DMA == 16)
         if (tile == 4) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 3, GATED, DMA>(a, s);
+    if constexpr (sizeof(T) >= 4)
+        if (tile == 5) return ga_launch<T, AKC, BKC, 64, 32, 2, 2, 2, GATED, DMA>(a, s);
     if (tile == 2) return ga_launch<T, AKC, BKC, 64, 64, 2, 2, 2, GATED, DMA>(a, s);
     return ga_launch<T, AKC, BKC, 128, 16, 4, 1, 2, GATED, DMA>(a, s);
 }

@@ -15,7 +15,7 @@ bool gemm_act_pack(int mode, i64 m, i64 n, i64 k) {
 
 namespace {
 
-// Microseconds that a square tile takes, by how many of its workgroups a CU
+// Microseconds that a tile takes, by how many of its workgroups a CU
 // holds at once (256 CUs): per step of K (128 bytes), and for its start and
 // epilogue; measured on outputs of 256 to 8192 rows and columns, K of 256 to
 // 11456.  A larger tile reads less per flop, a smaller one fills the CUs and
@@ -26,18 +26,23 @@ namespace {
 // CU holds four workgroups of the one, three of the other).  32- and 64-bit
 // products wait for the MFMAs, not for what a larger tile would save: 64 x 64
 // f32 134 us at 2000^3 (128 x 128: 142 in two pieces), 989 at 4096^3 (966), f64
-// 256 (275) and 2020 (1943).  (1024 x 4096 x 1024 of 16-bit operands that go
-// through registers: 31 us, 2048 x 4096 x 512 33; with 128 x 128 tiles 39.)
+// 256 (275) and 2020 (1943); 64 x 32 where columns are few or tiles do not fill
+// the CUs: f32 32 x 4096 x 4096 20 us (64 x 64: 27), 130 x 1000 x 3000 20 (23),
+// 1024^3 26 (30), f64 32 x 4096 x 4096 38 (50); 2000^3 276 (257), f32 440 x 5716 x
+// 6329 297 (274).  16-bit operands that go through registers: 1024 x 4096 x 1024
+// 31 us, 2048 x 4096 x 512 33 (128 x 128: 39).
 enum { HALF_DMA, HALF_REGS, SINGLE, DOUBLE };
-struct GaCost { int kind, tile, size, per_cu; double step[4], ends[4]; };
+struct GaCost { int kind, tile, rows, cols, per_cu; double step[6], ends[6]; };
 const GaCost ga_costs[] = {
-    {HALF_DMA, 0, 256, 1, {1.72}, {11}},
-    {HALF_DMA, 1, 128, 2, {0.70, 0.95}, {4, 7}},
-    {HALF_DMA, 2, 64, 4, {0.515, 0.54, 0.60, 0.68}, {1, 2, 3, 3}},
-    {HALF_DMA, 4, 64, 3, {0.36, 0.45, 0.60}, {1, 2, 3}},
-    {HALF_REGS, 2, 64, 4, {0.55, 0.78, 1.10, 1.50}, {1, 2, 3, 3}},
-    {SINGLE, 2, 64, 4, {0.72, 1.10, 1.60, 2.10}, {1, 2, 3, 3}},
-    {DOUBLE, 2, 64, 4, {0.72, 1.15, 1.55, 2.05}, {1, 2, 3, 3}},
+    {HALF_DMA, 0, 256, 256, 1, {1.72}, {11}},
+    {HALF_DMA, 1, 128, 128, 2, {0.70, 0.95}, {4, 7}},
+    {HALF_DMA, 2, 64, 64, 4, {0.515, 0.54, 0.60, 0.68}, {1, 2, 3, 3}},
+    {HALF_DMA, 4, 64, 64, 3, {0.36, 0.45, 0.60}, {1, 2, 3}},
+    {HALF_REGS, 2, 64, 64, 4, {0.55, 0.78, 1.10, 1.50}, {1, 2, 3, 3}},
+    {SINGLE, 2, 64, 64, 4, {0.72, 1.10, 1.50, 2.00}, {1, 2, 3, 3}},
+    {SINGLE, 5, 64, 32, 6, {0.50, 0.61, 0.88, 1.09, 1.45, 1.75}, {1, 2, 3, 3, 3, 3}},
+    {DOUBLE, 2, 64, 64, 4, {0.72, 1.15, 1.50, 2.00}, {1, 2, 3, 3}},
+    {DOUBLE, 5, 64, 32, 6, {0.60, 0.68, 0.90, 1.12, 1.45, 1.75}, {1, 2, 3, 3, 3, 3}},
 };
 double ga_time(const GaCost& c, i64 wgs, int steps) {
     const i64 full = wgs / (256 * c.per_cu), rest = wgs - full * 256 * c.per_cu;
@@ -76,7 +81,7 @@ GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool 
         double best = 0;
         for (const GaCost& c : ga_costs) {
             if (c.kind != kind) continue;
-            const i64 t = tiles(c.size, c.size);
+            const i64 t = tiles(c.rows, c.cols);
             for (int want = 1; want == 1 || (want <= steps / 4 && t * want <= 1024); ++want) {
                 const int per = (steps + want - 1) / want, sp = (steps + per - 1) / per;
                 if (sp != want) continue;
