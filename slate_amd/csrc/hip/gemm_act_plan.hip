@@ -61,10 +61,16 @@ double ga_time(const GaCost& c, i64 wgs, int steps) {
 GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool bkc, bool dma) {
     GemmActPlan p;
     // Up to 16 columns and both operands along k: 4096 x 4096 bf16 times one
-    // column 9.2 us against 14.9 us of the tiles with K split (16 columns of
-    // 8192 x 2048: 12.0 against 14.6; 33 of 2048 x 8192 would be 29.6 against
-    // 19.0).  Below 1024 rows it fills too few CUs.
-    if (mode <= GA_GATED && akc && bkc && n <= 16 && m >= 1024) {
+    // column 8.6 us against 14.9 us of the tiles with K split (16 columns of
+    // 8192 x 2048: 10.6 against 14.6; 33 of 2048 x 8192 would be 29.6 against
+    // 19.0).  Below 1024 rows it fills too few CUs; and a CU with two of its
+    // workgroups takes twice as long, so that where many have one less than
+    // others, rows are long and columns more than a few, K is split instead (15
+    // columns: f32 5120 x 5888 32 us against 45, 4096 x 5888 28 against 27; one
+    // column: bf16 5120 x 5888 19 against 18).
+    const i64 groups = (m + 15) / 16, turns = (groups + 255) / 256 * 256;
+    const bool uneven = groups > 256 && 10 * turns >= 13 * groups && n > 8 && k * es >= 8192;
+    if (mode <= GA_GATED && akc && bkc && n <= 16 && m >= 1024 && !uneven) {
         p.tile = -1;
         return p;
     }
