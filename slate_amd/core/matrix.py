@@ -83,6 +83,7 @@ class BaseMatrix:
     """Shared-storage view (SLATE BaseMatrix)."""
 
     _kind = "general"
+    _whole = True           # every element of the m x n range is the matrix's own (no triangle, no band)
 
     def __init__(self, storage: MatrixStorage, ioffset=0, joffset=0, mt=None, nt=None,
                  row0_offset=0, col0_offset=0, last_mb=None, last_nb=None,
@@ -98,9 +99,14 @@ class BaseMatrix:
         self._diag = Diag(diag)
 
     # ---------------------------------------------------------------- copy
+    def _become(self, matrix):
+        """Take over another matrix's view (the converting constructors)."""
+        self.__dict__.update(matrix.__dict__)
+        self.__dict__.pop("_operand", None)     # what models/ffn.py remembers of a view
+
     def _clone(self, cls=None, **kw):
         new = _copy.copy(self)
-        new.__dict__.pop("_operand", None)      # what models/ffn.py remembers of a view
+        new.__dict__.pop("_operand", None)
         if cls is not None:
             new.__class__ = cls
         for k, v in kw.items():
@@ -605,6 +611,7 @@ def _as_colmajor(A, m, n, ld):
 
 class BaseTrapezoidMatrix(BaseMatrix):
     _kind = "trapezoid"
+    _whole = False
 
     def _in_shape(self, i, j):
         gi, gj = self._global_ij(i, j)
@@ -621,7 +628,7 @@ class TrapezoidMatrix(BaseTrapezoidMatrix):
     def __init__(self, uplo=Uplo.Lower, m=0, n=0, nb=256, p=None, q=None, comm=None, dtype=torch.float64,
                  device=None, diag=Diag.NonUnit, _storage=None, matrix: Optional[BaseMatrix] = None, **kw):
         if matrix is not None:
-            self.__dict__.update(matrix.__dict__)
+            self._become(matrix)
             self._uplo, self._diag = Uplo(uplo), Diag(diag)
             return
         if _storage is None:
@@ -677,7 +684,7 @@ class _SquareSym(BaseTrapezoidMatrix):
         if isinstance(n, BaseMatrix):
             matrix, n = n, 0
         if matrix is not None:
-            self.__dict__.update(matrix.__dict__)
+            self._become(matrix)
             self._uplo = Uplo(uplo)
             self._diag = Diag.NonUnit
             return
@@ -725,6 +732,8 @@ class BaseBandMatrix(BaseMatrix):
     band matrices, the kl extra upper tile diagonals of the LU fill-in) are
     allocated, as per-column slabs (core/band_storage.py)."""
 
+    _whole = False
+
     def __init__(self, storage, kl, ku, **kw):
         super().__init__(storage, **kw)
         self._kl, self._ku = kl, ku
@@ -754,7 +763,7 @@ class BandMatrix(BaseBandMatrix):
     def __init__(self, m=0, n=0, kl=0, ku=0, nb=256, p=None, q=None, comm=None, dtype=torch.float64,
                  device=None, _storage=None, matrix=None, **kw):
         if matrix is not None:
-            self.__dict__.update(matrix.__dict__)
+            self._become(matrix)
             self._kl, self._ku = kl, ku
             return
         if _storage is None:
@@ -781,7 +790,7 @@ class TriangularBandMatrix(BaseTriangularBandMatrix):
     def __init__(self, uplo=Uplo.Lower, diag=Diag.NonUnit, n=0, kd=0, nb=256, p=None, q=None, comm=None,
                  dtype=torch.float64, device=None, _storage=None, matrix=None, **kw):
         if matrix is not None:
-            self.__dict__.update(matrix.__dict__)
+            self._become(matrix)
             self._uplo, self._diag, self._kd = Uplo(uplo), Diag(diag), kd
             self._kl, self._ku = (kd, 0) if self._uplo == Uplo.Lower else (0, kd)
             return
@@ -797,7 +806,7 @@ class HermitianBandMatrix(BaseTriangularBandMatrix):
     def __init__(self, uplo=Uplo.Lower, n=0, kd=0, nb=256, p=None, q=None, comm=None, dtype=torch.float64,
                  device=None, _storage=None, matrix=None, **kw):
         if matrix is not None:
-            self.__dict__.update(matrix.__dict__)
+            self._become(matrix)
             self._uplo, self._kd = Uplo(uplo), kd
             self._kl, self._ku = (kd, 0) if self._uplo == Uplo.Lower else (0, kd)
             return

@@ -104,11 +104,11 @@ def run_on_block_cyclic(A, fn, opts, *others):
     s = A.storage
     nb = max(s.tileMb(0) if s.mt else 1, 1)
     B = type(A).__new__(type(A))
-    B.__dict__.update(A.__dict__)
+    B._become(A)
     twin = Matrix(A.m(), A.n(), nb=nb, comm=s.comm, dtype=s.dtype, device=s.device)
     twin.insertLocalTiles(device=s.device if s.device.type == "cuda" else -1)
     redistribute(A, twin)
-    B.__dict__.update(twin.__dict__)
+    B._become(twin)
     B._uplo, B._diag = A._uplo, A._diag
     r = fn(B, opts, *others)
     redistribute(twin, A)

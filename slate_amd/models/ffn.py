@@ -52,9 +52,10 @@ _DEVICES = {}          # one object per device, so that operands compare them by
 class _Opd:
     """One rank's strided column-major operand: first and one past the last
     address, leading dimension, stored and logical shape, whether it enters
-    transposed, and the tensor that owns it."""
+    transposed, and the tensor that owns it.  That of a view: the tile table of
+    its storage and the version at which it was whole."""
 
-    __slots__ = ("ptr", "end", "ld", "rows", "cols", "m", "n", "trans", "t", "dt", "dev", "version")
+    __slots__ = ("ptr", "end", "ld", "rows", "cols", "m", "n", "trans", "t", "dt", "dev", "table", "version")
 
     def __init__(self, ptr, ld, rows, cols, trans, t):
         self.dt, self.dev = (None, None) if t is None else (t.dtype, _DEVICES.setdefault(t.device, t.device))
@@ -86,11 +87,11 @@ def _of_tensor(t, rows, cols, trans=False, name="matrix"):
 
 def _opd(M, name="matrix"):
     """The (one) rank's operand of a view.  A view remembers it, and uses it again
-    while no state of its storage's tiles has changed (new buffers and writes on
-    the other side do) and its buffer is at the same place."""
+    while it has the same storage, no state of whose tiles has changed (new buffers
+    and writes on the other side do), and its buffer is at the same place."""
     s = M.storage
     x = M.__dict__.get("_operand")
-    if x is not None and x.version == s.table.version() and x.t.data_ptr() == x.ptr:
+    if x is not None and x.table is s.table and x.version == s.table.version() and x.t.data_ptr() == x.ptr:
         return x
     slot = s.origin_slot
     if M._mt == s.mt and M._nt == s.nt and not (M.row0_offset or M.col0_offset) and M.last_mb is None \
@@ -100,6 +101,7 @@ def _opd(M, name="matrix"):
         t = M.local_block().data
         rows, cols = t.shape
     x = _of_tensor(t, rows, cols, M._op is not Op.NoTrans, name)
+    x.table = s.table
     x.version = s.table.version() if s._valid.get(slot) == s.table.version() else -1
     M.__dict__["_operand"] = x
     return x
@@ -114,7 +116,7 @@ def _operands(what, names, mats):
             out.append(_NONE)
             continue
         s = M.storage
-        if M._kind != "general" or s.bc is None:
+        if not M._whole or s.bc is None:
             raise SlateError(f"{what}: {name} must be a general block-cyclic matrix")
         if s.origin_slot is None:
             raise SlateError(f"{what}: {name} has no tiles (insertLocalTiles)")
@@ -209,7 +211,7 @@ def _check(mats, shapes, what):
         if M is None:
             continue
         s = M.storage
-        if getattr(M, "_kind", "general") != "general" or s.bc is None:
+        if not M._whole or s.bc is None:
             raise SlateError(f"{what}: {name} must be a general block-cyclic matrix")
         if first is None:
             first = s
@@ -738,12 +740,12 @@ def _clip_views(mats, what):
     for M in mats:
         s = M.storage
         slot = s.origin_slot
+        if not M._whole or s.bc is None:
+            raise SlateError(f"{what}: general block-cyclic matrices are wanted")
         x = M.__dict__.get("_operand")
-        # (a remembered operand was looked at before; its use, as in _opd, without the call)
+        # (the use of a remembered operand, as in _opd, without the call)
         now = s.table.version()
-        if x is None or x.version != now or x.t.data_ptr() != x.ptr:
-            if M._kind != "general" or s.bc is None:
-                raise SlateError(f"{what}: general block-cyclic matrices are wanted")
+        if x is None or x.table is not s.table or x.version != now or x.t.data_ptr() != x.ptr:
             if slot is None:
                 raise SlateError(f"{what}: a matrix has no tiles (insertLocalTiles)")
             x = _opd(M)

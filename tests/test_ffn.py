@@ -922,3 +922,48 @@ def test_short_last_step(dt, ta, tb):
             sl.gemm_bias_act(p.alpha, *p.handles()[:3], p.act, p.beta, *p.handles()[3:])
             assert torch.equal(p.C, first)
         Gated(dt, "cuda", k, 264, 328, ta, tb).check_grad(("B",))
+
+
+def other_kinds(A):
+    """Views of a square general matrix whose elements are not all its own."""
+    up = sl.Uplo.Upper
+    return [sl.HermitianMatrix(sl.Uplo.Lower, A), sl.SymmetricMatrix(up, A), sl.TrapezoidMatrix(up, matrix=A),
+            sl.TriangularMatrix(sl.Uplo.Lower, sl.Diag.NonUnit, A), sl.BandMatrix(kl=1, ku=2, matrix=A),
+            sl.TriangularBandMatrix(sl.Uplo.Lower, kd=2, matrix=A), sl.HermitianBandMatrix(sl.Uplo.Lower, kd=2, matrix=A)]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_other_kinds_refused(dev):
+    """Hermitian, triangular and band views are refused whether or not the
+    matrix they were made of has been an operand before."""
+    x = cm(8, 8, torch.float32, 1, dev)
+    was = x.clone()
+    for used in (False, True):
+        A = mat(x, nb=4)
+        if used:
+            sl.global_norm([A])
+        for H in other_kinds(A):
+            for call in (lambda: sl.global_norm([H]), lambda: sl.clip_norm(1e-3, [H]), lambda: sl.clip_norm(1e-3, [A], [H]),
+                         lambda: sl.gemm_bias_act(1.0, H, A, None, "relu", 0.0, None, mat(cm(8, 8, torch.float32, 2, dev))),
+                         lambda: sl.gemm_gated(H, A, mat(x), "relu", mat(cm(8, 8, torch.float32, 2, dev)))):
+                with pytest.raises(SlateError):
+                    call()
+            with pytest.raises(SlateError):
+                sl.global_norm([H])                          # and the second time
+    assert torch.equal(x, was)
+
+
+def test_operand_of_another_storage():
+    """A view that is given another storage has that one's operand."""
+    x, y = (cm(8, 8, torch.float32, i, "cpu") for i in (1, 2))
+    A, B = mat(x), mat(y)
+    sl.global_norm([A])
+    A.storage = B.storage
+    assert abs(sl.global_norm([A]) - float(y.double().norm())) <= 1e-12 * 8
+    C = mat(cm(8, 8, torch.float32, 3, "cpu"))
+    A, B = mat(x), mat(y)
+    sl.gemm_bias_act(1.0, A, A, None, "identity", 0.0, None, C)
+    A.storage = B.storage
+    sl.gemm_bias_act(1.0, A, A, None, "identity", 0.0, None, C)
+    y64 = y.double()
+    within(C.to_dense(), y64 @ y64, 2.0 ** -24 * (12 * (y64.abs() @ y64.abs()) + (y64 @ y64).abs()))
