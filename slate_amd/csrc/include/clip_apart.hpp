@@ -1,6 +1,6 @@
 // Do the address ranges of the matrices of a clipping call lie apart?  Six
 // integers per matrix: A, lda, B, ldb, rows, columns; ea and eb bytes per
-// element.  A matrix that is scaled in place counts once.
+// element.  A matrix that is scaled in place (same memory, same type) counts once.
 #pragma once
 #include <algorithm>
 #include <cstdint>
@@ -17,7 +17,7 @@ inline bool clip_apart(const int64_t* v, size_t count, int ea, int eb) {
     for (size_t i = 0; i < count; ++i, v += 6) {
         if (v[4] <= 0 || v[5] <= 0) continue;
         add(v[2], v[3], v[4], v[5], eb);
-        if (v[0] != v[2] || v[1] != v[3]) add(v[0], v[1], v[4], v[5], ea);
+        if (v[0] != v[2] || v[1] != v[3] || ea != eb) add(v[0], v[1], v[4], v[5], ea);
     }
     // disjoint intervals: each ends before the next begins
     std::sort(lo.begin(), lo.end());

@@ -967,3 +967,25 @@ def test_operand_of_another_storage():
     sl.gemm_bias_act(1.0, A, A, None, "identity", 0.0, None, C)
     y64 = y.double()
     within(C.to_dense(), y64 @ y64, 2.0 ** -24 * (12 * (y64.abs() @ y64.abs()) + (y64 @ y64).abs()))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", HALF)
+def test_clip_types_share_memory(dev, dt):
+    """16-bit matrices and float32 ones over the same memory: not 'in place', whatever their leading dimensions."""
+    buf = torch.zeros(64, dtype=torch.float32, device=dev)
+    half = buf.view(dt)
+    x = half[:32].view(4, 8).t()                             # 8 x 4, at the front of the buffer
+    x.copy_(torch.arange(1, 33, device=dev).view(4, 8).t())
+    was = buf.clone()
+    for y in (buf[:32].view(4, 8).t(), buf.as_strided((8, 4), (1, 16)), buf[8:40].view(4, 8).t()):
+        for limit in (1e9, 1.0):
+            with pytest.raises(SlateError, match="overlap"):
+                sl.clip_norm(limit, [mat(x)], [mat(y)])
+    a, b = half[:8][:, None], buf[:8][:, None]               # one column each
+    with pytest.raises(SlateError, match="overlap"):
+        sl.clip_norm(1.0, [mat(a)], [mat(b)])
+    assert torch.equal(buf, was)
+    y = buf[32:].view(4, 8).t()
+    sl.clip_norm(1e9, [mat(x)], [mat(y)])
+    assert torch.equal(y, x.float())
