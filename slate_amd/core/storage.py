@@ -113,6 +113,7 @@ class MatrixStorage:
         self.tiles = {}            # (i, j, slot) -> 2-D tensor (col-major view)
         self.local = {}            # slot -> contiguous local buffer (block-cyclic case)
         self.origin_slot = None
+        self.wraps = False         # is a local buffer the caller's own?
         self.lock = threading.RLock()
         self._valid = {}           # slot -> table version at which prepare_local found it whole
         self._marked = None        # (slot, table version) after the last mark_local_modified
@@ -197,6 +198,7 @@ class MatrixStorage:
                 buf = torch.zeros((bc.nloc, bc.lld), dtype=self.dtype, device=dev).t()
             else:
                 buf = buffer
+                self.wraps = True
                 slate_assert(buf.shape[0] >= bc.mloc and buf.shape[1] >= bc.nloc, "local buffer too small")
                 slate_assert(buf.stride(0) == 1 or buf.shape[0] <= 1, "local buffer must be column-major")
                 bc.lld = max(1, buf.stride(1))

@@ -23,7 +23,9 @@ moves them) and makes its block of C with one launch: the epilogue needs the
 whole sum, and partial sums in 16 bits would be rounded on the way.
 
 Calls enqueue on the current stream of the matrices' device, never
-synchronise, and can be captured into a hipGraph (on one rank).
+synchronise, and can be captured into a hipGraph (on one rank).  On p x q ranks
+the products wait once where matrices over buffers of the caller are written or
+stand beside written ones: the ranks agree on whether any of these overlap.
 """
 from __future__ import annotations
 
@@ -186,6 +188,45 @@ def _outputs(what, outs, ins, same=None):
         for ny, y in outs[:i]:
             if y.ptr < hi and lo < y.end and _overlap(x, y):
                 raise SlateError(f"{what}: outputs {nx} and {ny} overlap")
+
+
+def _rect(M):
+    """A view's block of its storage: first row and column, one past the last ones."""
+    r, c = M.global_offsets()
+    return r, c, r + M._um(), c + M._un()
+
+
+def _share(X, Y, may):
+    """Do two views of one storage share elements?  may: they may be the same view."""
+    a, b = _rect(X), _rect(Y)
+    if may and a == b and (X._op is Op.NoTrans) == (Y._op is Op.NoTrans):
+        return False
+    return max(a[0], b[0]) < min(a[2], b[2]) and max(a[1], b[1]) < min(a[3], b[3])
+
+
+def _apart(what, outs, ins, same=None, ask=True):
+    """:func:`_outputs` for matrices [(name, M)] on a grid of ranks, with one
+    verdict on every rank: views of one storage are compared by their global
+    indexes.  Buffers of the caller are compared by the addresses on this rank;
+    then (ask) the ranks tell each other, and the call waits for the device."""
+    found = comm = None
+    for i, (nx, X) in enumerate(outs):
+        if X is None:
+            continue
+        for ny, Y in ins + outs[:i]:
+            if Y is None:
+                continue
+            may = i == 0 and ny == same
+            if X.storage is Y.storage:
+                if _share(X, Y, may):
+                    raise SlateError(f"{what}: output {nx} overlaps {ny}")
+            elif ask and (X.storage.wraps or Y.storage.wraps):
+                comm = X.storage.comm
+                x, y = _opd(X), _opd(Y)
+                if not (may and (x.ptr, x.ld, x.trans) == (y.ptr, y.ld, y.trans)) and _overlap(x, y):
+                    found = found or f"output {nx} overlaps {ny}"
+    if comm is not None and comm.allreduce_scalar(float(found is not None), "max"):
+        raise SlateError(f"{what}: {found or 'an output overlaps another matrix on another rank'}")
 
 
 def _act(act):
@@ -437,6 +478,7 @@ def gemm_bias_act(alpha, A, B, bias, act, beta, R, C, Z=None, opts=None):
             bshape, bmode = _bias_of(what, bias, m, n)
             _check(dict(A=A, B=B, bias=bias, R=R, C=C, Z=Z),
                    dict(A=(m, k), B=(k, n), bias=bshape, R=(m, n), C=(m, n), Z=(m, n)), what)
+            _apart(what, [("C", C), ("Z", Z)], [("A", A), ("B", B), ("bias", bias), ("R", R)], "R")
             _run_dist(PLAIN, alpha, [A], [B], [C], bias, bmode, a, beta, R, (Z,))
             return C
         oa, ob, o1, orr, oc, oz = _operands(what, ("A", "B", "bias", "R", "C", "Z"), mats)
@@ -473,6 +515,7 @@ def gemm_gated(A1, A2, B, act, C, Z1=None, Z2=None, opts=None):
             m, n, k = C.m(), C.n(), A1.n()
             _check(dict(A1=A1, A2=A2, B=B, C=C, Z1=Z1, Z2=Z2),
                    dict(A1=(m, k), A2=(m, k), B=(k, n), C=(m, n), Z1=(m, n), Z2=(m, n)), what)
+            _apart(what, [("C", C), ("Z1", Z1), ("Z2", Z2)], [("A1", A1), ("A2", A2), ("B", B)])
             outs = [M if M is None or M._op == Op.NoTrans else _grid_work(M, m, n) for M in (C, Z1, Z2)]
             _run_dist(GATED, 1.0, [A1, A2], [B], outs[:1], act=a, Z=tuple(outs[1:]))
             for w, M in zip(outs, (C, Z1, Z2)):
@@ -557,7 +600,8 @@ def gemm_bias_act_grad(alpha, A, B, act, Z, dC, dA, dB, dbias, opts=None):
     dA and dB have the shapes of op(A) and op(B) (pass a transposed view for an
     operand that entered transposed); None leaves a gradient out.  ``Z`` is what
     the forward pass stored (may be None for the identity).  The residual's
-    gradient is beta dC.  dZ is rounded to the matrices' type between the two
+    gradient is beta dC.  dA, dB and dbias overlap no other matrix of the call.
+    dZ is rounded to the matrices' type between the two
     steps, the bias gradient is summed from its unrounded values."""
     what, mats = "gemm_bias_act_grad", (A, B, Z, dC, dA, dB, dbias)
     a = _act(act)
@@ -569,6 +613,7 @@ def gemm_bias_act_grad(alpha, A, B, act, Z, dC, dA, dB, dbias, opts=None):
             bshape, bmode = _bias_of(what, dbias, m, n)
             _check(dict(A=A, B=B, Z=Z, dC=dC, dA=dA, dB=dB, dbias=dbias),
                    dict(A=(m, k), B=(k, n), Z=(m, n), dC=(m, n), dA=(m, k), dB=(k, n), dbias=bshape), what)
+            _apart(what, [("dA", dA), ("dB", dB), ("dbias", dbias)], [("A", A), ("B", B), ("Z", Z), ("dC", dC)])
             dZ = _dz_dist(a, dC, (Z if a else None, None), dbias, bmode)[0]
             if dA is not None:
                 _run_dist_any(PLAIN, alpha, [dZ], [_t(B)], [dA])
@@ -625,6 +670,7 @@ def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
         dA1 = dZ1 op(B)^T,  dA2 = dZ2 op(B)^T,  dB = op(A1)^T dZ1 + op(A2)^T dZ2
 
     with Z1, Z2 as the forward pass stored them; None leaves a gradient out.
+    dA1, dA2 and dB overlap no other matrix of the call.
     Both weight gradients are one launch, and dB is one sum over both products,
     rounded once."""
     what, mats = "gemm_gated_grad", (A1, A2, B, Z1, Z2, dC, dA1, dA2, dB)
@@ -637,6 +683,8 @@ def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
             m, n, k = dC.m(), dC.n(), A1.n()
             w, z = (m, k), (m, n)
             _check(dict(zip(names, mats)), dict(zip(names, (w, w, (k, n), z, z, z, w, w, (k, n)))), what)
+            pairs = list(zip(names, mats))
+            _apart(what, pairs[6:], pairs[:6])
             dZ = _dz_dist(a, dC, (Z1, Z2), None, 0)
             for d, g in zip(dZ, (dA1, dA2)):
                 if g is not None:
@@ -788,6 +836,29 @@ def _clip_apart(what, va, vb):
                 raise SlateError(f"{what}: matrices {p if p >= 0 else ~p} and {q if q >= 0 else ~q} of the call overlap")
 
 
+def _clip_apart_grid(what, A, B, va, vb):
+    """:func:`_clip_apart` on a grid of ranks.  Views of one storage are compared
+    by their global indexes, and refused on every rank alike; -> what buffers of
+    the caller share on this rank."""
+    views = {}
+    for i, M in enumerate(B):
+        views.setdefault(id(M.storage), []).append((i, True, M))
+    if B is not A:
+        for i, M in enumerate(A):
+            views.setdefault(id(M.storage), []).append((i, False, M))
+    for group in views.values():
+        for k, (i, w, X) in enumerate(group):
+            for j, v, Y in group[:k]:
+                if (w or v) and _share(X, Y, i == j and w is not v):
+                    raise SlateError(f"{what}: matrices {j} and {i} of the call overlap")
+    if len(views) > 1 and any(M.storage.wraps for M in (*A, *B)):
+        try:
+            _clip_apart(what, va, vb)
+        except SlateError as e:
+            return e
+    return None
+
+
 def clip_norm(max_norm, A, B=None, opts=None):
     """B_i = min(1, max_norm / s) A_i with s the Frobenius norm of all matrices
     of the list A together; returns s as a float64 tensor on the matrices'
@@ -798,7 +869,8 @@ def clip_norm(max_norm, A, B=None, opts=None):
     are copied (left) as they are, so that a caller can look at s and skip the
     step.  The squares are summed in 64 bits, in an order that depends on the
     sizes alone.  Matrices written overlap no other matrix of the call, except
-    that B_i may be A_i."""
+    that B_i may be A_i.  (On a grid, where buffers of the caller do so on some
+    ranks only, those ranks raise and s is NaN on the others.)"""
     what = "clip_norm"
     limit = float(max_norm)
     if not limit >= 0:
@@ -854,11 +926,15 @@ def _clip(what, limit, A, B):
                     _clip_apart(what, va, vb)
                     mod.clip_norm(ca, cb, mats, top, part, norm, scale, False, st)
             else:
-                if scale:
-                    _clip_apart(what, va, vb)
+                shared = _clip_apart_grid(what, A, B, va, vb) if scale else None
                 n = mod.clip_sum(ca, mats, part, st)
                 mod.clip_join(part, n, norm + 8, st)
+                if shared is not None:
+                    # the others are in the sum already: a NaN keeps them from scaling
+                    ws[1:4].fill_(float("nan"))
                 comm.allreduce(ws[1:4], "sum")
+                if shared is not None:
+                    raise shared
                 mod.clip_scale(ca, cb, mats, top, norm + 8, 1, norm, scale, st)
         if scale:
             for s in todo:

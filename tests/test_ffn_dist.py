@@ -132,3 +132,85 @@ def _clip(rank, size, p, q):
 @pytest.mark.parametrize("p,q", [(2, 1), (2, 2)])
 def test_clip(p, q):
     run_dist(_clip, p * q, p, q)
+
+
+def _refused(call, match="overlap"):
+    with pytest.raises(sl.SlateError, match=match):
+        call()
+
+
+def _overlaps(rank, size, p, q):
+    """Outputs that share elements with other matrices are refused on every
+    rank, as on one; nothing is written."""
+    dt, n = torch.float64, 16
+    mats = [rnd(n, n, dt, i) for i in range(8)]
+    A, A2, B, R, C, Z, G, X = M = [spread(x, 4, p, q) for x in mats]
+    none = None
+    for call in (lambda: sl.gemm_bias_act_grad(1.0, A, B, "gelu", Z, G, A, X, none),
+                 lambda: sl.gemm_bias_act_grad(1.0, A, B, "gelu", Z, G, X, X, none),
+                 lambda: sl.gemm_bias_act_grad(1.0, A, B, "gelu", Z, G, X, Z, none),
+                 lambda: sl.gemm_bias_act_grad(1.0, A, B, "gelu", Z, G, none, none, G.slice(0, n - 1, 3, 3)),
+                 lambda: sl.gemm_bias_act(1.0, A, B, none, "gelu", 0.0, none, C, C),
+                 lambda: sl.gemm_bias_act(1.0, A, B, none, "gelu", 0.0, none, A),
+                 lambda: sl.gemm_bias_act(1.0, A, B, none, "gelu", 0.0, none, A.transpose()),
+                 lambda: sl.gemm_bias_act(1.0, A, B, none, "gelu", 1.0, C.transpose(), C),
+                 lambda: sl.gemm_bias_act(1.0, A, B, C.slice(0, n - 1, 2, 2), "gelu", 1.0, none, C),
+                 lambda: sl.gemm_bias_act(1.0, A.slice(0, 7, 0, n - 1), B, none, "gelu", 1.0, C.slice(1, 8, 0, n - 1),
+                                          C.slice(0, 7, 0, n - 1)),
+                 lambda: sl.gemm_gated(A, A2, B, "silu", C, Z, Z), lambda: sl.gemm_gated(A, A2, B, "silu", B),
+                 lambda: sl.gemm_gated_grad(A, A2, B, "silu", Z, C, G, A, R, X),
+                 lambda: sl.gemm_gated_grad(A, A2, B, "silu", Z, C, G, R, R, X),
+                 lambda: sl.clip_norm(1.0, [A, A]), lambda: sl.clip_norm(1.0, [A, B], [X, A]),
+                 lambda: sl.clip_norm(1.0, [A.slice(0, 4, 0, 4), A.slice(4, 8, 4, 8)]),
+                 lambda: sl.clip_norm(1.0, [A, A.slice(n - 1, n - 1, n - 1, n - 1)])):   # one rank's element
+        _refused(call)
+    for x, m in zip(mats, M):
+        assert torch.equal(D(m), x)
+    # blocks of one matrix that lie apart, the residual's own matrix, and scaling into itself are taken
+    sl.gemm_bias_act(1.0, A, B, none, "identity", 1.0, R, R)
+    within(D(R), mats[3] + mats[0] @ mats[2], 40 * 2.0 ** -53 * (mats[3].abs() + mats[0].abs() @ mats[2].abs()))
+    sl.gemm_bias_act(1.0, A.slice(0, 7, 0, 7), A.slice(0, 7, 8, 15), none, "relu", 0.0, none, A.slice(8, 15, 0, 7))
+    want = (mats[0][:8, :8] @ mats[0][:8, 8:]).clamp(min=0)
+    within(D(A)[8:, :8], want, 40 * 2.0 ** -53 * (mats[0][:8, :8].abs() @ mats[0][:8, 8:].abs()) + 1e-300)
+    s = float(sl.clip_norm(1.0, [B, C.slice(0, 7, 0, 15), C.slice(8, 15, 0, 15)],
+                           [B, X.slice(0, 7, 0, 15), X.slice(8, 15, 0, 15)]))
+    want = math.sqrt(float((mats[2] ** 2).sum() + (mats[4] ** 2).sum()))
+    assert abs(s - want) <= 1e-12 * want
+    assert float((D(X) - mats[4] / want).abs().max()) <= 1e-15
+
+
+@pytest.mark.parametrize("p,q", [(2, 1), (2, 2)])
+def test_overlaps(p, q):
+    run_dist(_overlaps, p * q, p, q)
+
+
+def _own_buffers(rank, size):
+    """Buffers of the caller that overlap on one rank only: every rank is told
+    (clipping: that rank, and the others' norm is NaN), none waits for another."""
+    n, dt = 16, torch.float64
+    buf = torch.randn(n // size * n * 2, generator=torch.Generator().manual_seed(rank), dtype=dt)
+    was = buf.clone()
+    half = n // size * n
+
+    def wrap(first):
+        return sl.Matrix.fromScaLAPACK(n, n, buf[first:first + half].view(n, n // size).t(), nb=4, p=size, q=1)
+
+    A, B = wrap(0), wrap(half if rank == 0 else half - 8)
+    E, F = (spread(rnd(n, n, dt, i), 4, size, 1) for i in (1, 2))
+    _refused(lambda: sl.gemm_bias_act(1.0, A, E, None, "relu", 0.0, None, B))
+    _refused(lambda: sl.gemm_bias_act_grad(1.0, A, E, "relu", F, F, B, None, None))
+    _refused(lambda: sl.gemm_gated_grad(A, E, E, "relu", F, F, F, None, None, B))
+    if rank == 0:
+        assert math.isnan(float(sl.clip_norm(1.0, [A, B])))
+    else:
+        _refused(lambda: sl.clip_norm(1.0, [A, B]))
+    assert torch.equal(buf, was)
+    A, B = wrap(0), wrap(half)
+    sl.gemm_bias_act(1.0, E, F, None, "identity", 0.0, None, B)
+    e, f = rnd(n, n, dt, 1), rnd(n, n, dt, 2)
+    within(D(B), e @ f, 40 * 2.0 ** -53 * (e.abs() @ f.abs()))
+    assert torch.equal(buf[:half], was[:half])
+
+
+def test_own_buffers():
+    run_dist(_own_buffers, 2)
