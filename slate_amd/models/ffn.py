@@ -136,13 +136,19 @@ def _operands(what, names, mats):
 
 
 def _one(mats):
-    """Is every matrix on one rank?"""
+    """1: every matrix is this rank's alone; 2: each is on one rank, some among
+    several; 0: some is on several."""
+    one = 1
     for M in mats:
         if M is not None:
             s = M.storage
-            if s.bc is None or (s.comm.size > 1 and s.bc.p * s.bc.q > 1):
-                return s.bc is None         # not block-cyclic: the checks refuse it
-    return True
+            if s.bc is None:
+                return 1                    # not block-cyclic: the checks refuse it
+            if s.comm.size > 1:
+                if s.bc.p * s.bc.q > 1:
+                    return 0
+                one = 2
+    return one
 
 
 def _shape(what, name, x, m, n):
@@ -260,6 +266,8 @@ def _check(mats, shapes, what):
                 raise SlateError(f"{what}: element type {s.dtype} (bfloat16, float16, float32 or float64 are wanted)")
         elif s.dtype != first.dtype:
             raise SlateError(f"{what}: {name} has type {s.dtype}, the others {first.dtype}")
+        elif s.comm.ranks != first.comm.ranks:
+            raise SlateError(f"{what}: {name} has another communicator than the others")
         if s.origin_slot is None:
             raise SlateError(f"{what}: {name} has no tiles (insertLocalTiles)")
         if _where(s) != _where(first):
@@ -473,14 +481,17 @@ def gemm_bias_act(alpha, A, B, bias, act, beta, R, C, Z=None, opts=None):
         return C
     what, mats = "gemm_bias_act", (A, B, bias, R, C, Z)
     with trace_block(what):
-        if not _one(mats):
+        one = _one(mats)
+        if one != 1:
             m, n, k = C.m(), C.n(), A.n()
             bshape, bmode = _bias_of(what, bias, m, n)
             _check(dict(A=A, B=B, bias=bias, R=R, C=C, Z=Z),
                    dict(A=(m, k), B=(k, n), bias=bshape, R=(m, n), C=(m, n), Z=(m, n)), what)
-            _apart(what, [("C", C), ("Z", Z)], [("A", A), ("B", B), ("bias", bias), ("R", R)], "R")
-            _run_dist(PLAIN, alpha, [A], [B], [C], bias, bmode, a, beta, R, (Z,))
-            return C
+            _apart(what, [("C", C), ("Z", Z)], [("A", A), ("B", B), ("bias", bias), ("R", R)], "R", not one)
+            if not one:
+                _run_dist(PLAIN, alpha, [A], [B], [C], bias, bmode, a, beta, R, (Z,))
+            if not one or C.storage.bc.pr < 0:
+                return C
         oa, ob, o1, orr, oc, oz = _operands(what, ("A", "B", "bias", "R", "C", "Z"), mats)
         m, n, k = oc.m, oc.n, oa.n
         _shape(what, "A", oa, m, k)
@@ -511,17 +522,20 @@ def gemm_gated(A1, A2, B, act, C, Z1=None, Z2=None, opts=None):
     a = _act(act)
     what, mats = "gemm_gated", (A1, A2, B, C, Z1, Z2)
     with trace_block(what):
-        if not _one(mats):
+        one = _one(mats)
+        if one != 1:
             m, n, k = C.m(), C.n(), A1.n()
             _check(dict(A1=A1, A2=A2, B=B, C=C, Z1=Z1, Z2=Z2),
                    dict(A1=(m, k), A2=(m, k), B=(k, n), C=(m, n), Z1=(m, n), Z2=(m, n)), what)
-            _apart(what, [("C", C), ("Z1", Z1), ("Z2", Z2)], [("A1", A1), ("A2", A2), ("B", B)])
-            outs = [M if M is None or M._op == Op.NoTrans else _grid_work(M, m, n) for M in (C, Z1, Z2)]
-            _run_dist(GATED, 1.0, [A1, A2], [B], outs[:1], act=a, Z=tuple(outs[1:]))
-            for w, M in zip(outs, (C, Z1, Z2)):
-                if w is not M:
-                    _copy_out(w, M)
-            return C
+            _apart(what, [("C", C), ("Z1", Z1), ("Z2", Z2)], [("A1", A1), ("A2", A2), ("B", B)], None, not one)
+            if not one:
+                outs = [M if M is None or M._op == Op.NoTrans else _grid_work(M, m, n) for M in (C, Z1, Z2)]
+                _run_dist(GATED, 1.0, [A1, A2], [B], outs[:1], act=a, Z=tuple(outs[1:]))
+                for w, M in zip(outs, (C, Z1, Z2)):
+                    if w is not M:
+                        _copy_out(w, M)
+            if not one or C.storage.bc.pr < 0:
+                return C
         o1, o2, ob, oc, z1, z2 = _operands(what, ("A1", "A2", "B", "C", "Z1", "Z2"), mats)
         m, n, k = oc.m, oc.n, o1.n
         _shape(what, "A1", o1, m, k)
@@ -608,18 +622,22 @@ def gemm_bias_act_grad(alpha, A, B, act, Z, dC, dA, dB, dbias, opts=None):
     if Z is None and a:
         raise SlateError(f"{what}: Z is wanted for activation {act}")
     with trace_block(what):
-        if not _one(mats):
+        one = _one(mats)
+        if one != 1:
             m, n, k = dC.m(), dC.n(), A.n()
             bshape, bmode = _bias_of(what, dbias, m, n)
             _check(dict(A=A, B=B, Z=Z, dC=dC, dA=dA, dB=dB, dbias=dbias),
                    dict(A=(m, k), B=(k, n), Z=(m, n), dC=(m, n), dA=(m, k), dB=(k, n), dbias=bshape), what)
-            _apart(what, [("dA", dA), ("dB", dB), ("dbias", dbias)], [("A", A), ("B", B), ("Z", Z), ("dC", dC)])
-            dZ = _dz_dist(a, dC, (Z if a else None, None), dbias, bmode)[0]
-            if dA is not None:
-                _run_dist_any(PLAIN, alpha, [dZ], [_t(B)], [dA])
-            if dB is not None:
-                _run_dist_any(PLAIN, alpha, [_t(A)], [dZ], [dB])
-            return
+            _apart(what, [("dA", dA), ("dB", dB), ("dbias", dbias)], [("A", A), ("B", B), ("Z", Z), ("dC", dC)],
+                   None, not one)
+            if not one:
+                dZ = _dz_dist(a, dC, (Z if a else None, None), dbias, bmode)[0]
+                if dA is not None:
+                    _run_dist_any(PLAIN, alpha, [dZ], [_t(B)], [dA])
+                if dB is not None:
+                    _run_dist_any(PLAIN, alpha, [_t(A)], [dZ], [dB])
+            if not one or dC.storage.bc.pr < 0:
+                return
         oa, ob, oz, oc, ga, gb, gv = _operands(what, ("A", "B", "Z", "dC", "dA", "dB", "dbias"), mats)
         m, n, k = oc.m, oc.n, oa.n
         for name, x, r, c in (("A", oa, m, k), ("B", ob, k, n), ("Z", oz, m, n), ("dA", ga, m, k), ("dB", gb, k, n)):
@@ -679,19 +697,22 @@ def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
     if Z1 is None or Z2 is None:
         raise SlateError(f"{what}: Z1 and Z2 are wanted")
     with trace_block(what):
-        if not _one(mats):
+        one = _one(mats)
+        if one != 1:
             m, n, k = dC.m(), dC.n(), A1.n()
             w, z = (m, k), (m, n)
             _check(dict(zip(names, mats)), dict(zip(names, (w, w, (k, n), z, z, z, w, w, (k, n)))), what)
             pairs = list(zip(names, mats))
-            _apart(what, pairs[6:], pairs[:6])
-            dZ = _dz_dist(a, dC, (Z1, Z2), None, 0)
-            for d, g in zip(dZ, (dA1, dA2)):
-                if g is not None:
-                    _run_dist_any(PLAIN, 1.0, [d], [_t(B)], [g])
-            if dB is not None:
-                _run_dist_any(SUM, 1.0, [_t(A1), _t(A2)], dZ, [dB])
-            return
+            _apart(what, pairs[6:], pairs[:6], None, not one)
+            if not one:
+                dZ = _dz_dist(a, dC, (Z1, Z2), None, 0)
+                for d, g in zip(dZ, (dA1, dA2)):
+                    if g is not None:
+                        _run_dist_any(PLAIN, 1.0, [d], [_t(B)], [g])
+                if dB is not None:
+                    _run_dist_any(SUM, 1.0, [_t(A1), _t(A2)], dZ, [dB])
+            if not one or dC.storage.bc.pr < 0:
+                return
         o1, o2, ob, z1, z2, oc, g1, g2, gb = opds = _operands(what, names, mats)
         m, n, k = oc.m, oc.n, o1.n
         w, z = (m, k), (m, n)

@@ -214,3 +214,52 @@ def _own_buffers(rank, size):
 
 def test_own_buffers():
     run_dist(_own_buffers, 2)
+
+
+def _one_of(rank, size):
+    """Matrices on one rank of a larger communicator: the others take part without elements."""
+    m, n, k, dt = 12, 9, 10, torch.float64
+    a, a2, b, r, g = rnd(m, k, dt, 1), rnd(m, k, dt, 2), rnd(k, n, dt, 3), rnd(m, n, dt, 4), rnd(m, n, dt, 5)
+    A, A2, B, R, G, C, Z, Z2 = (spread(x, 4, 1, 1) for x in (a, a2, b, r, g, 0 * r, 0 * r, 0 * r))
+    tol = 400 * 2.0 ** -53
+    for bias in (rnd(m, 1, dt, 6), rnd(1, n, dt, 6), None):
+        bv = None if bias is None else spread(bias, 4, 1, 1)
+        sl.gemm_bias_act(1.0, A, B, bv, "gelu", 1.0, R, C, Z)
+        z = a @ b + (0 if bias is None else bias)
+        y, s = act64("gelu", z)
+        assert float((D(Z) - z).abs().max()) <= tol * 10 and float((D(C) - y - r).abs().max()) <= tol * 10
+        dA, dB, db = spread(0 * a, 4, 1, 1), spread(0 * b, 4, 1, 1), None if bv is None else spread(0 * bias, 4, 1, 1)
+        sl.gemm_bias_act_grad(1.0, A, B, "gelu", Z, G, dA, dB, db)
+        dz = g * s
+        assert float((D(dA) - dz @ b.t()).abs().max()) <= tol * 100 and float((D(dB) - a.t() @ dz).abs().max()) <= tol * 100
+        if db is not None:
+            d = 1 if bias.shape[1] == 1 else 0
+            assert float((D(db) - dz.sum(d, keepdim=True)).abs().max()) <= tol * 100
+    sl.gemm_gated(A, A2, B, "silu", C, Z, Z2)
+    v, s = act64("silu", a @ b)
+    assert float((D(C) - v * (a2 @ b)).abs().max()) <= tol * 100
+    sl.gemm_gated_grad(A, A2, B, "silu", Z, Z2, G, None, None, dB)
+    want = a.t() @ (g * (a2 @ b) * s) + a2.t() @ (g * v)
+    assert float((D(dB) - want).abs().max()) <= tol * 1000
+    # refusals are every rank's
+    long = spread(rnd(m + 1, 1, dt, 6), 4, 1, 1)
+    _refused(lambda: sl.gemm_bias_act(1.0, A, B, long, "gelu", 1.0, R, C, Z), "bias")
+    _refused(lambda: sl.gemm_bias_act(1.0, B, A, None, "gelu", 1.0, R, C, Z), "wanted")
+    _refused(lambda: sl.gemm_bias_act_grad(1.0, A, B, "gelu", Z, G, dA, dB, long), "bias")
+    _refused(lambda: sl.gemm_gated(A, A2, B, "silu", C, Z, Z))
+    _refused(lambda: sl.gemm_gated_grad(A, A2, B, "silu", Z, Z2, G, A, None, dB))
+    # no rank waits for another: the one with the elements may call alone
+    if rank == 0:
+        sl.gemm_bias_act(1.0, A, B, bv, "gelu", 1.0, R, C, Z)
+    # another communicator
+    from slate_amd.parallel.comm import self_comm
+    own = sl.Matrix.fromLAPACK(m, n, torch.zeros(n, m, dtype=dt).t(), nb=4, comm=self_comm())
+    _refused(lambda: sl.gemm_bias_act(1.0, A, B, None, "gelu", 0.0, None, own), "communicator")
+    two = spread(0 * r, 4, size, 1)
+    _refused(lambda: sl.gemm_bias_act(1.0, A, B, None, "gelu", 1.0, own, two), "communicator")
+    sl.gemm_bias_act(1.0, A, B, None, "identity", 0.0, None, two)
+    assert float((D(two) - a @ b).abs().max()) <= tol * 10
+
+
+def test_one_of_two():
+    run_dist(_one_of, 2)
