@@ -150,7 +150,21 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(ClipArgs a) {
     const double norm = clip_norm_of(a, lds);
     if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
     const bool cut = norm > a.limit && norm < __builtin_huge_val();
-    const R f = cut ? (R)(a.limit / norm) : R(1);
+    // The factor as f 2^e: e is 0 where limit / norm is a normal number of the
+    // sums' type; below it would lose bits, or all of them, and ordinary products
+    // with it (elements of 2e38, limit 1e-6).  Scaling by 2^e is exact.
+    const double q = a.limit / norm;
+    R f = (R)q;
+    int e = 0, en;
+    if (cut && q < (sizeof(R) == 4 ? 0x1p-126 : 0x1p-1022)) {
+        const double part = 0.5 * frexp(a.limit, &e);
+        f = (R)(part / frexp(norm, &en));          // in [1/4, 1]
+        e += 1 - en;
+    }
+    auto scaled = [&](R x) {
+        if constexpr (sizeof(R) == 4) return cut ? __builtin_amdgcn_ldexpf(x * f, e) : x;
+        else return cut ? __builtin_amdgcn_ldexp(x * f, e) : x;
+    };
     // backwards: what the first pass read last is still in the cache
     for (int u = a.first[a.count] - 1 - (int)blockIdx.x; u >= 0; u -= gridDim.x) {
         const int c = clip_find(a, u);
@@ -169,12 +183,11 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(ClipArgs a) {
             for (int b = 0; b < N; ++b) {
                 vB y;
                 #pragma unroll
-                for (int e = 0; e < E; ++e) y[e] = (TB)(cut ? (R)x[b][e] * f : (R)x[b][e]);
+                for (int k = 0; k < E; ++k) y[k] = (TB)scaled((R)x[b][k]);
                 *reinterpret_cast<vB*>(B + i + b * (256 * E) + j * v.ldb) = y;
             }
         }, [&](i64 i, i64 j) {
-            const R x = (R)A[i + j * v.lda];
-            B[i + j * v.ldb] = (TB)(cut ? x * f : x);
+            B[i + j * v.ldb] = (TB)scaled((R)A[i + j * v.lda]);
         });
     }
 }

@@ -162,7 +162,14 @@ void clip_scale(char ta, char tb, const std::vector<i64>& v, double limit, const
     *norm_out = norm;
     if (!scale) return;
     const bool cut = norm > limit && norm < std::numeric_limits<double>::infinity();
-    const double f = cut ? limit / norm : 1.0;
+    // the factor as f 2^e: beyond the normal numbers limit / norm has lost bits
+    double f = cut ? limit / norm : 1.0;
+    int e = 0, en;
+    if (f < std::numeric_limits<double>::min()) {
+        f = 0.5 * std::frexp(limit, &e);
+        f /= std::frexp(norm, &en);                // in (1/4, 1)
+        e += 1 - en;
+    }
     real_dispatch(ta, [&](auto za) { real_dispatch(tb, [&](auto zb) {
         using TA = decltype(za); using TB = decltype(zb);
         for (size_t q = 0; q + 5 < v.size(); q += 6) {
@@ -171,7 +178,7 @@ void clip_scale(char ta, char tb, const std::vector<i64>& v, double limit, const
             TB* B = ptr<TB>((uintptr_t)v[q + 2]);
             for (i64 j = 0; j < v[q + 5]; ++j)
                 for (i64 i = 0; i < v[q + 4]; ++i)
-                    B[i + j * v[q + 3]] = put<TB>((double)A[i + j * v[q + 1]] * f);
+                    B[i + j * v[q + 3]] = put<TB>(std::ldexp((double)A[i + j * v[q + 1]] * f, e));
         }
     }); });
 }

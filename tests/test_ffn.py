@@ -989,3 +989,34 @@ def test_clip_types_share_memory(dev, dt):
     y = buf[32:].view(4, 8).t()
     sl.clip_norm(1e9, [mat(x)], [mat(y)])
     assert torch.equal(y, x.float())
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt,out", CLIP_TYPES[:6])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_clip_far_factors(dev, dt, out, pad):
+    """Factors that the sums' type does not hold, or not with all its bits: the
+    scaled elements are off as others are (4 w and the store's rounding; a
+    subnormal result by its half step once more)."""
+    rt = torch.float64 if dt == torch.float64 else torch.float32
+    top = math.frexp(torch.finfo(dt).max)[1]
+    step = torch.finfo(out).tiny * torch.finfo(out).eps
+    for size in (2.0 ** (top - 7), 2.0 ** (top - 12)):
+        unit = cm(60, 33, dt, 1, dev).double().clamp(-8, 8)
+        x, y = cm(60, 33, dt, 1, dev, 1.0, pad), cm(60, 33, out, 2, dev, 1.0, pad)
+        unit[3, 4], unit[5, 6] = 1 / size, 0.0
+        norm = float(unit.norm())                                     # x = size unit, exactly
+        for limit in (1.0, 1e-3, 1e-6, size * 2.0 ** -126, size * 2.0 ** -100, torch.finfo(rt).tiny, 1e-310, 5e-324):
+            x.copy_(unit * size)
+            part, e = math.frexp(limit)
+            want = torch.ldexp(torch.ldexp(unit * (part / norm), torch.tensor(e // 2, device=dev)),
+                               torch.tensor(e - e // 2, device=dev))
+            s = float(sl.clip_norm(limit, [mat(x)], [mat(y)]))
+            assert abs(s / size - norm) <= 2000 * 2.0 ** -53 * norm
+            # the sum of 1980 squares, the product, the store; what ends subnormal by half a step of
+            # either the product or the store
+            rel = u_of(out) + 4 * w_of(out) + 2000 * 2.0 ** -53
+            assert ((y.double() - want).abs() <= rel * want.abs() + step).all(), (size, limit)
+            if dt == out:
+                sl.clip_norm(limit, [mat(x)])
+                assert torch.equal(x, y)
