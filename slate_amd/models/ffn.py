@@ -563,7 +563,7 @@ def _act_grad(m, n, act, dC, Z1, Z2, dZ1, dZ2, db=_NONE, bias_mode=0, wide=False
     t = dC.t
     if m == 0 or n == 0:
         if db.t is not None:
-            db.t.zero_()
+            db.t[:db.rows, :db.cols].zero_()
         return
     mod, dt = kmod(t), REAL_CODE[t.dtype]
     nbytes = mod.act_grad_ws(dt, bias_mode, m, n)
@@ -776,7 +776,7 @@ def _dz_dist(act, dC, Z, dbias, bmode):
     if dbias is not None:
         wide = torch.float64 if s.dtype == torch.float64 else torch.float32
         sums = torch.zeros(lb.mloc if bmode == 1 else lb.nloc, dtype=wide, device=lb.data.device)
-        db = _Opd(sums.data_ptr(), 1, sums.numel(), 1, False, sums)
+        db = _Opd(sums.data_ptr(), sums.numel(), sums.numel(), 1, False, sums.view(-1, 1))
     if s.bc.pr >= 0 and (act or two or dbias is not None):
         oz = [_NONE if z is None else _opd(z) for z in Zw]
         od = [_opd(d) for d in dZ] if act or two else [_NONE]

@@ -1020,3 +1020,16 @@ def test_clip_far_factors(dev, dt, out, pad):
             if dt == out:
                 sl.clip_norm(limit, [mat(x)])
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("trans", [False, True])
+def test_no_tokens_in_a_larger_buffer(dev, dt, trans):
+    """The zero bias gradient of an empty batch does not reach what lies around the vector."""
+    A, B = cm(16, 32, dt, 1, dev), torch.empty(0, 32, dtype=dt, device=dev).t()
+    E = mat(torch.empty(16, 0, dtype=dt, device=dev).t(), True) if trans else mat(torch.empty(0, 16, dtype=dt, device=dev).t())
+    whole = torch.ones(2, 24, dtype=dt, device=dev).t()
+    b = sl.Matrix.fromScaLAPACK(16, 1, whole, nb=8)
+    sl.gemm_bias_act_grad(1.0, mat(A), mat(B), "gelu", E, E, None, None, b)
+    assert (whole[:16, 0] == 0).all() and (whole[16:] == 1).all() and (whole[:, 1] == 1).all()
