@@ -372,10 +372,11 @@ class MatrixStorage:
     def mark_local_modified(self, slot):
         """After a whole-local-buffer kernel wrote `slot` (the post-condition
         of every driver: with SLATE_AMD_DEBUG=1 the MOSI checker runs here)."""
-        if self._marked == (slot, self.table.version()):
+        now = self.table.version()
+        if self._marked == (slot, now):
             return                     # nothing changed a state since
         self.table.mark_all(slot, _host.MOSI_Modified)
-        self._marked = (slot, self.table.version())
+        self._marked = (slot, now + 1)     # (not where another thread changed one meanwhile)
         from ..utils.debug import Debug
         if Debug.enabled():
             Debug.assert_mosi(self, "mark_local_modified")
@@ -392,6 +393,9 @@ class MatrixStorage:
             if slot not in self.local:
                 self.allocate_local(slot)
             other = HOST if slot == DEV else DEV
+            # the version without changes but those made here: one made meanwhile by
+            # another thread (tileModified takes no lock) is seen by the next call
+            seen = self.table.version()
             need = False
             for (i, j, s) in self.table.instances():
                 if s == slot and self.tileIsLocal(i, j) and \
@@ -413,10 +417,11 @@ class MatrixStorage:
                                                    (i, j, srcs[0]) not in self.tiles):
                             self.local_tile_view(slot, i, j).copy_(sd)
                     self.table.set_state(i, j, slot, _host.MOSI_Shared)
+                    seen += 1
             from ..utils.debug import Debug
             if Debug.enabled():
                 Debug.assert_mosi(self, "prepare_local")
-            self._valid[slot] = self.table.version()
+            self._valid[slot] = seen
             return self.local[slot]
 
     def sync_origin(self):

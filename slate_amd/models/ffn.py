@@ -104,7 +104,7 @@ def _opd(M, name="matrix"):
         rows, cols = t.shape
     x = _of_tensor(t, rows, cols, M._op is not Op.NoTrans, name)
     x.table = s.table
-    x.version = s.table.version() if s._valid.get(slot) == s.table.version() else -1
+    x.version = s._valid.get(s.origin_slot, -1)      # (an older one is never met again)
     M.__dict__["_operand"] = x
     return x
 

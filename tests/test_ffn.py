@@ -1033,3 +1033,65 @@ def test_no_tokens_in_a_larger_buffer(dev, dt, trans):
     b = sl.Matrix.fromScaLAPACK(16, 1, whole, nb=8)
     sl.gemm_bias_act_grad(1.0, mat(A), mat(B), "gelu", E, E, None, None, b)
     assert (whole[:16, 0] == 0).all() and (whole[16:] == 1).all() and (whole[:, 1] == 1).all()
+
+
+class _Meddling:
+    """A storage's tile table that another thread changes right after a call of `name`."""
+
+    def __init__(self, table, name, act):
+        self._table, self._name, self._act = table, name, act
+
+    def __getattr__(self, k):
+        f = getattr(self._table, k)
+        if k != self._name:
+            return f
+
+        def call(*a):
+            r = f(*a)
+            act, self._act = self._act, None
+            if act is not None:
+                act()
+            return r
+        return call
+
+
+def _two_sides():
+    """An 8 x 8 matrix with a buffer on either side (both in host memory here)."""
+    from slate_amd.core.storage import DEV, HOST
+    x = cm(8, 8, torch.float64, 1, "cpu")
+    s = mat(x, nb=4).storage
+    y = s.allocate_local(DEV)
+    s.prepare_local(DEV)
+    return x, y, s, HOST, DEV
+
+
+def test_change_while_a_side_is_made_valid(monkeypatch):
+    """A tile modified on the other side after the scan of the states is copied by the next call."""
+    from slate_amd.utils.debug import Debug
+    x, y, s, HOST, DEV = _two_sides()
+    todo = [True]
+
+    def enabled():                                       # asked between the scan and its end
+        if todo:
+            todo.clear()
+            x[0, 0] = 7.0
+            s.tileModified(0, 0, HOST, True)
+        return False
+
+    monkeypatch.setattr(Debug, "enabled", enabled)
+    s.tileModified(1, 1, HOST, True)
+    s.prepare_local(DEV)
+    s.prepare_local(DEV)
+    assert not todo and y[0, 0] == 7.0 and torch.equal(x, y[:8, :8])
+
+
+def test_change_while_a_side_is_marked():
+    """A tile modified on the other side right after a mark is marked by the next one."""
+    from slate_amd import _native
+    x, y, s, HOST, DEV = _two_sides()
+    s.table = _Meddling(s.table, "mark_all", lambda: s.tileModified(0, 0, HOST, True))
+    s.mark_local_modified(DEV)
+    assert s.table.state(0, 0, DEV) == _native._host.MOSI_Invalid
+    s.mark_local_modified(DEV)
+    assert s.table.state(0, 0, DEV) == _native._host.MOSI_Modified
+    assert s.table.state(0, 0, HOST) == _native._host.MOSI_Invalid
