@@ -91,6 +91,18 @@ class BlockCyclic:
         return (i % self.p) * self.q + (j % self.q)
 
 
+_debug = None
+
+
+def debug_checks() -> bool:
+    """Do the debug checks run?  (utils/debug.py imports this module.)"""
+    global _debug
+    if _debug is None:
+        from ..utils.debug import Debug
+        _debug = Debug
+    return _debug.enabled()
+
+
 class MatrixStorage:
     def __init__(self, m: int, n: int, tileMb: Callable, tileNb: Callable,
                  tileRank: Callable, comm, dtype=torch.float64,
@@ -373,19 +385,17 @@ class MatrixStorage:
         """After a whole-local-buffer kernel wrote `slot` (the post-condition
         of every driver: with SLATE_AMD_DEBUG=1 the MOSI checker runs here)."""
         now = self.table.version()
-        if self._marked == (slot, now):
-            return                     # nothing changed a state since
-        self.table.mark_all(slot, _host.MOSI_Modified)
-        self._marked = (slot, now + 1)     # (not where another thread changed one meanwhile)
-        from ..utils.debug import Debug
-        if Debug.enabled():
-            Debug.assert_mosi(self, "mark_local_modified")
+        if self._marked != (slot, now):        # (else nothing changed a state since)
+            self.table.mark_all(slot, _host.MOSI_Modified)
+            self._marked = (slot, now + 1)     # (not where another thread changed one meanwhile)
+        if debug_checks():
+            _debug.assert_mosi(self, "mark_local_modified")
 
     def prepare_local(self, slot) -> torch.Tensor:
         """Make the contiguous local buffer valid in `slot` and return it."""
         bc = self.bc
         slate_assert(bc is not None, "prepare_local requires block-cyclic storage")
-        if self._valid.get(slot) == self.table.version() and slot in self.local:
+        if self._valid.get(slot) == self.table.version() and slot in self.local and not debug_checks():
             return self.local[slot]    # no tile state changed since it was found whole
         with self.lock:
             if self.origin_slot is None:
@@ -418,9 +428,8 @@ class MatrixStorage:
                             self.local_tile_view(slot, i, j).copy_(sd)
                     self.table.set_state(i, j, slot, _host.MOSI_Shared)
                     seen += 1
-            from ..utils.debug import Debug
-            if Debug.enabled():
-                Debug.assert_mosi(self, "prepare_local")
+            if debug_checks():
+                _debug.assert_mosi(self, "prepare_local")
             self._valid[slot] = seen
             return self.local[slot]
 

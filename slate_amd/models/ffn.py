@@ -35,7 +35,7 @@ from .. import ops
 from .._native import REAL_CODE, kmod, raw_stream
 from ..core.enums import Activation, Op
 from ..core.exceptions import SlateError
-from ..core.storage import DEV
+from ..core.storage import DEV, debug_checks
 from ..utils.trace import trace_block
 from ._panels import col_bcast, row_bcast
 from ._util import grid_of, tiles_local_before
@@ -90,10 +90,12 @@ def _of_tensor(t, rows, cols, trans=False, name="matrix"):
 def _opd(M, name="matrix"):
     """The (one) rank's operand of a view.  A view remembers it, and uses it again
     while it has the same storage, no state of whose tiles has changed (new buffers
-    and writes on the other side do), and its buffer is at the same place."""
+    and writes on the other side do), and its buffer is at the same place.  (With
+    the debug checks on, prepare_local runs them on every call.)"""
     s = M.storage
     x = M.__dict__.get("_operand")
-    if x is not None and x.table is s.table and x.version == s.table.version() and x.t.data_ptr() == x.ptr:
+    if x is not None and x.table is s.table and x.version == s.table.version() and x.t.data_ptr() == x.ptr \
+            and not debug_checks():
         return x
     slot = s.origin_slot
     if M._mt == s.mt and M._nt == s.nt and not (M.row0_offset or M.col0_offset) and M.last_mb is None \
@@ -805,7 +807,7 @@ def _clip_views(mats, what):
     if not isinstance(mats, (list, tuple)):
         raise SlateError(f"{what}: a list of matrices is wanted")
     out, todo, dt, dev, comm = [], [], None, None, None
-    add = out.append
+    add, anew = out.append, debug_checks()
     for M in mats:
         s = M.storage
         slot = s.origin_slot
@@ -814,7 +816,7 @@ def _clip_views(mats, what):
         x = M.__dict__.get("_operand")
         # (the use of a remembered operand, as in _opd, without the call)
         now = s.table.version()
-        if x is None or x.table is not s.table or x.version != now or x.t.data_ptr() != x.ptr:
+        if anew or x is None or x.table is not s.table or x.version != now or x.t.data_ptr() != x.ptr:
             if slot is None:
                 raise SlateError(f"{what}: a matrix has no tiles (insertLocalTiles)")
             x = _opd(M)
@@ -825,7 +827,7 @@ def _clip_views(mats, what):
             raise SlateError(f"{what}: the matrices differ in type or device ({x.dt} on {x.dev}, {dt} on {dev})")
         elif s.comm is not comm and s.comm.ranks != comm.ranks:
             raise SlateError(f"{what}: the matrices differ in communicator")
-        if s._marked != (slot, now):
+        if anew or s._marked != (slot, now):
             todo.append(s)
         add(x)
     return out, todo

@@ -1095,3 +1095,30 @@ def test_change_while_a_side_is_marked():
     s.mark_local_modified(DEV)
     assert s.table.state(0, 0, DEV) == _native._host.MOSI_Modified
     assert s.table.state(0, 0, HOST) == _native._host.MOSI_Invalid
+
+
+def test_debug_checks_where_states_are_remembered(monkeypatch):
+    """With the debug checks on, a call that remembers its operands runs them too."""
+    from slate_amd import _native
+    from slate_amd.utils.debug import Debug
+    monkeypatch.setattr(Debug, "_on", False)
+    x, y, s, HOST, DEV = _two_sides()
+    A = mat(x, nb=4)
+    A.storage = s
+    sl.global_norm([A])
+    x[1, 2] += 1.0                                       # both sides are valid, and differ now
+    sl.global_norm([A])
+    C = mat(cm(8, 8, torch.float64, 2, "cpu"))
+    monkeypatch.setattr(Debug, "_on", True)
+    for call in (lambda: s.prepare_local(HOST), lambda: s.prepare_local(DEV), lambda: sl.global_norm([A]),
+                 lambda: sl.clip_norm(1.0, [A]),
+                 lambda: sl.gemm_bias_act(1.0, A, A, None, "relu", 0.0, None, C)):
+        with pytest.raises(SlateError, match="MOSI"):
+            call()
+    monkeypatch.setattr(Debug, "_on", False)
+    s = mat(x, nb=4).storage
+    s.table.set_state(0, 0, HOST, _native._host.MOSI_Shared | _native._host.MOSI_OnHold)
+    s.mark_local_modified(HOST)
+    monkeypatch.setattr(Debug, "_on", True)
+    with pytest.raises(SlateError, match="MOSI"):
+        s.mark_local_modified(HOST)
