@@ -134,10 +134,13 @@ def build(verbose=False, hip=True, host=True):
             HIPFLAGS + ["-fvisibility=hidden"] + inc,
             ["--offload-arch=" + ARCH, "-L" + os.path.join(ROCM, "lib"), "-lamdhip64"], verbose))
         # Python-free native library (include/slate_amd/slate_native.hh): the
-        # same kernel objects (minus the pybind11 units) + the C++ host
+        # same kernel objects (minus the pybind11 units and the kernels of
+        # models/ffn.py, which it has no entry points for) + the C++ host
         # runtime / drivers of csrc/native, linked against HIP and RCCL only
+        without = ("bindings", "bindings_ffn", "devpool", "act_grad", "clip", "copy16",
+                   "gemm_act_b", "gemm_act_d", "gemm_act_h", "gemm_act_plan", "gemm_act_s")
         kobjs = [o for o in sorted(glob.glob(os.path.join(BUILD, "_hip", "*.hip.o")))
-                 if os.path.basename(o) not in ("bindings.hip.o", "bindings_ffn.hip.o", "devpool.hip.o")]
+                 if os.path.basename(o)[:-len(".hip.o")] not in without]
         out.append(_build_module(
             "libslate_amd_native", os.path.join(HERE, "csrc", "native"), [".hip"], hipcc,
             HIPFLAGS + ["-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(ROCM, "include")],
