@@ -1122,3 +1122,79 @@ def test_debug_checks_where_states_are_remembered(monkeypatch):
     monkeypatch.setattr(Debug, "_on", True)
     with pytest.raises(SlateError, match="MOSI"):
         s.mark_local_modified(HOST)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("k", [3, 641, 4096, 4099])
+@pytest.mark.parametrize("pad,off", [(0, 0), (3, 1), (5, 0)])
+def test_few_columns(dt, k, pad, off):
+    """Up to 16 columns and both operands along k, 1024 rows or more: whole batches of slabs and a
+    ragged end of K, columns and rows past the matrix, operands off 16 bytes."""
+    for m, n in ((1024, 1), (1030, 2), (4096, 7), (1024, 15), (1030, 16)):
+        Product(dt, "cuda", m, n, k, "T", "N", act="gelu", bias=1 + n % 2, pad=pad, off=off, cpad=pad).check()
+        Gated(dt, "cuda", m, n, k, "T", "N", pad=pad, off=off).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("m,n,k", [(5120, 15, 5888), (5120, 8, 5888), (4096, 15, 5888), (8192, 16, 5888), (5121, 9, 5887),
+                                   (4097, 16, 1000), (1023, 16, 5888), (1024, 17, 5888)])
+def test_few_columns_borders(dt, m, n, k):
+    """Either side of the rules that send few columns to tiles with K in pieces."""
+    Product(dt, "cuda", m, n, k, "T", "N", act="silu").check()
+    Gated(dt, "cuda", m, n, k, "T", "N").check()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("count", [71, 72, 73, 143, 144, 145])
+@pytest.mark.parametrize("empty", [0, 3])
+def test_clip_launches(dev, count, empty):
+    """Matrices that fill one launch or two of 72 exactly, and one less and more; empty ones take no place."""
+    xs = clip_case(torch.float32, dev, [(1 + 7 * i % 23, 1 + i % 11) for i in range(count)], 1.0)
+    s, f = clip_want(xs, 2.0)
+    no = clip_case(torch.float32, dev, [(0, 4), (5, 0), (0, 0)][:empty])
+    a = [mat(x) for x in no[:1] + xs[:50] + no[1:] + xs[50:]]
+    ys = [torch.full_like(x, float("nan")) for x in xs]
+    b = [mat(y) for y in no[:1] + ys[:50] + no[1:] + ys[50:]]
+    for got in (sl.clip_norm(2.0, a, b), sl.clip_norm(2.0, a)):
+        # the squares of 24 bits are exact in 53, their sum of n terms is off by n halves of an ulp
+        n = sum(x.numel() for x in xs)
+        assert abs(float(got) - s) <= (n + 4) * 2.0 ** -53 * s
+    for x, y, was in zip(xs, ys, clip_case(torch.float32, dev, [(1 + 7 * i % 23, 1 + i % 11) for i in range(count)], 1.0)):
+        want = was.double() * f
+        assert ((y.double() - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all()
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("src", TYPES)
+@pytest.mark.parametrize("dst", TYPES)
+@pytest.mark.parametrize("uplo", ["L", "U"])
+@pytest.mark.parametrize("trans", ["N", "T"])
+def test_copy_half_triangle(dev, src, dst, uplo, trans):
+    """One triangle's copy to and from the 16-bit types; the other keeps its elements."""
+    if src not in HALF and dst not in HALF:
+        pytest.skip("the other kernels")
+    for m, n in ((67, 45), (300, 33), (33, 300), (1, 5), (5, 1)):
+        x = cm(*((m, n) if trans == "N" else (n, m)), src, 3, dev)
+        y = cm(m, n, dst, 4, dev, 1.0, 3)
+        keep = y.clone()
+        ops.gecopy(x, y, uplo, trans)
+        want = (x if trans == "N" else x.t()).cpu().to(dst)
+        tri = torch.ones(m, n).tril().bool() if uplo == "L" else torch.ones(m, n).triu().bool()
+        assert torch.equal(y.cpu(), torch.where(tri, want, keep.cpu()))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("src,dst", [(torch.float32, torch.bfloat16), (torch.float16, torch.float64), (torch.bfloat16,) * 2])
+def test_copy_half_kinds(dev, src, dst):
+    """sl.copy of triangular and Hermitian matrices to and from the 16-bit types."""
+    for uplo in (sl.Uplo.Lower, sl.Uplo.Upper):
+        for kind in (sl.TriangularMatrix, sl.HermitianMatrix):
+            x, y = cm(45, 45, src, 3, dev), cm(45, 45, dst, 4, dev)
+            keep = y.clone()
+            sl.copy(kind(uplo, mat(x, nb=16)), kind(uplo, mat(y, nb=16)))
+            tri = torch.ones(45, 45).tril().bool()
+            tri = tri if uplo == sl.Uplo.Lower else tri.t()
+            assert torch.equal(y.cpu(), torch.where(tri, x.cpu().to(dst), keep.cpu()))
