@@ -129,6 +129,7 @@ class Option(enum.IntEnum):
     # MI355X extensions
     UseGraph = 100        # capture the factorization DAG into a hipGraph
     PanelStreamPriority = 101
+    PreciseGradient = 102 # 16-bit backward passes: the gradient between two products in two parts
 
 
 class LayoutConvert(_CharEnum):

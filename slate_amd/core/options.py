@@ -42,6 +42,7 @@ DEFAULTS = {
     Option.PrintWidth: 10,
     Option.PrintPrecision: 4,
     Option.UseGraph: False,
+    Option.PreciseGradient: False,
 }
 
 

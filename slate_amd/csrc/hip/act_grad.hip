@@ -3,8 +3,9 @@
 //   dZ  = dC o act'(Z), db = row (or column) sums of dZ
 // Memory bound: each of dC, Z1, Z2 is read once and dZ1, dZ2 written once, in
 // 16-byte accesses where rows allow it.  dZ is rounded to the operands' type,
-// which the MFMA of the two products that read it takes; the bias gradient
-// sums the unrounded values in 32 (64) bits, per chunk in registers, the
+// which the MFMA of the two products that read it takes, and, where the caller
+// wants it, what that rounding leaves over as a second matrix of the type; the
+// bias gradient sums the unrounded values in 32 (64) bits, per chunk in registers, the
 // chunks in order: no atomics, the same result on every run.  4096 x 8192 bf16:
 // 48 us plain (4.2 TB/s), 65 us gated (5.2 TB/s).
 #include "gemm_act.hpp"
@@ -12,6 +13,12 @@
 namespace slate_hip {
 
 namespace {
+
+// d less its rounding to T (an infinity or a NaN is whole in the rounded value)
+template <typename T, typename R> __device__ inline R ag_rest(R d) {
+    const R h = (R)(T)d;
+    return fabs(h) < (R)__builtin_huge_val() ? d - h : R(0);
+}
 
 // grid.x: blocks of E 2^tx rows (bias_mode 0, 1), grid.y: chunks of columns; the
 // 256 threads lie 2^tx along the rows and 256 / 2^tx along the columns, so that
@@ -56,6 +63,13 @@ __global__ void __launch_bounds__(256) act_grad_rows_kernel(ActGradArgs a, i64 c
             for (int e = 0; e < E; ++e) if (e < left) x[e] = (T)v[e];
         }
     };
+    // what their rounding leaves over
+    auto rest = [&](void* p, i64 n, const R* v) {
+        R y[E];
+        #pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = ag_rest<T>(v[e]);
+        put(p, n, y);
+    };
     // UN columns' loads are in flight per thread: 4096 x 8192 bf16 48 us with one
     // (two: 51, four: 54), gated 64 us with two (one: 71)
     constexpr int UN = GATED ? 2 : 1;
@@ -73,6 +87,10 @@ __global__ void __launch_bounds__(256) act_grad_rows_kernel(ActGradArgs a, i64 c
         }
         if (a.dZ1) put(a.dZ1, n, d1);
         if constexpr (GATED) put(a.dZ2, n, d2);
+        if constexpr (sizeof(T) == 2) {
+            if (a.dL1) rest(a.dL1, n, d1);
+            if (GATED && a.dL2) rest(a.dL2, n, d2);
+        }
     };
     if (left > 0)
         for (i64 n = n0 + w; n < n1; n += ny * UN) {
@@ -128,6 +146,8 @@ __global__ void __launch_bounds__(256) act_grad_cols_kernel(ActGradArgs a, i64 r
         }
         const R g = (R) static_cast<const T*>(a.dC)[m + n * a.lddc] * d;
         if (a.dZ1) static_cast<T*>(a.dZ1)[m + n * a.lddz] = (T)g;
+        if constexpr (sizeof(T) == 2)
+            if (a.dL1) static_cast<T*>(a.dL1)[m + n * a.lddz] = (T)ag_rest<T>(g);
         s += g;
     }
     s = wave_sum(s);

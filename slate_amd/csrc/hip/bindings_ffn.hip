@@ -46,14 +46,16 @@ int bytes_of(char t) { return t == 'd' ? 8 : t == 's' ? 4 : 2; }
 
 // A backward pass: dZ (and the bias gradient), then the products that read it.
 // v: rows, columns, act, dC, ldc, Z1, ldz1, Z2, ldz2, db, incb, bias_mode, how many
-// dZ are made; then 18 integers for each product: mode, op(A) and op(B) transposed,
-// m, n, k and address and leading dimension of A, A2, B, B2, C, C2, where the
-// addresses -1 and -2 are the dZ made here.  The workspace holds them, the bias
+// dZ are made, whether with what their rounding leaves over, and T; then 10 + 4 T
+// integers for each product: mode, op(A) and op(B) transposed, m, n, k and address
+// and leading dimension of T matrices A, T matrices B, C and C2, where the address
+// -1 - i is the i-th dZ made here (the rests behind them).  The workspace holds them, the bias
 // gradient's partial sums, and behind them what one product after the other wants.
 // -> its size; without one nothing is launched.
 template <typename T> i64 ffn_grad(double alpha, const std::vector<i64>& v, char* ws, hipStream_t s) {
-    constexpr size_t HEAD = 13, PER = 18;
-    if (v.size() < HEAD || (v.size() - HEAD) % PER) throw std::invalid_argument("ffn_grad: 13 + 18 n integers are wanted");
+    constexpr size_t HEAD = 15;
+    const size_t T_ = v.size() < HEAD ? 0 : (size_t)v[14], PER = 10 + 4 * T_;
+    if (T_ < 2 || T_ > 4 || (v.size() - HEAD) % PER) throw std::invalid_argument("ffn_grad: 15 + (10 + 4 T) n integers are wanted");
     auto round = [](i64 x, i64 to) { return (x + to - 1) / to * to; };
     ActGradArgs g;
     g.m = v[0]; g.n = v[1]; g.act = (int)v[2];
@@ -61,7 +63,7 @@ template <typename T> i64 ffn_grad(double alpha, const std::vector<i64>& v, char
     g.Z1 = P((uintptr_t)v[5]); g.ldz1 = v[6];
     g.Z2 = P((uintptr_t)v[7]); g.ldz2 = v[8];
     g.db = W((uintptr_t)v[9]); g.incb = v[10]; g.bias_mode = (int)v[11];
-    const int ndz = (int)v[12];
+    const int made = (int)v[12], ndz = v[13] ? 2 * made : made;
     g.lddz = round(std::max<i64>(g.m, 1), g.m >= 64 ? 64 : 8);
     const i64 dz = round(g.lddz * g.n * (i64)sizeof(T), 256);
     const i64 sums = g.bias_mode ? (i64)act_grad_chunks(g.bias_mode, sizeof(T), g.m, g.n) * (g.bias_mode == 1 ? g.m : g.n) *
@@ -70,8 +72,10 @@ template <typename T> i64 ffn_grad(double alpha, const std::vector<i64>& v, char
     // (an address to plan with: as aligned as the workspace's)
     char* base = ws ? ws : reinterpret_cast<char*>(4096);
     if (ws && (ndz || g.bias_mode)) {
-        if (ndz > 0) g.dZ1 = base;
-        if (ndz > 1) g.dZ2 = base + dz;
+        if (made > 0) g.dZ1 = base;
+        if (made > 1) g.dZ2 = base + dz;
+        if (ndz > made) g.dL1 = base + made * dz;
+        if (ndz > made && made > 1) g.dL2 = base + 3 * dz;
         g.part = base + ndz * dz;
         act_grad<T>(g, s);
     }
@@ -84,15 +88,19 @@ template <typename T> i64 ffn_grad(double alpha, const std::vector<i64>& v, char
         a.m = x[3]; a.n = x[4]; a.k = x[5];
         auto at = [&](int j, i64& ld) -> void* {
             ld = x[j + 1];
-            if (x[j] >= 0 || x[j] < -2) return W((uintptr_t)x[j]);
+            if (x[j] >= 0 || x[j] < -ndz) return W((uintptr_t)x[j]);
             ld = g.lddz;
-            return base + (x[j] == -2 ? dz : 0);
+            return base + (-1 - x[j]) * dz;
         };
-        for (int j = 0; j < 2; ++j) {
+        const int nt = (int)T_;
+        for (int j = 0; j < nt; ++j) {
             a.A[j] = at(6 + 2 * j, a.lda[j]);
-            a.B[j] = at(10 + 2 * j, a.ldb[j]);
-            a.C[j] = W((uintptr_t)x[14 + 2 * j]);
-            a.ldc[j] = x[15 + 2 * j];
+            a.B[j] = at(6 + 2 * nt + 2 * j, a.ldb[j]);
+            if (x[6 + 2 * j]) a.terms = j + 1;
+        }
+        for (int j = 0; j < 2; ++j) {
+            a.C[j] = W((uintptr_t)x[6 + 4 * nt + 2 * j]);
+            a.ldc[j] = x[7 + 4 * nt + 2 * j];
         }
         a.part = base + rest;
         a.plan = !ws;
@@ -110,12 +118,21 @@ void register_ffn(py::module& m) {
                          uintptr_t A0, i64 lda0, uintptr_t A1, i64 lda1, uintptr_t B0, i64 ldb0, uintptr_t B1, i64 ldb1,
                          uintptr_t C0, i64 ldc0, uintptr_t C1, i64 ldc1, uintptr_t bias, i64 incb, int bias_mode,
                          int act, double beta, uintptr_t R, i64 ldr, uintptr_t Z0, i64 ldz0, uintptr_t Z1, i64 ldz1,
-                         uintptr_t ws, uintptr_t st) {
+                         const py::list& more, uintptr_t ws, uintptr_t st) {
         GemmActArgs a;
         a.m = mm; a.n = n; a.k = k;
         a.mode = mode; a.alpha = alpha; a.beta = beta; a.act = act;
         a.A[0] = P(A0); a.lda[0] = lda0; a.A[1] = P(A1); a.lda[1] = lda1;
         a.B[0] = P(B0); a.ldb[0] = ldb0; a.B[1] = P(B1); a.ldb[1] = ldb1;
+        a.terms = mode == GA_SUM ? 2 : 1;
+        if (PyList_GET_SIZE(more.ptr())) {          // a sum's third and fourth product: A, lda, B, ldb each
+            const auto x = ints(more);
+            if (mode != GA_SUM || x.size() % 4 || x.size() > 8) throw std::invalid_argument("gemm_act: a sum has up to four products");
+            for (size_t i = 0; i < x.size(); i += 4, ++a.terms) {
+                a.A[a.terms] = P((uintptr_t)x[i]); a.lda[a.terms] = x[i + 1];
+                a.B[a.terms] = P((uintptr_t)x[i + 2]); a.ldb[a.terms] = x[i + 3];
+            }
+        }
         a.C[0] = W(C0); a.ldc[0] = ldc0; a.C[1] = W(C1); a.ldc[1] = ldc1;
         a.Z[0] = W(Z0); a.ldz[0] = ldz0; a.Z[1] = W(Z1); a.ldz[1] = ldz1;
         a.bias = P(bias); a.incb = incb; a.bias_mode = bias_mode;
@@ -137,12 +154,12 @@ void register_ffn(py::module& m) {
         return bytes;
     });
     m.def("act_grad", [](char dt, i64 mm, i64 n, int act, uintptr_t dC, i64 lddc, uintptr_t Z1, i64 ldz1, uintptr_t Z2,
-                         i64 ldz2, uintptr_t dZ1, uintptr_t dZ2, i64 lddz, uintptr_t db, i64 incb, int bias_mode,
+                         i64 ldz2, uintptr_t dZ1, uintptr_t dZ2, uintptr_t dL1, uintptr_t dL2, i64 lddz, uintptr_t db, i64 incb, int bias_mode,
                          bool wide, uintptr_t ws, uintptr_t st) {
         ActGradArgs a;
         a.m = mm; a.n = n; a.act = act;
         a.dC = P(dC); a.lddc = lddc; a.Z1 = P(Z1); a.ldz1 = ldz1; a.Z2 = P(Z2); a.ldz2 = ldz2;
-        a.dZ1 = W(dZ1); a.dZ2 = W(dZ2); a.lddz = lddz;
+        a.dZ1 = W(dZ1); a.dZ2 = W(dZ2); a.dL1 = W(dL1); a.dL2 = W(dL2); a.lddz = lddz;
         a.db = W(db); a.incb = incb; a.bias_mode = bias_mode; a.wide = wide;
         a.part = W(ws);
         if (bias_mode && !ws) throw std::invalid_argument("act_grad: workspace missing");

@@ -11,16 +11,17 @@ enum : int { GA_PLAIN = 0, GA_GATED = 1, GA_SUM = 2, GA_PAIR = 3 };
 // ---------------------------------------------------------------- arguments
 struct GemmActArgs {
     i64 m = 0, n = 0, k = 0;
-    const void* A[2] = {nullptr, nullptr};
-    const void* B[2] = {nullptr, nullptr};
+    const void* A[4] = {};
+    const void* B[4] = {};
     void* C[2] = {nullptr, nullptr};
     void* Z[2] = {nullptr, nullptr};
-    i64 lda[2] = {0, 0}, ldb[2] = {0, 0}, ldc[2] = {0, 0}, ldz[2] = {0, 0};
+    i64 lda[4] = {}, ldb[4] = {}, ldc[2] = {0, 0}, ldz[2] = {0, 0};
     const void* bias = nullptr;
     const void* R = nullptr;
     i64 incb = 1, ldr = 0;
     double alpha = 1, beta = 0;
     int mode = GA_PLAIN;
+    int terms = 1;          // GA_SUM: how many products are added (2 to 4)
     int bias_mode = 0;      // 0 none, 1 one value per row of C, 2 one per column
     int act = ACT_IDENTITY;
     // filled by the launcher
@@ -37,17 +38,18 @@ struct GemmActArgs {
 // Which kernel, and in how many pieces K: from sizes, types and alignment alone.
 // tile -1: the kernel for few columns; bytes: workspace.
 struct GemmActPlan { int tile = 0, splits = 1, per_split = 0; i64 ldp = 0, bytes = 0; };
-GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool bkc, bool dma);
-bool gemm_act_pack(int mode, i64 m, i64 n, i64 k);    // lay operands whose rows lie across 16 bytes out anew?
+GemmActPlan gemm_act_plan(int es, int mode, int terms, i64 m, i64 n, i64 k, bool akc, bool bkc, bool dma);
+bool gemm_act_pack(int mode, int terms, i64 m, i64 n, i64 k);    // lay operands whose rows lie across 16 bytes out anew?
 // Launches and returns 0, or returns the workspace wanted where part is null.
 template <typename T> i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s);
 
 // dZ = dC o act'(Z) (dZ1 = dC o Z2 o act'(Z1), dZ2 = dC o act(Z1) where Z2 is
-// given), and the sums of dZ over the columns (bias_mode 1) or rows (2)
+// given), and the sums of dZ over the columns (bias_mode 1) or rows (2).  Where
+// dL1 (dL2) is given, 16-bit types: what the rounding of dZ left over, rounded
 struct ActGradArgs {
     i64 m = 0, n = 0;
     const void *dC = nullptr, *Z1 = nullptr, *Z2 = nullptr;
-    void *dZ1 = nullptr, *dZ2 = nullptr;
+    void *dZ1 = nullptr, *dZ2 = nullptr, *dL1 = nullptr, *dL2 = nullptr;
     i64 lddc = 0, ldz1 = 0, ldz2 = 0, lddz = 0;
     void* db = nullptr;
     i64 incb = 1;

@@ -1,6 +1,7 @@
 // Matrix products with a fused epilogue for gfx950 (bf16, f16, f32, f64):
 //
-//   plain   Z = alpha sum_p op(A_p) op(B_p) + bias,  C = act(Z) + beta R
+//   plain   Z = alpha op(A) op(B) + bias,            C = act(Z) + beta R
+//   sum     C = alpha sum_p op(A_p) op(B_p)          (two to four products)
 //   gated   Z_i = op(A_i) op(B),                     C = act(Z_1) o Z_2
 //   pair    C_i = alpha op(A_i) op(B_i)              (two products, one launch)
 //
@@ -488,12 +489,12 @@ __global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs
     const int inner = lin - grp * G * gn;
     const i64 m0 = (i64)(first + inner % gsz) * BMI, n0 = (i64)(inner / gsz) * BN;
     const int pair = a.mode == GA_PAIR ? blockIdx.z : 0;
-    const int total = a.nsteps * (a.mode == GA_SUM ? 2 : 1);
+    const int total = a.nsteps * a.terms;
     const int s0 = a.splits > 1 ? (int)blockIdx.y * a.per_split : 0;
     const int s1 = a.splits > 1 ? min(total, s0 + a.per_split) : total;
 
     const i64 rowsA = a.m - m0, rowsB = a.n - n0;
-    const bool sum = a.mode == GA_SUM;
+    const bool sum = a.terms > 1;
     auto slabA = [&](int q, i64 k0) { return static_cast<const T*>(a.A[q]) + (AKC ? m0 * a.lda[q] + k0 : m0 + k0 * a.lda[q]); };
     auto slabB = [&](int q, i64 k0) { return static_cast<const T*>(a.B[q]) + (BKC ? n0 * a.ldb[q] + k0 : n0 + k0 * a.ldb[q]); };
 
@@ -521,13 +522,13 @@ __global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs
         #pragma unroll
         for (int i = 0; i < PB; ++i) offB[i] = IB::template offset<W>(min(wid + i * NW, PCB - 1), lane, ld, rowsB);
     };
-    int curp = sum ? (s0 >= nsteps ? 1 : 0) : pair;
-    int kt = sum && s0 >= nsteps ? s0 - nsteps : s0;      // step of its product being staged
+    int curp = pair, kt = s0;                             // product, and its step being staged
+    while (curp + 1 < a.terms && kt >= nsteps) { kt -= nsteps; ++curp; }
     if constexpr (DMA) aim(curp, (i64)kt * KB);
 
     // stages one step after the other
     auto issue = [&](char* slot) {
-        if (sum && kt == nsteps) { kt = 0; curp = 1; aim(1, 0); }
+        if (sum && kt == nsteps) { kt = 0; aim(++curp, 0); }
         const i64 k0 = (i64)kt++ * KB;
         if (k0 < kfull) {
             #pragma unroll
@@ -586,7 +587,7 @@ __global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs
     if constexpr (!DMA) point(curp, (i64)kt * KB);
     // (after the last slab it reads that one again)
     auto fetch = [&](Held& x) {
-        if (sum && kt == nsteps) { kt = 0; curp = 1; point(1, 0); }
+        if (sum && kt == nsteps) { kt = 0; point(++curp, 0); }
         const int lA = (int)min(kA - (i64)kt * KB, (i64)KB), lB = (int)min(kB - (i64)kt * KB, (i64)KB);
         x.whole = lA == KB && lB == KB && (AKC || availA >= BMI) && (BKC || availB >= BN);
         #pragma unroll

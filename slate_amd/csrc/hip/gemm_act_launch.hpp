@@ -104,13 +104,14 @@ template <typename T>
 i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
     constexpr int ES = sizeof(T), E = 16 / ES, KB = 128 / ES;
     if (a.m <= 0 || a.n <= 0) return 0;
+    if (a.mode != GA_SUM) a.terms = 1;
     const bool gated = a.mode == GA_GATED, akc = ta != 'N', bkc = tb == 'N';
-    const int na = a.mode == GA_PLAIN ? 1 : 2, nb = a.mode == GA_SUM || a.mode == GA_PAIR ? 2 : 1;
+    const int na = a.mode == GA_SUM ? a.terms : a.mode == GA_PLAIN ? 1 : 2, nb = a.mode == GA_SUM ? a.terms : a.mode == GA_PAIR ? 2 : 1;
     // LDS-DMA moves 16 bytes from 16-byte-aligned addresses at 32-bit offsets
     // inside a tile; a slab whose last vector would pass the end of the last
     // column goes through registers, as the ragged end of K does
     bool dma = true, small = true;       // 32-bit offsets: `small`
-    GaOperand op[4];
+    GaOperand op[8];
     int nop = 0;
     auto look = [&](const void*& q, i64& ld, bool kc, i64 rows) {
         GaOperand x{&q, &ld, kc ? a.k : rows, kc ? rows : a.k, kc};
@@ -122,8 +123,8 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
     };
     for (int i = 0; i < na; ++i) look(a.A[i], a.lda[i], akc, a.m);
     for (int i = 0; i < nb; ++i) look(a.B[i], a.ldb[i], bkc, a.n);
-    const bool pack = ES == 2 && !dma && gemm_act_pack(a.mode, a.m, a.n, a.k) && ga_packed(op, nop, ES);
-    const GemmActPlan p = gemm_act_plan(ES, a.mode, a.m, a.n, a.k, akc, bkc, dma || pack);
+    const bool pack = ES == 2 && !dma && gemm_act_pack(a.mode, a.terms, a.m, a.n, a.k) && ga_packed(op, nop, ES);
+    const GemmActPlan p = gemm_act_plan(ES, a.mode, a.terms, a.m, a.n, a.k, akc, bkc, dma || pack);
     if (p.tile < 0) {
         if (!a.plan) ga_skinny<T>(a, gated, s);
         return 0;

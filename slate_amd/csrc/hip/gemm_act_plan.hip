@@ -9,8 +9,8 @@ namespace slate_hip {
 // against 362 us, 512 x 4096 x 4096 47 against 61, 2000^3 51 against 52; where
 // the operands are long for what is computed, or small, it loses: 4096 x 128 x
 // 4096 35 against 28 us, 1000^3 20 against 15.
-bool gemm_act_pack(int mode, i64 m, i64 n, i64 k) {
-    return (mode == GA_PLAIN ? 1 : 2) * m * n * k >= 8000000000 && m * n >= 256 * (m + n);
+bool gemm_act_pack(int mode, int terms, i64 m, i64 n, i64 k) {
+    return (mode == GA_PLAIN ? 1 : mode == GA_SUM ? terms : 2) * m * n * k >= 8000000000 && m * n >= 256 * (m + n);
 }
 
 namespace {
@@ -58,7 +58,7 @@ double ga_time(const GaCost& c, i64 wgs, int steps) {
 
 }  // namespace
 
-GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool bkc, bool dma) {
+GemmActPlan gemm_act_plan(int es, int mode, int terms, i64 m, i64 n, i64 k, bool akc, bool bkc, bool dma) {
     GemmActPlan p;
     // Up to 16 columns and both operands along k: 4096 x 4096 bf16 times one
     // column 8.6 us against 14.9 us of the tiles with K split (16 columns of
@@ -75,7 +75,7 @@ GemmActPlan gemm_act_plan(int es, int mode, i64 m, i64 n, i64 k, bool akc, bool 
         return p;
     }
     const i64 rows = mode == GA_GATED ? 2 * m : m, pairs = mode == GA_PAIR ? 2 : 1;
-    const int steps = std::max<int>(1, (int)((k * es + 127) / 128) * (mode == GA_SUM ? 2 : 1));
+    const int steps = std::max<int>(1, (int)((k * es + 127) / 128) * terms);
     auto tiles = [&](i64 bm, i64 bn) { return ((rows + bm - 1) / bm) * ((n + bn - 1) / bn) * pairs; };
     if (n > 16) {
         // The tile and the pieces of K (4 steps or more) with the least time by

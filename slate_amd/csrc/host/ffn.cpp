@@ -190,13 +190,20 @@ void register_ffn(py::module& m) {
                          uintptr_t A0, i64 lda0, uintptr_t A1, i64 lda1, uintptr_t B0, i64 ldb0, uintptr_t B1, i64 ldb1,
                          uintptr_t C0, i64 ldc0, uintptr_t C1, i64 ldc1, uintptr_t bias, i64 incb, int bias_mode,
                          int act, double beta, uintptr_t R, i64 ldr, uintptr_t Z0, i64 ldz0, uintptr_t Z1, i64 ldz1,
-                         uintptr_t, uintptr_t) {
+                         const std::vector<i64>& more, uintptr_t, uintptr_t) {
+        if (more.size() % 4 || (mode != SUM && !more.empty())) throw std::invalid_argument("gemm_act: bad terms of a sum");
         real_dispatch(dt, [&](auto z) {
             using T = decltype(z);
-            const uintptr_t A[2] = {A0, A1}, B[2] = {B0, B1}, C[2] = {C0, C1}, Z[2] = {Z0, Z1};
-            const i64 lda[2] = {lda0, lda1}, ldb[2] = {ldb0, ldb1}, ldc[2] = {ldc0, ldc1}, ldz[2] = {ldz0, ldz1};
+            std::vector<uintptr_t> A = {A0, A1}, B = {B0, B1};
+            std::vector<i64> lda = {lda0, lda1}, ldb = {ldb0, ldb1};
+            for (size_t i = 0; i < more.size(); i += 4) {
+                A.push_back((uintptr_t)more[i]); lda.push_back(more[i + 1]);
+                B.push_back((uintptr_t)more[i + 2]); ldb.push_back(more[i + 3]);
+            }
+            const uintptr_t C[2] = {C0, C1}, Z[2] = {Z0, Z1};
+            const i64 ldc[2] = {ldc0, ldc1}, ldz[2] = {ldz0, ldz1};
             std::vector<double> D[2];
-            const int outs = mode == GATED || mode == PAIR ? 2 : 1, sums = mode == SUM ? 2 : 1;
+            const int outs = mode == GATED || mode == PAIR ? 2 : 1, sums = mode == SUM ? (int)A.size() : 1;
             for (int h = 0; h < outs; ++h) {
                 D[h].assign((size_t)(m * n), 0.0);
                 for (int p = 0; p < sums; ++p) {
@@ -228,7 +235,7 @@ void register_ffn(py::module& m) {
     });
     m.def("act_grad_ws", [](char, int, i64, i64) { return (i64)0; });
     m.def("act_grad", [](char dt, i64 m, i64 n, int act, uintptr_t dC, i64 lddc, uintptr_t Z1, i64 ldz1, uintptr_t Z2,
-                         i64 ldz2, uintptr_t dZ1, uintptr_t dZ2, i64 lddz, uintptr_t db, i64 incb, int bias_mode,
+                         i64 ldz2, uintptr_t dZ1, uintptr_t dZ2, uintptr_t dL1, uintptr_t dL2, i64 lddz, uintptr_t db, i64 incb, int bias_mode,
                          bool wide, uintptr_t, uintptr_t) {
         real_dispatch(dt, [&](auto z) {
             using T = decltype(z);
@@ -241,6 +248,10 @@ void register_ffn(py::module& m) {
                     const double d1 = Z2 ? g * (double)ptr<const T>(Z2)[i + j * ldz2] * d : g * d;
                     if (dZ1) ptr<T>(dZ1)[i + j * lddz] = put<T>(d1);
                     if (dZ2) ptr<T>(dZ2)[i + j * lddz] = put<T>(g * v);
+                    // what their rounding leaves over (nothing of an infinity or a NaN)
+                    auto rest = [](double d) { const double h = (double)put<T>(d); return put<T>(std::isfinite(h) ? d - h : 0.0); };
+                    if (dL1) ptr<T>(dL1)[i + j * lddz] = rest(d1);
+                    if (dL2) ptr<T>(dL2)[i + j * lddz] = rest(g * v);
                     if (bias_mode) sum[(size_t)(bias_mode == 1 ? i : j)] += d1;
                 }
             for (size_t i = 0; i < sum.size(); ++i) {

@@ -33,8 +33,9 @@ import torch
 
 from .. import ops
 from .._native import REAL_CODE, kmod, raw_stream
-from ..core.enums import Activation, Op
+from ..core.enums import Activation, Op, Option
 from ..core.exceptions import SlateError
+from ..core.options import get_option
 from ..core.storage import DEV, debug_checks
 from ..utils.trace import trace_block
 from ._panels import col_bcast, row_bcast
@@ -47,6 +48,7 @@ _ACT.update({a.name.lower(): i for a, i in list(_ACT.items())})
 _BYTES = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4, torch.float64: 8, torch.complex64: 8, torch.complex128: 16}
 
 
+_HALF = (torch.bfloat16, torch.float16)
 _DEVICES = {}          # one object per device, so that operands compare them by identity
 
 
@@ -322,8 +324,10 @@ class _on:
             self.ctx.__exit__(*e)
 
 
-def _launch(mode, alpha, A1, A2, B1, B2, C1, C2, bias=_NONE, bias_mode=0, act=0, beta=0.0, R=_NONE, Z1=_NONE, Z2=_NONE):
-    """One rank's product(s); outputs, R and Z not transposed."""
+def _launch(mode, alpha, A1, A2, B1, B2, C1, C2, bias=_NONE, bias_mode=0, act=0, beta=0.0, R=_NONE, Z1=_NONE, Z2=_NONE,
+            more=()):
+    """One rank's product(s); outputs, R and Z not transposed; more: the third and
+    fourth operands (A, B) of a sum."""
     t = C1.t
     m, n, k = C1.rows, C1.cols, A1.n
     if m == 0 or n == 0:
@@ -333,11 +337,11 @@ def _launch(mode, alpha, A1, A2, B1, B2, C1, C2, bias=_NONE, bias_mode=0, act=0,
     if beta == 0:
         R = _NONE
     if ops._FLOPS is not None:
-        ops._FLOPS[0] += 2 * m * n * k * (1 if mode == PLAIN else 2)
+        ops._FLOPS[0] += 2 * m * n * k * (1 if mode == PLAIN else 2 + len(more))
     call = kmod(t).gemm_act
     args = (REAL_CODE[t.dtype], mode, A1.op, B1.op, m, n, k, alpha, A1.ptr, A1.ld, A2.ptr, A2.ld, B1.ptr, B1.ld,
             B2.ptr, B2.ld, C1.ptr, C1.ld, C2.ptr, C2.ld, bias.ptr, _inc(bias), bias_mode, act, beta, R.ptr, R.ld,
-            Z1.ptr, Z1.ld, Z2.ptr, Z2.ld)
+            Z1.ptr, Z1.ld, Z2.ptr, Z2.ld, [i for a, b in more for i in (a.ptr, a.ld, b.ptr, b.ld)])
     st = raw_stream(t)
     nbytes = call(*args, 0, st)
     if nbytes:                                  # few tiles: partial sums of pieces of k
@@ -449,17 +453,20 @@ def _run_dist(mode, alpha, A, B, C, bias=None, bias_mode=0, act=0, beta=0.0, R=N
     Zw = [None if z is None else (z if _placed(z, W[0]) else _grid_work(W[0], z.m(), z.n())) for z in Z]
     Rw = None if R is None or beta == 0 else _onto(R, W[0])
     if alpha != 0:
-        As = [_gather_k(a, W[0], True) for a in A]
-        Bs = [_gather_k(b, W[0], False) for b in B]
+        # (the terms of a sum may share operands: each is gathered once)
+        As = {id(a): _gather_k(a, W[0], True) for a in {id(a): a for a in A}.values()}
+        Bs = {id(b): _gather_k(b, W[0], False) for b in {id(b): b for b in B}.values()}
+        As, Bs = [As[id(a)] for a in A], [Bs[id(b)] for b in B]
     else:
         lb = W[0].local_block()
         As, Bs = [_like(_opd(W[0]), lb.mloc, 0)], [_like(_opd(W[0]), 0, lb.nloc)]
     b = _NONE if bias is None else _vector(bias, bias_mode, W[0])
     if grid_rank:
+        more = list(zip(As[2:], Bs[2:]))
         As, Bs, Ws = ((x + [_NONE])[:2] for x in (As, Bs, [_opd(w) for w in W]))
         with _on(Ws[0].t):
             _launch(mode, alpha, *As, *Bs, *Ws, b, bias_mode, act, beta, _NONE if Rw is None else _opd(Rw),
-                    *[_NONE if z is None else _opd(z) for z in Zw])
+                    *[_NONE if z is None else _opd(z) for z in Zw], more=more)
     _modified(*W, *Zw)
     for w, c in zip(list(W) + Zw, list(C) + list(Z)):
         if w is not None and w is not c:
@@ -560,8 +567,9 @@ def gemm_gated(A1, A2, B, act, C, Z1=None, Z2=None, opts=None):
 
 
 # ----------------------------------------------------------------- gradients
-def _act_grad(m, n, act, dC, Z1, Z2, dZ1, dZ2, db=_NONE, bias_mode=0, wide=False):
-    """One rank's elementwise pass; operands not transposed."""
+def _act_grad(m, n, act, dC, Z1, Z2, dZ1, dZ2, db=_NONE, bias_mode=0, wide=False, rest=(_NONE, _NONE)):
+    """One rank's elementwise pass; operands not transposed; rest: for what the
+    rounding of dZ1 and dZ2 leaves over."""
     t = dC.t
     if m == 0 or n == 0:
         if db.t is not None:
@@ -570,32 +578,39 @@ def _act_grad(m, n, act, dC, Z1, Z2, dZ1, dZ2, db=_NONE, bias_mode=0, wide=False
     mod, dt = kmod(t), REAL_CODE[t.dtype]
     nbytes = mod.act_grad_ws(dt, bias_mode, m, n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
-    mod.act_grad(dt, m, n, act, dC.ptr, dC.ld, Z1.ptr, Z1.ld, Z2.ptr, Z2.ld, dZ1.ptr, dZ2.ptr, dZ1.ld,
-                 db.ptr, _inc(db), bias_mode, wide, 0 if ws is None else ws.data_ptr(), raw_stream(t))
+    mod.act_grad(dt, m, n, act, dC.ptr, dC.ld, Z1.ptr, Z1.ld, Z2.ptr, Z2.ld, dZ1.ptr, dZ2.ptr,
+                 rest[0].ptr, rest[1].ptr, dZ1.ld, db.ptr, _inc(db), bias_mode, wide, 0 if ws is None else ws.data_ptr(), raw_stream(t))
 
 
 class _Made:
-    """Stands for a dZ in the workspace of :func:`_grad_run`."""
+    """Stands for a dZ, or what its rounding leaves over, in the workspace of :func:`_grad_run`."""
     __slots__ = ("ptr", "ld")
 
     def __init__(self, ptr):
         self.ptr, self.ld = ptr, 0
 
 
-_DZ1, _DZ2 = _Made(-1), _Made(-2)
+_DZ = [_Made(-1 - i) for i in range(4)]
 
 
-def _step(steps, mode, k, a, at, b, bt, c, a2=_NONE, b2=_NONE, c2=_NONE):
-    """Adds a product op(a) op(b) into c, of either orientation, to steps; at and
-    bt: does the operand enter transposed?"""
+def _step(steps, mode, k, A, at, B, bt, c, c2=_NONE):
+    """Adds products op(A_i) op(B_i) into c, of either orientation, to steps; at
+    and bt: do the operands enter transposed?"""
     if c.t is None:
         return
     if ops._FLOPS is not None:
-        ops._FLOPS[0] += 2 * c.rows * c.cols * k * (1 if mode == PLAIN else 2)
+        ops._FLOPS[0] += 2 * c.rows * c.cols * k * len(A)
     if c.trans:
-        a, at, a2, b, bt, b2 = b, not bt, b2, a, not at, a2
-    steps += (mode, at, bt, c.rows, c.cols, k, a.ptr, a.ld, a2.ptr, a2.ld, b.ptr, b.ld, b2.ptr, b2.ld,
-              c.ptr, c.ld, c2.ptr, c2.ld)
+        A, at, B, bt = B, not bt, A, not at
+    steps += (mode, at, bt, c.rows, c.cols, k)
+    fill = [0, 0] * (steps[14] - len(A))
+    for x in A:
+        steps += (x.ptr, x.ld)
+    steps += fill
+    for x in B:
+        steps += (x.ptr, x.ld)
+    steps += fill
+    steps += (c.ptr, c.ld, c2.ptr, c2.ld)
 
 
 def _grad_run(alpha, oc, steps):
@@ -617,8 +632,11 @@ def gemm_bias_act_grad(alpha, A, B, act, Z, dC, dA, dB, dbias, opts=None):
     operand that entered transposed); None leaves a gradient out.  ``Z`` is what
     the forward pass stored (may be None for the identity).  The residual's
     gradient is beta dC.  dA, dB and dbias overlap no other matrix of the call.
-    dZ is rounded to the matrices' type between the two
-    steps, the bias gradient is summed from its unrounded values."""
+    dZ is rounded to the matrices' type between the two steps, the bias gradient
+    is summed from its unrounded values.  With Option.PreciseGradient, what the
+    rounding of a 16-bit dZ leaves over enters the products as a second matrix:
+    dA and dB are then off by little more than their own rounding (by 1.4 times
+    it without), for twice the operations."""
     what, mats = "gemm_bias_act_grad", (A, B, Z, dC, dA, dB, dbias)
     a = _act(act)
     if Z is None and a:
@@ -633,11 +651,11 @@ def gemm_bias_act_grad(alpha, A, B, act, Z, dC, dA, dB, dbias, opts=None):
             _apart(what, [("dA", dA), ("dB", dB), ("dbias", dbias)], [("A", A), ("B", B), ("Z", Z), ("dC", dC)],
                    None, not one)
             if not one:
-                dZ = _dz_dist(a, dC, (Z if a else None, None), dbias, bmode)[0]
+                dZ = _dz_dist(a, dC, (Z if a else None, None), dbias, bmode, _precise(opts, dC.dtype))
                 if dA is not None:
-                    _run_dist_any(PLAIN, alpha, [dZ], [_t(B)], [dA])
+                    _run_dist_any(PLAIN, alpha, dZ, [_t(B)] * len(dZ), [dA])
                 if dB is not None:
-                    _run_dist_any(PLAIN, alpha, [_t(A)], [dZ], [dB])
+                    _run_dist_any(PLAIN, alpha, [_t(A)] * len(dZ), dZ, [dB])
             if not one or dC.storage.bc.pr < 0:
                 return
         oa, ob, oz, oc, ga, gb, gv = _operands(what, ("A", "B", "Z", "dC", "dA", "dB", "dbias"), mats)
@@ -656,31 +674,45 @@ def gemm_bias_act_grad(alpha, A, B, act, Z, dC, dA, dB, dbias, opts=None):
                     mode = 3 - mode
             if oc.t.is_cuda and m and n:
                 made = dZ is None
-                if made:
-                    dZ = _DZ1
-                steps = [oc.rows, oc.cols, a, oc.ptr, oc.ld, oz.ptr, oz.ld, 0, 0, gv.ptr, _inc(gv), mode, made]
-                tr = oc.trans
-                _step(steps, PLAIN, n if alpha else 0, dZ, tr, ob, not ob.trans, ga)
-                _step(steps, PLAIN, m if alpha else 0, oa, not oa.trans, dZ, tr, gb)
+                two = made and _precise(opts, oc.dt)
+                dZ = (oc,) if not made else _DZ[:2] if two else _DZ[:1]
+                steps = [oc.rows, oc.cols, a, oc.ptr, oc.ld, oz.ptr, oz.ld, 0, 0, gv.ptr, _inc(gv), mode, made, two, 2]
+                tr, how = oc.trans, SUM if two else PLAIN
+                _step(steps, how, n if alpha else 0, dZ, tr, (ob,) * len(dZ), not ob.trans, ga)
+                _step(steps, how, m if alpha else 0, (oa,) * len(dZ), not oa.trans, dZ, tr, gb)
                 _grad_run(alpha, oc, steps)
                 _modified(dA, dB, dbias)
                 return
-            if dZ is None:
+            made = dZ is None
+            if made:
                 dZ = _like(oc, oc.rows, oc.cols, oc.trans)
+            parts = [dZ]
+            if made and _precise(opts, oc.dt):
+                parts.append(_like(oc, oc.rows, oc.cols, oc.trans))
             if a or mode:
-                _act_grad(oc.rows, oc.cols, a, oc, oz, _NONE, _NONE if dZ is oc else dZ, _NONE, gv, mode)
+                _act_grad(oc.rows, oc.cols, a, oc, oz, _NONE, dZ if made else _NONE, _NONE, gv, mode,
+                          rest=(*parts[1:], _NONE, _NONE)[:2])
             if dA is not None:
-                _product(PLAIN, alpha, dZ, _NONE, ob.T, _NONE, ga, _NONE)
+                _product(PLAIN, alpha, parts, [ob.T] * len(parts), [ga])
             if dB is not None:
-                _product(PLAIN, alpha, oa.T, _NONE, dZ, _NONE, gb, _NONE)
+                _product(PLAIN, alpha, [oa.T] * len(parts), parts, [gb])
         _modified(dA, dB, dbias)
 
 
-def _product(mode, alpha, A1, A2, B1, B2, C1, C2):
-    """One rank's product(s) into outputs of either orientation."""
-    if C1.trans:
-        A1, A2, B1, B2, C1, C2 = (x if x is _NONE else x.T for x in (B1, B2, A1, A2, C1, C2))
-    _launch(mode, alpha, A1, A2, B1, B2, C1, C2)
+def _precise(opts, dt):
+    """Are the parts of dZ that 16 bits do not hold wanted?"""
+    return dt in _HALF and get_option(opts, Option.PreciseGradient, False)
+
+
+def _product(mode, alpha, A, B, C):
+    """One rank's product(s) op(A_i) op(B_i) into outputs of either orientation; those
+    of one output are added."""
+    if C[0].trans:
+        A, B, C = ([x.T for x in y] for y in (B, A, C))
+    if mode == PLAIN and len(A) > 1:
+        mode = SUM
+    (a1, a2), (b1, b2), (c1, c2) = ((*x, _NONE)[:2] for x in (A, B, C))
+    _launch(mode, alpha, a1, a2, b1, b2, c1, c2, more=list(zip(A[2:], B[2:])))
 
 
 def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
@@ -692,7 +724,8 @@ def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
     with Z1, Z2 as the forward pass stored them; None leaves a gradient out.
     dA1, dA2 and dB overlap no other matrix of the call.
     Both weight gradients are one launch, and dB is one sum over both products,
-    rounded once."""
+    rounded once.  dZ1 and dZ2 are rounded to the matrices' type;
+    Option.PreciseGradient as for :func:`gemm_bias_act_grad`."""
     what, mats = "gemm_gated_grad", (A1, A2, B, Z1, Z2, dC, dA1, dA2, dB)
     names = ("A1", "A2", "B", "Z1", "Z2", "dC", "dA1", "dA2", "dB")
     a = _act(act)
@@ -707,12 +740,12 @@ def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
             pairs = list(zip(names, mats))
             _apart(what, pairs[6:], pairs[:6], None, not one)
             if not one:
-                dZ = _dz_dist(a, dC, (Z1, Z2), None, 0)
-                for d, g in zip(dZ, (dA1, dA2)):
+                dZ = _dz_dist(a, dC, (Z1, Z2), None, 0, _precise(opts, dC.dtype))
+                for d, g in ((dZ[::2], dA1), (dZ[1::2], dA2)):
                     if g is not None:
-                        _run_dist_any(PLAIN, 1.0, [d], [_t(B)], [g])
+                        _run_dist_any(PLAIN, 1.0, d, [_t(B)] * len(d), [g])
                 if dB is not None:
-                    _run_dist_any(SUM, 1.0, [_t(A1), _t(A2)], dZ, [dB])
+                    _run_dist_any(SUM, 1.0, [_t(A1), _t(A2)] * (len(dZ) // 2), dZ, [dB])
             if not one or dC.storage.bc.pr < 0:
                 return
         o1, o2, ob, z1, z2, oc, g1, g2, gb = opds = _operands(what, names, mats)
@@ -731,39 +764,45 @@ def gemm_gated_grad(A1, A2, B, act, Z1, Z2, dC, dA1, dA2, dB, opts=None):
             if dB is not None and o2.trans != o1.trans:
                 o2 = _turn(o2, o1.trans)
             if oc.t.is_cuda and m and n:
-                steps = [oc.rows, oc.cols, a, oc.ptr, oc.ld, z1.ptr, z1.ld, z2.ptr, z2.ld, 0, 1, 0, 2]
-                if dA1 is not None and dA2 is not None and g1.trans == g2.trans:
-                    _step(steps, PAIR, n, _DZ1, tr, ob, not ob.trans, g1, _DZ2, ob, g2)
+                two = _precise(opts, oc.dt)
+                steps = [oc.rows, oc.cols, a, oc.ptr, oc.ld, z1.ptr, z1.ld, z2.ptr, z2.ld, 0, 1, 0, 2, two, 4 if two else 2]
+                if two:
+                    _step(steps, SUM, n, _DZ[::2], tr, (ob, ob), not ob.trans, g1)
+                    _step(steps, SUM, n, _DZ[1::2], tr, (ob, ob), not ob.trans, g2)
+                elif dA1 is not None and dA2 is not None and g1.trans == g2.trans:
+                    _step(steps, PAIR, n, _DZ[:2], tr, (ob, ob), not ob.trans, g1, g2)
                 else:
-                    _step(steps, PLAIN, n, _DZ1, tr, ob, not ob.trans, g1)
-                    _step(steps, PLAIN, n, _DZ2, tr, ob, not ob.trans, g2)
-                _step(steps, SUM, m, o1, not o1.trans, _DZ1, tr, gb, o2, _DZ2)
+                    _step(steps, PLAIN, n, _DZ[:1], tr, (ob,), not ob.trans, g1)
+                    _step(steps, PLAIN, n, _DZ[1:2], tr, (ob,), not ob.trans, g2)
+                _step(steps, SUM, m, (o1, o2, o1, o2) if two else (o1, o2), not o1.trans, _DZ if two else _DZ[:2], tr, gb)
                 _grad_run(1.0, oc, steps)
                 _modified(dA1, dA2, dB)
                 return
-            d1, d2 = _like(oc, oc.rows, oc.cols, tr), _like(oc, oc.rows, oc.cols, tr)
-            _act_grad(oc.rows, oc.cols, a, oc, z1, z2, d1, d2)
-            if dA1 is not None and dA2 is not None and g1.trans == g2.trans:
-                _product(PAIR, 1.0, d1, d2, ob.T, ob.T, g1, g2)
+            d = [_like(oc, oc.rows, oc.cols, tr) for _ in range(4 if _precise(opts, oc.dt) else 2)]
+            _act_grad(oc.rows, oc.cols, a, oc, z1, z2, d[0], d[1], rest=(*d[2:], _NONE, _NONE)[:2])
+            if dA1 is not None and dA2 is not None and g1.trans == g2.trans and len(d) == 2:
+                _product(PAIR, 1.0, d, [ob.T, ob.T], [g1, g2])
             else:
-                for d, g in ((d1, g1), (d2, g2)):
+                for x, g in ((d[::2], g1), (d[1::2], g2)):
                     if g.t is not None:
-                        _product(PLAIN, 1.0, d, _NONE, ob.T, _NONE, g, _NONE)
+                        _product(PLAIN, 1.0, x, [ob.T] * len(x), [g])
             if dB is not None:
-                _product(SUM, 1.0, o1.T, o2.T, d1, d2, gb, _NONE)
+                _product(SUM, 1.0, [o1.T, o2.T] * (len(d) // 2), d, [gb])
         _modified(dA1, dA2, dB)
 
 
 def _run_dist_any(mode, alpha, A, B, C):
-    """_run_dist into outputs of either orientation."""
+    """_run_dist into outputs of either orientation; products of one output are added."""
+    if mode == PLAIN and len(A) > 1:
+        mode = SUM
     if C[0]._op != Op.NoTrans:
         A, B, C = [_t(x) for x in B], [_t(x) for x in A], [_t(x) for x in C]
     _run_dist(mode, alpha, A, B, C)
 
 
-def _dz_dist(act, dC, Z, dbias, bmode):
-    """dZ (one or two matrices, from offset 0 on dC's grid) and the bias
-    gradient: local sums in 32 (64) bits, one all-reduce over the process row
+def _dz_dist(act, dC, Z, dbias, bmode, precise):
+    """dZ (one or two matrices, from offset 0 on dC's grid; precise: behind them
+    what their rounding leaves over) and the bias gradient: local sums in 32 (64) bits, one all-reduce over the process row
     (column), one rounding."""
     W = dC if dC.storage.bc.mb == dC.storage.bc.nb and _placed(dC, dC) else None
     if W is None:
@@ -772,7 +811,8 @@ def _dz_dist(act, dC, Z, dbias, bmode):
         redistribute_pieces(dC, W)
     Zw = [None if z is None else _onto(z, W) for z in Z]
     two = Zw[1] is not None
-    dZ = [_grid_work(W, dC.m(), dC.n()) for _ in range(2 if two else 1)] if act or two else [W]
+    made = 2 if two else 1
+    dZ = [_grid_work(W, dC.m(), dC.n()) for _ in range(2 * made if precise else made)] if act or two else [W]
     lb, s = W.local_block(), W.storage
     db, sums = _NONE, None
     if dbias is not None:
@@ -783,7 +823,8 @@ def _dz_dist(act, dC, Z, dbias, bmode):
         oz = [_NONE if z is None else _opd(z) for z in Zw]
         od = [_opd(d) for d in dZ] if act or two else [_NONE]
         with _on(lb.data):
-            _act_grad(lb.mloc, lb.nloc, act, _opd(W), oz[0], oz[1], od[0], od[1] if two else _NONE, db, bmode, True)
+            _act_grad(lb.mloc, lb.nloc, act, _opd(W), oz[0], oz[1], od[0], od[1] if two else _NONE, db, bmode, True,
+                      (*od[made:], _NONE, _NONE)[:2])
     if act or two:
         _modified(*dZ)
     if dbias is not None:

@@ -1198,3 +1198,82 @@ def test_copy_half_kinds(dev, src, dst):
             tri = torch.ones(45, 45).tril().bool()
             tri = tri if uplo == sl.Uplo.Lower else tri.t()
             assert torch.equal(y.cpu(), torch.where(tri, x.cpu().to(dst), keep.cpu()))
+
+
+def precise_grads(dt, dev, m, n, k, ta="T", tb="N", act="gelu", pad=0, off=0, gated=False, opts={"PreciseGradient": True},
+                  which=("A1", "A2", "B")):
+    """Gradients with what the rounding of dZ leaves over, and [(got, wanted, bound)].
+
+    Two parts of 16 bits hold dZ to u^2 of itself and half the smallest step; the
+    products' sums have twice the terms."""
+    u, w = u_of(dt), w_of(dt)
+    g = Gated(dt, dev, m, n, k, ta, tb, act, pad, off)
+    a1, a2, b = g.dense()
+    z1, z2, c = g.Z1.double(), g.Z2.double(), g.G.double()
+    v, s = act64(act, z1)
+    left = (u * u if u > w else 0) + 4 * w
+    d = {x: cm(*getattr(g, x).shape, dt, 9, dev) if x in which else None for x in ("A1", "A2", "B")}
+    t = {"A1": ta == "T", "A2": ta == "T", "B": tb == "T"}
+    out = [None if d[x] is None else mat(d[x], t[x]) for x in ("A1", "A2", "B")]
+    A1, A2, B = g.handles()
+    bt, a1t, a2t = b.t().contiguous(), a1.t().contiguous(), a2.t().contiguous()
+    one = c * z2 if gated else c
+    dz1, f1 = one * s, 32 * w * (1 + z1.abs()) * one.abs() + left * (one * s).abs() + tiny(dt)
+    terms = [("A1", dz1 @ bt, f1 @ bt.abs() + 2 * (n + 4) * w * (dz1.abs() @ bt.abs()))]
+    bsum, bbound = a1t @ dz1, a1t.abs() @ f1 + 4 * (m + 4) * w * (a1t.abs() @ dz1.abs())
+    if gated:
+        sl.gemm_gated_grad(A1, A2, B, act, mat(g.Z1), mat(g.Z2), mat(g.G), *out, opts)
+        dz2, f2 = c * v, 32 * w * (1 + z1.abs()) * (c * z1).abs() + left * (c * v).abs() + tiny(dt)
+        terms.append(("A2", dz2 @ bt, f2 @ bt.abs() + 2 * (n + 4) * w * (dz2.abs() @ bt.abs())))
+        bsum, bbound = bsum + a2t @ dz2, bbound + a2t.abs() @ f2 + 4 * (m + 4) * w * (a2t.abs() @ dz2.abs())
+    else:
+        sl.gemm_bias_act_grad(1.0, A1, B, act, mat(g.Z1), mat(g.G), out[0], out[2], None, opts)
+    terms.append(("B", bsum, bbound))
+    return [(d[x].t() if t[x] else d[x], want, e + tiny(dt) + u * (want.abs() + e)) for x, want, e in terms if x in which]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("ta,tb", ["TN", "NN", "NT", "TT"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_precise_gradient(dev, dt, ta, tb, gated):
+    for m, n, k, act, pad, off in ((70, 33, 50, "gelu", 0, 0), (48, 1, 40, "silu", 8, 0), (131, 67, 75, "gelu_tanh", 3, 1),
+                                   (1, 1, 1, "relu", 0, 0)):
+        for which in (("A1", "A2", "B"), ("B",), ("A1", "B")):
+            for got, want, e in precise_grads(dt, dev, m, n, k, ta, tb, act, pad, off, gated, which=which):
+                within(got, want, e)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k,pad", [(1024, 2048, 512, 0), (4000, 3, 640, 0), (600, 5000, 128, 0), (2051, 2049, 2053, 1),
+                                       (328, 264, 200, 0), (2560, 515, 1024, 0)])
+def test_precise_gradient_sizes(dt, gated, m, n, k, pad):
+    """K in pieces that begin in any of two or four products, short last steps, operands laid out anew."""
+    first = precise_grads(dt, "cuda", m, n, k, pad=pad, gated=gated)
+    for got, want, e in first:
+        within(got, want, e)
+    for (x, _, _), (y, _, _) in zip(first, precise_grads(dt, "cuda", m, n, k, pad=pad, gated=gated)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dt", HALF)
+def test_precise_gradient_choice(dev, dt):
+    """The option lowers the error of dA and dB, changes nothing of 32 bits, and keeps infinities."""
+    err = {}
+    for on in (False, True):
+        got = precise_grads(dt, dev, 96, 64, 80, opts={sl.Option.PreciseGradient: on}, gated=True)
+        err[on] = [float((x.double() - w).norm() / w.norm()) for x, w, _ in got]
+    # one rounding of random relative size against two of the same: by 2^0.5, a tenth less for chance
+    assert all(a > 1.27 * b for a, b in zip(err[False], err[True])), err
+    a, b = (precise_grads(torch.float32, dev, 40, 24, 32, opts=o) for o in (None, {"PreciseGradient": True}))
+    assert all(torch.equal(x[0], y[0]) for x, y in zip(a, b))
+    one = torch.ones(1, 1, dtype=dt, device=dev)
+    big = torch.full((1, 1), torch.finfo(dt).max, dtype=dt, device=dev)
+    for z2, g, want in ((big, big, float("inf")), (big, one, float(big)), (one * float("nan"), one, float("nan"))):
+        d = torch.empty(1, 1, dtype=dt, device=dev)
+        sl.gemm_gated_grad(mat(one), mat(one), mat(one), "identity", mat(one), mat(z2), mat(g), mat(d), None, None,
+                           {"PreciseGradient": True})
+        assert float(d) == want or want != want and d.isnan().all()

@@ -263,3 +263,35 @@ def _one_of(rank, size):
 
 def test_one_of_two():
     run_dist(_one_of, 2)
+
+
+def _precise(rank, size, p, q, dt):
+    m, n, k = 37, 29, 43
+    u, w = u_of(dt), w_of(dt)
+    a, a2, b, z1, z2, g = (rnd(*s, dt, i) for i, s in enumerate(((m, k), (m, k), (k, n), (m, n), (m, n), (m, n))))
+    A, A2, B, Z1, Z2, G = (spread(x, 8, p, q) for x in (a, a2, b, z1, z2, g))
+    dA, dA2, dB, db = (spread(0 * x, 8, p, q) for x in (a, a, b, a[:, :1]))
+    opts = {"PreciseGradient": True}
+    a, a2, b, z1, z2, g = (x.double() for x in (a, a2, b, z1, z2, g))
+    for gated in (False, True):
+        v, s = act64("silu", z1)
+        c = g * z2 if gated else g
+        dz = [c * s] + [g * v] * gated
+        f = [(u * u + 4 * w) * x.abs() + 32 * w * (1 + z1.abs()) * y.abs() for x, y in zip(dz, (c, g * z1))]
+        if gated:
+            sl.gemm_gated_grad(A, A2, B, "silu", Z1, Z2, G, dA, dA2, dB, opts)
+        else:
+            sl.gemm_bias_act_grad(1.0, A, B, "silu", Z1, G, dA, dB, db, opts)
+            within(D(db), dz[0].sum(1, keepdim=True), (f[0] + 64 * w * dz[0].abs()).sum(1, keepdim=True) +
+                   1.1 * u * dz[0].sum(1, keepdim=True).abs())
+        for got, x, y in zip((dA, dA2), dz, f):
+            want, e = x @ b.t(), (y + 2 * (n + 4) * w * x.abs()) @ b.abs().t()
+            within(D(got), want, e + u * (want.abs() + e))
+        want = sum(i.t() @ x for i, x in zip((a, a2), dz))
+        e = sum(i.abs().t() @ (y + 4 * (m + 4) * w * x.abs()) for i, x, y in zip((a, a2), dz, f))
+        within(D(dB), want, e + u * (want.abs() + e))
+
+
+@pytest.mark.parametrize("p,q", [(2, 1), (2, 2)])
+def test_precise_gradient(p, q):
+    run_dist(_precise, p * q, p, q, torch.bfloat16)
