@@ -851,17 +851,17 @@ def _clip_views(mats, what):
     add, anew = out.append, debug_checks()
     for M in mats:
         s = M.storage
-        slot = s.origin_slot
-        if not M._whole or s.bc is None:
-            raise SlateError(f"{what}: general block-cyclic matrices are wanted")
+        slot, table = s.origin_slot, s.table
         x = M.__dict__.get("_operand")
         # (the use of a remembered operand, as in _opd, without the call)
-        now = s.table.version()
-        if anew or x is None or x.table is not s.table or x.version != now or x.t.data_ptr() != x.ptr:
+        now = table.version()
+        if not M._whole or x is None or x.version != now or x.table is not table or x.t.data_ptr() != x.ptr or anew:
+            if not M._whole or s.bc is None:
+                raise SlateError(f"{what}: general block-cyclic matrices are wanted")
             if slot is None:
                 raise SlateError(f"{what}: a matrix has no tiles (insertLocalTiles)")
             x = _opd(M)
-            now = s.table.version()
+            now = table.version()
         if dt is None:
             dt, dev, comm = x.dt, x.dev, s.comm
         elif x.dt is not dt or x.dev is not dev:
