@@ -460,9 +460,9 @@ template <typename T, int BM, int BN, int WVM, int WVN, int S> struct GaEpi {
 // elsewhere: four times the instructions, still asynchronous (1503 x 777 x 1001
 // f32: 38 us against 53 us through registers).  0: every slab goes through
 // registers, two slabs ahead of its products.
-// Two workgroups a CU at least: with one, the compiler keeps the sums in vector
-// registers between steps and copies them to accumulation registers and back in
-// each (f64 4096^3 2230 us against 2010).
+// Two waves a SIMD at least (one workgroup of 512 threads a CU, two of 256): with
+// one, the compiler keeps the sums in vector registers between steps and copies
+// them to accumulation registers and back in each (f64 4096^3 2230 us against 2010).
 template <typename T, bool AKC, bool BKC, int BM, int BN, int WVM, int WVN, int S, bool GATED, int DMA>
 __global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs a) {
     using TR = ga_traits<T>;
@@ -806,9 +806,11 @@ __global__ void __launch_bounds__(64 * WVM * WVN, 2) gemm_act_kernel(GemmActArgs
 // interleaved slabs of 128 bytes per row, fragments straight from memory to
 // registers with 2 U of them in flight per wave and operand (no LDS, no
 // barrier in the loop); the waves' sums are added in LDS in their order.
-// One column: 4096 x 4096 bf16 8.6 us (3.9 TB/s), two f16 matrices of 8192 x
-// 4096 29 us (4.6 TB/s).  Columns that lie across 16 bytes cost 2.5 times as
-// much (bf16 5120 x 11772: 138 us, 44 aligned).
+// One column: 4096 x 4096 bf16 9.1 us (3.7 TB/s), f64 27 us (5.0 TB/s), two f16
+// matrices of 8192 x 4096 29 us (4.6 TB/s).  Columns of 16-bit elements that lie
+// across 4 bytes take twice the time (bf16 5120 x 11771 65 us, 11776 32; two f16 of
+// 8192 x 4096 57), columns across 16 bytes alone a tenth more (11772: 35; f32
+// 4096 x 4095 17.3, 4096 15.5).
 template <typename T, bool GATED, int NW>
 __global__ void __launch_bounds__(64 * NW) gemm_act_skinny_kernel(GemmActArgs a) {
     using TR = ga_traits<T>;
