@@ -1277,3 +1277,37 @@ def test_precise_gradient_choice(dev, dt):
         sl.gemm_gated_grad(mat(one), mat(one), mat(one), "identity", mat(one), mat(z2), mat(g), mat(d), None, None,
                            {"PreciseGradient": True})
         assert float(d) == want or want != want and d.isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+def test_precise_gradient_graph(gated):
+    """The option's backward pass captured and replayed, with eager work between."""
+    s, _ = block(torch.bfloat16, "cuda", 77, 256, 520)
+    H = {n: mat(v, n in ("wg", "wu", "dwg", "dwu")) for n, v in s.items()}
+    for n in ("z1", "z2", "dh"):
+        s[n].copy_(cm(*s[n].shape, torch.bfloat16, 30 + len(n), "cuda"))
+    names = ("dwg", "dwu", "dx") if gated else ("dwg", "dx")
+    opts = {"PreciseGradient": True}
+
+    def step():
+        if gated:
+            sl.gemm_gated_grad(H["wg"], H["wu"], H["x"], "silu", H["z1"], H["z2"], H["dh"], H["dwg"], H["dwu"], H["dx"], opts)
+        else:
+            sl.gemm_bias_act_grad(1.0, H["wg"], H["x"], "silu", H["z1"], H["dh"], H["dwg"], H["dx"], None, opts)
+
+    step()
+    want = {n: s[n].clone() for n in names}
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for _ in range(3):
+        for n in names:
+            s[n].fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        for n in names:
+            assert torch.equal(s[n], want[n]), n
+        step()
+        torch.cuda.synchronize()
