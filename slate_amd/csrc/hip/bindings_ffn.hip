@@ -54,8 +54,10 @@ int bytes_of(char t) { return t == 'd' ? 8 : t == 's' ? 4 : 2; }
 // -> its size; without one nothing is launched.
 template <typename T> i64 ffn_grad(double alpha, const std::vector<i64>& v, char* ws, hipStream_t s) {
     constexpr size_t HEAD = 15;
-    const size_t T_ = v.size() < HEAD ? 0 : (size_t)v[14], PER = 10 + 4 * T_;
-    if (T_ < 2 || T_ > 4 || (v.size() - HEAD) % PER) throw std::invalid_argument("ffn_grad: 15 + (10 + 4 T) n integers are wanted");
+    const int nt = v.size() < HEAD ? 0 : (int)v[14];
+    const size_t PER = 10 + 4 * nt;
+    if (nt < 2 || nt > 4 || (v.size() - HEAD) % PER)
+        throw std::invalid_argument("ffn_grad: 15 + (10 + 4 T) n integers are wanted, T 2 to 4");
     auto round = [](i64 x, i64 to) { return (x + to - 1) / to * to; };
     ActGradArgs g;
     g.m = v[0]; g.n = v[1]; g.act = (int)v[2];
@@ -92,7 +94,6 @@ template <typename T> i64 ffn_grad(double alpha, const std::vector<i64>& v, char
             ld = g.lddz;
             return base + (-1 - x[j]) * dz;
         };
-        const int nt = (int)T_;
         for (int j = 0; j < nt; ++j) {
             a.A[j] = at(6 + 2 * j, a.lda[j]);
             a.B[j] = at(6 + 2 * nt + 2 * j, a.ldb[j]);

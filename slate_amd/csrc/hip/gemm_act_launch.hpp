@@ -106,7 +106,8 @@ i64 gemm_act(GemmActArgs a, char ta, char tb, hipStream_t s) {
     if (a.m <= 0 || a.n <= 0) return 0;
     if (a.mode != GA_SUM) a.terms = 1;
     const bool gated = a.mode == GA_GATED, akc = ta != 'N', bkc = tb == 'N';
-    const int na = a.mode == GA_SUM ? a.terms : a.mode == GA_PLAIN ? 1 : 2, nb = a.mode == GA_SUM ? a.terms : a.mode == GA_PAIR ? 2 : 1;
+    const int na = a.mode == GA_SUM ? a.terms : a.mode == GA_PLAIN ? 1 : 2;
+    const int nb = a.mode == GA_SUM ? a.terms : a.mode == GA_PAIR ? 2 : 1;
     // LDS-DMA moves 16 bytes from 16-byte-aligned addresses at 32-bit offsets
     // inside a tile; a slab whose last vector would pass the end of the last
     // column goes through registers, as the ragged end of K does
